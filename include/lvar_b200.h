@@ -284,6 +284,106 @@ int lvar_qkv_prologue(const void* qkv, int64_t s_b, int64_t s_l, int64_t s_w, in
                       void* v_cache, int64_t v_sb, int64_t v_sh, int64_t v_sl, int32_t cache_pos, int32_t B, int32_t L,
                       int32_t H, int32_t c, lvar_stream_t stream);
 
+/* A key/value cache in pages, for sequences of different length.  k, v: [num_pages, Hkv, page_size, D] with the given
+ * strides in elements (innermost 1, 16-byte aligned rows), bf16, or e4m3 when `scales` is set: uint8
+ * [num_pages, Hkv, page_size, 2] (innermost two contiguous; page and head strides multiples of 4), for every row of K ([0])
+ * and V ([1]) the biased exponent x of the power of two 2^(x - 127) that its e4m3 values are multiplied by.
+ * table: int32 [B, max_pages] (rows t_sb apart): position j of sequence b lies in page table[b, j / page_size], row
+ * j mod page_size.  Entries behind a sequence's end are not read (any value may stand there); several sequences may share
+ * a page that none of them writes.  page_size: a multiple of 16 up to 512; D in {64, 128}. */
+typedef struct lvar_paged_cache {
+  void* k;
+  int64_t k_sp, k_sh, k_sl;
+  void* v;
+  int64_t v_sp, v_sh, v_sl;
+  uint8_t* scales; /* null: bf16 cache */
+  int64_t s_sp, s_sh;
+  const int32_t* table;
+  int64_t t_sb;
+  int32_t num_pages, page_size, Hkv, D, B, max_pages;
+} lvar_paged_cache;
+
+/* Arguments of lvar_paged_write. Zero-initialise, then fill. */
+typedef struct lvar_paged_write_args {
+  lvar_paged_cache cache;
+  /* new tokens: bf16, element (b, l, h, e) at b*sb + l*sl + h*sh + e (strides multiples of 8, 16-byte aligned); q may be
+     null with Hq = 0: rows are only appended */
+  const void* q;
+  int64_t q_sb, q_sl, q_sh;
+  const void* k;
+  int64_t k_sb, k_sl, k_sh;
+  const void* v;
+  int64_t v_sb, v_sl, v_sh;
+  void* q_out; /* bf16 [B, Hq, L, D] */
+  int64_t qo_sb, qo_sh, qo_sl;
+  const int32_t* start; /* [B]: token l of sequence b goes to position start[b] + l */
+  const int32_t* count; /* [B] or null (all L): tokens l >= count[b] are padding: not written, q_out 0 */
+  /* norm 1: x / max(|x|, 1e-12), q times scale_mul[h] (fp32 [Hq]); norm 2: x * rsqrt(mean x^2 + eps) * weight (fp32 [D],
+     null: 1); norm 0: none.  q and k only. */
+  const float* scale_mul;
+  const float* q_weight;
+  const float* k_weight;
+  /* rotation by table row = position: fp32 [rope_rows, D/2], 16-byte aligned; null: none.  Element pairs (2i, 2i+1), or
+     (i, i + D/2) with rope_halves. */
+  const float* rope_cos;
+  const float* rope_sin;
+  int32_t* dev_status; /* optional; LVAR_DEV_BAD_INDEX: a position without a page (not written) or without a table row */
+  float eps;
+  int32_t norm, rope_halves, rope_rows, L, Hq;
+} lvar_paged_write_args;
+
+/* Arguments of lvar_paged_read. */
+typedef struct lvar_paged_read_args {
+  lvar_paged_cache cache;
+  void* k; /* bf16 [B, Hkv, n, D], element strides, multiples of 8 */
+  int64_t k_sb, k_sh, k_sl;
+  void* v;
+  int64_t v_sb, v_sh, v_sl;
+  const int32_t* lens; /* [B] */
+  int32_t* dev_status; /* optional; LVAR_DEV_BAD_INDEX: a row below lens[b] without a page (zeros are written) */
+  int32_t start, n;
+} lvar_paged_read_args;
+
+/* Arguments of lvar_paged_attn. */
+typedef struct lvar_paged_attn_args {
+  lvar_paged_cache cache;
+  const void* q; /* bf16 [B, Hq, T, D]; Hq a multiple of the cache's heads, query head h reads key head h / (Hq / Hkv) */
+  int64_t q_sb, q_sh, q_sl;
+  void* o; /* bf16 [B, Hq, T, D] */
+  int64_t o_sb, o_sh, o_sl;
+  float* M; /* optional row statistics, fp32 [B, Hq, T] contiguous, as in lvar_attn_args (a row that sees no key: -inf, 0) */
+  float* L;
+  const int32_t* lens; /* [B], device: keys of each sequence, the T new ones included; 0: an empty slot, o = 0 */
+  void* workspace;     /* lvar_paged_attn_workspace bytes, 16-byte aligned, owned by this call until it completes */
+  int64_t workspace_bytes;
+  int32_t* dev_status; /* optional; LVAR_DEV_BAD_INDEX: a length above max_len (cut there) or a page number outside the
+                          cache (its rows count as zeros) */
+  float scale;
+  int32_t Hq, T;
+  int32_t causal;  /* token t sees keys j <= len - T + t (else every key) */
+  int32_t max_len; /* no length exceeds it (it shapes the launch); at most 2^30 */
+} lvar_paged_attn_args;
+
+/* Writes new tokens' K and V rows into the pages, as they are or after the fused prologue of a self-attention layer (norm
+ * and rotation of q and k; all arithmetic fp32, rounded once).  e4m3 cache: row scale 2^e with the least e for which
+ * max |x| 2^-e <= 448, -100 <= e <= 120; elements that are not finite become NaN.  Two tokens must not share a place.
+ * The paged form of lvar_qkv_prologue (models/sparvar/basic_sparvar.py:321-350), with grouped heads, norm weights and
+ * half-split rotation. */
+int lvar_paged_write(const lvar_paged_write_args* args, lvar_stream_t stream);
+
+/* Rows start .. start + n - 1 of every sequence out of the pages as bf16 (an e4m3 times a power of two is exact), zeros for
+ * rows >= lens[b]: K and V for the attention entry points above, which take contiguous caches. */
+int lvar_paged_read(const lvar_paged_read_args* args, lvar_stream_t stream);
+
+/* Attention of T new tokens per sequence over the paged cache, o = softmax(scale q K^T + mask) V, split over the cache's
+ * length and joined; lengths are read on the device (capturable while they change).  Few tokens: bound by reading the
+ * cache once.  Fixed summation order for given lengths (bit-reproducible).  The generation-time counterpart of
+ * lvar_dense_attn at the call sites of models/sparvar/basic_sparvar.py:371-387 for the first scales. */
+int lvar_paged_attn(const lvar_paged_attn_args* args, lvar_stream_t stream);
+
+/* Bytes of workspace that lvar_paged_attn needs on the current device for these sizes (0: none), or a negative code. */
+int64_t lvar_paged_attn_workspace(int32_t B, int32_t Hq, int32_t Hkv, int32_t T, int32_t D, int32_t e4m3, int32_t max_len);
+
 /* Bilinear (align_corners = false) resize of an attention-output cache between two square token grids:
  * src bf16 [BH, src_side^2, D] -> dst bf16 [BH, dst_side^2, D] (strides in elements, D a multiple of 8).
  * Replaces upsample_Ocache(o, L_src, L_tgt, mode='2d', upsample_mode='bilinear')

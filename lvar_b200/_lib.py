@@ -61,6 +61,55 @@ class AttnArgs(C.Structure):
     ]
 
 
+class PagedCache(C.Structure):
+    """Mirror of ``lvar_paged_cache``; field order and types must match the header (as below)."""
+
+    _fields_ = [
+        ("k", C.c_void_p), ("k_sp", C.c_int64), ("k_sh", C.c_int64), ("k_sl", C.c_int64),
+        ("v", C.c_void_p), ("v_sp", C.c_int64), ("v_sh", C.c_int64), ("v_sl", C.c_int64),
+        ("scales", C.c_void_p), ("s_sp", C.c_int64), ("s_sh", C.c_int64),
+        ("table", C.c_void_p), ("t_sb", C.c_int64),
+        ("num_pages", C.c_int32), ("page_size", C.c_int32), ("Hkv", C.c_int32), ("D", C.c_int32), ("B", C.c_int32),
+        ("max_pages", C.c_int32),
+    ]
+
+
+class PagedWriteArgs(C.Structure):
+    _fields_ = [
+        ("cache", PagedCache),
+        ("q", C.c_void_p), ("q_sb", C.c_int64), ("q_sl", C.c_int64), ("q_sh", C.c_int64),
+        ("k", C.c_void_p), ("k_sb", C.c_int64), ("k_sl", C.c_int64), ("k_sh", C.c_int64),
+        ("v", C.c_void_p), ("v_sb", C.c_int64), ("v_sl", C.c_int64), ("v_sh", C.c_int64),
+        ("q_out", C.c_void_p), ("qo_sb", C.c_int64), ("qo_sh", C.c_int64), ("qo_sl", C.c_int64),
+        ("start", C.c_void_p), ("count", C.c_void_p),
+        ("scale_mul", C.c_void_p), ("q_weight", C.c_void_p), ("k_weight", C.c_void_p),
+        ("rope_cos", C.c_void_p), ("rope_sin", C.c_void_p), ("dev_status", C.c_void_p),
+        ("eps", C.c_float),
+        ("norm", C.c_int32), ("rope_halves", C.c_int32), ("rope_rows", C.c_int32), ("L", C.c_int32), ("Hq", C.c_int32),
+    ]
+
+
+class PagedReadArgs(C.Structure):
+    _fields_ = [
+        ("cache", PagedCache),
+        ("k", C.c_void_p), ("k_sb", C.c_int64), ("k_sh", C.c_int64), ("k_sl", C.c_int64),
+        ("v", C.c_void_p), ("v_sb", C.c_int64), ("v_sh", C.c_int64), ("v_sl", C.c_int64),
+        ("lens", C.c_void_p), ("dev_status", C.c_void_p),
+        ("start", C.c_int32), ("n", C.c_int32),
+    ]
+
+
+class PagedAttnArgs(C.Structure):
+    _fields_ = [
+        ("cache", PagedCache),
+        ("q", C.c_void_p), ("q_sb", C.c_int64), ("q_sh", C.c_int64), ("q_sl", C.c_int64),
+        ("o", C.c_void_p), ("o_sb", C.c_int64), ("o_sh", C.c_int64), ("o_sl", C.c_int64),
+        ("M", C.c_void_p), ("L", C.c_void_p), ("lens", C.c_void_p),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64), ("dev_status", C.c_void_p),
+        ("scale", C.c_float), ("Hq", C.c_int32), ("T", C.c_int32), ("causal", C.c_int32), ("max_len", C.c_int32),
+    ]
+
+
 # name -> (restype, argtypes); every symbol the header declares is listed here and checked at load.
 _SIGNATURES = {
     "lvar_dense_attn": (C.c_int, [C.POINTER(AttnArgs), C.c_void_p]),
@@ -94,6 +143,10 @@ _SIGNATURES = {
                           [C.c_int32] * 5 + [C.c_void_p]),
     "lvar_upsample_ocache": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int64, C.c_int32, C.c_int32, C.c_int32] +
                              [C.c_int64] * 4 + [C.c_void_p]),
+    "lvar_paged_write": (C.c_int, [C.POINTER(PagedWriteArgs), C.c_void_p]),
+    "lvar_paged_read": (C.c_int, [C.POINTER(PagedReadArgs), C.c_void_p]),
+    "lvar_paged_attn": (C.c_int, [C.POINTER(PagedAttnArgs), C.c_void_p]),
+    "lvar_paged_attn_workspace": (C.c_int64, [C.c_int32] * 7),
     "lvar_last_error": (C.c_char_p, []),
     "lvar_version": (C.c_char_p, []),
     "lvar_kernel_config_attn": (None, [C.POINTER(C.c_int32)] * 3),

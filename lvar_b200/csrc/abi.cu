@@ -116,6 +116,10 @@ int launch_qkv_prologue(const void* qkv, int64_t s_b, int64_t s_l, int64_t s_w, 
 int launch_upsample_ocache(const void* src, void* dst, int64_t BH, int src_side, int dst_side, int D,
                            int64_t src_bh_stride, int64_t src_row_stride, int64_t dst_bh_stride,
                            int64_t dst_row_stride, cudaStream_t stream);
+int launch_paged_write(const lvar_paged_write_args* a, cudaStream_t stream);
+int launch_paged_read(const lvar_paged_read_args* a, cudaStream_t stream);
+int launch_paged_attn(const lvar_paged_attn_args* a, cudaStream_t stream);
+int64_t paged_attn_workspace(int B, int Hq, int Hkv, int T, int D, int q8, int max_len);
 
 }  // namespace lvar
 
@@ -162,6 +166,22 @@ int lvar_upsample_ocache(const void* src, void* dst, int64_t BH, int32_t src_sid
                          int64_t dst_row_stride, lvar_stream_t stream) {
   return lvar::launch_upsample_ocache(src, dst, BH, src_side, dst_side, D, src_bh_stride, src_row_stride,
                                       dst_bh_stride, dst_row_stride, static_cast<cudaStream_t>(stream));
+}
+
+int lvar_paged_write(const lvar_paged_write_args* args, lvar_stream_t stream) {
+  return lvar::launch_paged_write(args, static_cast<cudaStream_t>(stream));
+}
+
+int lvar_paged_read(const lvar_paged_read_args* args, lvar_stream_t stream) {
+  return lvar::launch_paged_read(args, static_cast<cudaStream_t>(stream));
+}
+
+int lvar_paged_attn(const lvar_paged_attn_args* args, lvar_stream_t stream) {
+  return lvar::launch_paged_attn(args, static_cast<cudaStream_t>(stream));
+}
+
+int64_t lvar_paged_attn_workspace(int32_t B, int32_t Hq, int32_t Hkv, int32_t T, int32_t D, int32_t e4m3, int32_t max_len) {
+  return lvar::paged_attn_workspace(B, Hq, Hkv, T, D, e4m3, max_len);
 }
 
 int lvar_dense_attn(const lvar_attn_args* args, lvar_stream_t stream) {

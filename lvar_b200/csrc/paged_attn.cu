@@ -1,0 +1,910 @@
+// Attention of a few new tokens per sequence over the paged key/value cache:
+//   o[b,h,t,:] = sum_j softmax_j(scale q[b,h,t].K[b,h/G,j]) V[b,h/G,j,:],  j < len_b  (causal: j <= len_b - T + t).
+//
+// Bound by reading the cache (4 D bytes per cached row in bf16, 2 D + 2 in e4m3; 4 D flops per row and query row): the
+// G = Hq / Hkv query heads of a key head and the T tokens are the rows of one tile, so that a cached row crosses HBM
+// once for all of them.  A tile of 16 rows is what one warp-level matrix instruction takes (m16n8k16); the tensor-memory
+// instructions start at 64 rows, of which one to sixteen would be used, and their accumulators would have to come back
+// through tensor memory for the running softmax of every 64 keys.  16 rows per warp leave the matrix pipe several times
+// ahead of HBM (16 flops per byte against the 250 that the chip's ratio allows), so it is not what bounds the kernel.
+//
+// A CTA of four warps streams tiles of keys through a ring in shared memory (cp.async, 16 bytes, XOR-swizzled rows; rows
+// behind the sequence's end are zero-filled, so that nothing that lies in a page behind it is ever read).  With up to 16
+// rows the four warps take a quarter of a tile's keys each and have a running maximum, sum and accumulator of their own,
+// joined once at the end of the piece; with more rows (up to 64 per CTA) two or four warps share the keys and differ in
+// their rows.
+//
+// Split over the cache's length: all tiles of all (sequence, key head, row tile) items form one line that the CTAs (two
+// per SM) share evenly, whatever the lengths are: they are read on the device.  An item that falls to several CTAs leaves
+// at most two pieces per CTA in the workspace (unnormalised sums, maximum, sum), and a second kernel joins them in a
+// fixed order.  Where no item has more than a few tiles a CTA takes one item and there is no second kernel.
+//
+// e4m3 cache: K and V rows are widened to fp16 (exact), q is scaled by a power of two per row into fp16's range (exact but
+// for elements 2^-24 below the row's largest).  K's row scale multiplies the score.  V's row scale 2^e joins the exponent
+// of the weight, w = exp2(s + e - running maximum of (s + e)), so that the fp16 weights are always taken relative to the
+// largest CONTRIBUTION; the row sum keeps a maximum of its own.
+// Weights are rounded once, to bf16 (bf16 cache) or fp16 scaled by 2^15 (e4m3 cache); sums, maxima and accumulators are
+// fp32.
+#include <math.h>
+
+#include "paged.cuh"
+#include "ptx.cuh"
+
+namespace lvar {
+
+namespace {
+
+constexpr int kThreads = 128;
+constexpr int kSlotsPerCta = 2;
+
+struct PagedAttnParams {
+  PagedView c;
+  const int32_t* lens;
+  const __nv_bfloat16* q;
+  int64_t q_sb, q_sh, q_sl;
+  __nv_bfloat16* o;
+  int64_t o_sb, o_sh, o_sl;
+  float* M;  // [B, Hq, T] or null
+  float* L;
+  float* part;  // workspace of the split form
+  int32_t* status;
+  int B, Hkv, G, T, R;  // R = T * G rows per (sequence, key head)
+  int RT;               // row tiles
+  int causal, max_len;
+  int split;            // 0: CTA x takes item x
+  float scale_log2;
+};
+
+__device__ __forceinline__ void cp_async_16_zfill(uint32_t dst, const void* src, bool ok) {
+  const int n = ok ? 16 : 0;
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ void cp_async_4_zfill(uint32_t dst, const void* src, bool ok) {
+  const int n = ok ? 4 : 0;
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+}
+__device__ __forceinline__ void ldsm_x4_t(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+}
+__device__ __forceinline__ uint4 lds128(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
+  return v;
+}
+__device__ __forceinline__ uint2 lds64(uint32_t addr) {
+  uint2 v;
+  asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr));
+  return v;
+}
+__device__ __forceinline__ uint32_t lds32(uint32_t addr) {
+  uint32_t v;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr));
+  return v;
+}
+__device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// Two e4m3 bytes to two fp16 (exact); the low byte goes to the low half.
+__device__ __forceinline__ uint32_t widen2(uint32_t two) {
+  uint32_t r;
+  asm("{\n.reg .b16 t;\ncvt.u16.u32 t, %1;\ncvt.rn.f16x2.e4m3x2 %0, t;\n}" : "=r"(r) : "r"(two));
+  return r;
+}
+__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ float pow2i(int e) { return __int_as_float((e + 127) << 23); }  // -126 <= e <= 127
+
+template <int D, bool Q8>
+struct Geo {
+  static constexpr int RB = D * (Q8 ? 1 : 2);             // bytes of a cached row
+  static constexpr int KT = Q8 || D == 64 ? 128 : 64;     // keys per tile
+  static constexpr int CPR = RB / 16;                     // 16-byte chunks per row
+  static constexpr int RP = kThreads / CPR;               // rows per pass of the loaders
+  static constexpr int CPT = KT / RP;                     // passes
+  static constexpr int GROUP = RP < 16 ? 16 : RP;         // rows whose page is looked up at a time by one thread
+  static constexpr int PPG = GROUP / RP;
+  static constexpr int STAGE = 2 * KT * RB;               // K and V
+  static constexpr int STAGES = STAGE <= 16384 ? 6 : 3;
+  static constexpr int SCALE_STAGE = Q8 ? KT * 2 : 0;
+  static constexpr int RING = STAGES * (STAGE + SCALE_STAGE);
+  static constexpr int ML = 4 * 16 * 2 * 4;               // maxima and sums of the four warps' rows
+  static constexpr int SMEM = RING + ML + 64;
+  static_assert(4 * 16 * D * 4 <= STAGE, "the warps' accumulators are joined in a consumed stage");
+};
+
+// Byte offset of a 16-byte chunk inside a K or V tile.
+template <int RB>
+__device__ __forceinline__ uint32_t chunk_at(int row, int chunk) {
+  const int x = RB == 64 ? (row >> 1) & 3 : row & 7;
+  return (uint32_t)(row * RB + ((chunk ^ x) << 4));
+}
+
+struct Cursor {
+  int b, hr, tile, ntile, len;
+};
+
+// Length of a sequence as the kernel uses it: inside the caller's bound and the table's.
+__device__ __forceinline__ int length_of(const PagedAttnParams& p, int b) {
+  const int n = p.lens[b];
+  if (n > p.max_len && p.status) atomicCAS(p.status, 0, (int)DEV_BAD_INDEX);
+  return min(max(n, 0), p.max_len);
+}
+template <int KT>
+__device__ __forceinline__ int tiles_of(int len) {
+  return max(1, (len + KT - 1) / KT);
+}
+
+// The line of all tiles, shared by the CTAs: prefix sums over the sequences, one pass by the whole CTA.
+struct Line {
+  int64_t total;
+  int nc;  // CTAs that have tiles
+};
+
+template <int KT>
+__device__ __forceinline__ Line line_scan(const PagedAttnParams& p, int ctas, int64_t* sm, int64_t& excl, int& b0, int& b1) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int per = (p.B + kThreads - 1) / kThreads;
+  b0 = min(tid * per, p.B);
+  b1 = min(b0 + per, p.B);
+  const int HR = p.Hkv * p.RT;
+  int64_t mine = 0;
+  for (int b = b0; b < b1; ++b) mine += (int64_t)tiles_of<KT>(length_of(p, b)) * HR;
+  int64_t inc = mine;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const int64_t x = __shfl_up_sync(0xffffffffu, inc, d);
+    if (lane >= d) inc += x;
+  }
+  if (lane == 31) sm[warp] = inc;
+  __syncthreads();
+  int64_t before = 0, total = 0;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    if (w < warp) before += sm[w];
+    total += sm[w];
+  }
+  excl = before + inc - mine;
+  Line l;
+  l.total = total;
+  l.nc = (int)(total < ctas ? total : ctas);
+  return l;
+}
+__device__ __forceinline__ int64_t range_start(const Line& l, int c) { return l.total * c / l.nc; }
+
+// The item and tile at place x of the line, and the place of the item's first tile; by the whole CTA.
+template <int KT>
+__device__ __forceinline__ Cursor line_locate(const PagedAttnParams& p, int64_t x, int64_t excl, int b0, int b1, int64_t* sm,
+                                              int64_t& item_start) {
+  const int HR = p.Hkv * p.RT;
+  int64_t at = excl;
+  __syncthreads();
+  for (int b = b0; b < b1; ++b) {
+    const int len = length_of(p, b), n = tiles_of<KT>(len);
+    const int64_t end = at + (int64_t)n * HR;
+    if (x >= at && x < end) {
+      sm[0] = b;
+      sm[1] = at;
+      sm[2] = len;
+    }
+    at = end;
+  }
+  __syncthreads();
+  Cursor c;
+  c.b = (int)sm[0];
+  c.len = (int)sm[2];
+  c.ntile = tiles_of<KT>(c.len);
+  const int64_t in = x - sm[1];
+  c.hr = (int)(in / c.ntile);
+  c.tile = (int)(in - (int64_t)c.hr * c.ntile);
+  item_start = sm[1] + (int64_t)c.hr * c.ntile;
+  return c;
+}
+template <int KT>
+__device__ __forceinline__ void advance(const PagedAttnParams& p, Cursor& c) {
+  if (++c.tile < c.ntile) return;
+  c.tile = 0;
+  if (++c.hr < p.Hkv * p.RT) return;
+  c.hr = 0;
+  if (++c.b < p.B) {
+    c.len = length_of(p, c.b);
+    c.ntile = tiles_of<KT>(c.len);
+  }
+}
+
+template <int D, bool Q8>
+__device__ __forceinline__ void load_tile(const PagedAttnParams& p, const Cursor& cur, uint32_t ring, int stage) {
+  using X = Geo<D, Q8>;
+  const int tid = threadIdx.x;
+  const int chunk = tid % X::CPR, r0 = tid / X::CPR;
+  const int key0 = cur.tile * X::KT;
+  const int h = cur.hr / p.RT;
+  const int32_t* trow = p.c.table + cur.b * p.c.t_sb;
+  const uint8_t* kb = p.c.k + h * p.c.k_sh + chunk * 16;
+  const uint8_t* vb = p.c.v + h * p.c.v_sh + chunk * 16;
+  const uint32_t ks = ring + stage * X::STAGE, vs = ks + X::KT * X::RB;
+  int page[X::CPT / X::PPG];
+  uint32_t in[X::CPT / X::PPG];
+#pragma unroll
+  for (int g = 0; g < X::CPT / X::PPG; ++g) {
+    const int pos = key0 + g * X::GROUP + r0;
+    const uint32_t grp = (uint32_t)pos >> 4, pg = page_of_group(p.c, grp);
+    in[g] = (grp - pg * p.c.groups) * 16 + (pos & 15);
+    page[g] = pos < cur.len ? __ldg(trow + pg) : 0;
+  }
+#pragma unroll
+  for (int g = 0; g < X::CPT / X::PPG; ++g) {
+    if ((uint32_t)page[g] >= (uint32_t)p.c.num_pages && p.status) atomicCAS(p.status, 0, (int)DEV_BAD_INDEX);
+    const bool good = (uint32_t)page[g] < (uint32_t)p.c.num_pages;
+    const int64_t pg = good ? page[g] : 0;
+#pragma unroll
+    for (int j = 0; j < X::PPG; ++j) {
+      const int row = g * X::GROUP + j * X::RP + r0;
+      const bool ok = good && key0 + row < cur.len;
+      const int64_t r = in[g] + j * X::RP;
+      cp_async_16_zfill(ks + chunk_at<X::RB>(row, chunk), kb + pg * p.c.k_sp + r * p.c.k_sl, ok);
+      cp_async_16_zfill(vs + chunk_at<X::RB>(row, chunk), vb + pg * p.c.v_sp + r * p.c.v_sl, ok);
+    }
+  }
+  if constexpr (Q8) {
+    if (tid < X::KT / 2) {  // two rows' exponents
+      const int pos = key0 + tid * 2;
+      const uint32_t grp = (uint32_t)pos >> 4, pg = page_of_group(p.c, grp);
+      const uint32_t r = (grp - pg * p.c.groups) * 16 + (pos & 15);
+      const int page1 = pos < cur.len ? __ldg(trow + pg) : -1;
+      const bool ok = (uint32_t)page1 < (uint32_t)p.c.num_pages;
+      cp_async_4_zfill(ring + X::STAGES * X::STAGE + stage * X::SCALE_STAGE + tid * 4,
+                       p.c.scales + (ok ? page1 : 0) * p.c.s_sp + h * p.c.s_sh + r * 2, ok);
+    }
+  }
+}
+
+// One warp's running state over an item: two rows per thread (lane / 4 and + 8).
+template <int D>
+struct State {
+  float acc[D / 8][4];
+  float m[2], l[2];  // maximum of the scores (log2 units) and sum of exp2(s - m), per thread
+  float mt[2];       // e4m3: maximum of score + V exponent, which the accumulators are relative to
+};
+
+template <int D, bool Q8, int WR>
+__global__ void __launch_bounds__(kThreads, 2) paged_attn_kernel(const __grid_constant__ PagedAttnParams p) {
+  using X = Geo<D, Q8>;
+  constexpr int WK = 4 / WR;              // warps that share a row tile and differ in their keys
+  constexpr int KW = X::KT / WK;          // keys of a tile per warp
+  constexpr int NS = KW < 32 ? KW : 32;   // keys per step
+  constexpr int NT = NS / 8;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  const uint32_t ring = smem_u32(smem);
+  float* ml = reinterpret_cast<float*>(smem + X::RING);
+  int64_t* scan = reinterpret_cast<int64_t*>(smem + X::RING + X::ML);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int wr = warp % WR, wk = warp / WR, quad = lane & 3;
+
+  griddep_wait();
+  Cursor cons;
+  int nt;
+  bool whole_first = true;  // whether the CTA's first piece begins at its item's start
+  if (p.split) {
+    griddep_launch_dependents();
+    int64_t excl, item_start;
+    int b0, b1;
+    const Line line = line_scan<X::KT>(p, (int)gridDim.x, scan, excl, b0, b1);
+    const int c = blockIdx.x;
+    if (c >= line.nc) return;
+    const int64_t start = range_start(line, c);
+    nt = (int)(range_start(line, c + 1) - start);
+    cons = line_locate<X::KT>(p, start, excl, b0, b1, scan, item_start);
+    whole_first = item_start == start;
+  } else {
+    const int HR = p.Hkv * p.RT;
+    cons.b = blockIdx.x / HR;
+    cons.hr = blockIdx.x - cons.b * HR;
+    cons.tile = 0;
+    cons.len = length_of(p, cons.b);
+    cons.ntile = nt = tiles_of<X::KT>(cons.len);
+  }
+
+  Cursor prod = cons;
+#pragma unroll
+  for (int i = 0; i < X::STAGES - 1; ++i) {
+    if (i < nt) {
+      load_tile<D, Q8>(p, prod, ring, i);
+      advance<X::KT>(p, prod);
+    }
+    cp_async_commit();
+  }
+
+  State<D> st;
+  uint32_t qf[D / 16][4];
+  float qs[2];      // factor from the raw product to log2 units, per row
+  int limit[2];     // keys that the row sees
+  int see_all = 0;  // keys that every row of the item sees
+  bool first_piece = true, fresh = true;
+
+  for (int i = 0; i < nt; ++i) {
+    const int stage = i % X::STAGES;
+    cp_async_wait<X::STAGES - 2>();
+    __syncthreads();
+    if (i + X::STAGES - 1 < nt) {
+      load_tile<D, Q8>(p, prod, ring, (i + X::STAGES - 1) % X::STAGES);
+      advance<X::KT>(p, prod);
+    }
+    cp_async_commit();
+
+    const int rt = cons.hr % p.RT, h = cons.hr / p.RT;
+    if (fresh) {
+      fresh = false;
+#pragma unroll
+      for (int n = 0; n < D / 8; ++n) st.acc[n][0] = st.acc[n][1] = st.acc[n][2] = st.acc[n][3] = 0.f;
+      see_all = p.causal ? cons.len - p.T + 1 : cons.len;
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        st.m[x] = st.mt[x] = -INFINITY;
+        st.l[x] = 0.f;
+        const int r = rt * 16 * WR + wr * 16 + (lane >> 2) + x * 8;
+        const bool live = r < p.R;
+        const int t = live ? r / p.G : 0, g = live ? r - t * p.G : 0;
+        limit[x] = !live ? 0 : p.causal ? cons.len - p.T + t + 1 : cons.len;
+        const __nv_bfloat16* src = p.q + cons.b * p.q_sb + (int64_t)(h * p.G + g) * p.q_sh + t * p.q_sl;
+        qs[x] = p.scale_log2;
+        if constexpr (!Q8) {
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk) {
+            qf[kk][x] = live ? *reinterpret_cast<const uint32_t*>(src + kk * 16 + quad * 2) : 0u;
+            qf[kk][x + 2] = live ? *reinterpret_cast<const uint32_t*>(src + kk * 16 + quad * 2 + 8) : 0u;
+          }
+        } else {
+          // matrix step 4 i + s takes elements 16 (2 quad + i) + 4 s + {0..3} (D = 64: 16 quad + 4 s) from this thread
+          constexpr int CH = D / 64;
+          uint2 raw[D / 16];
+          float most = 0.f;
+          bool fine = true;
+#pragma unroll
+          for (int ch = 0; ch < CH; ++ch) {
+#pragma unroll
+            for (int s = 0; s < 4; ++s) {
+              const int e = 16 * (CH * quad + ch) + 4 * s;
+              raw[ch * 4 + s] = live ? *reinterpret_cast<const uint2*>(src + e) : make_uint2(0u, 0u);
+            }
+          }
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk) {
+            const uint32_t w[2] = {raw[kk].x, raw[kk].y};
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              const float a = fabsf(__uint_as_float(w[j] << 16)), b = fabsf(__uint_as_float(w[j] & 0xffff0000u));
+              fine = fine && a < INFINITY && b < INFINITY;
+              most = fmaxf(most, fmaxf(a, b));
+            }
+          }
+          most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
+          most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
+          const int e = min(max((int)(__float_as_uint(most) >> 23) - 127, -126), 126);
+          const unsigned fines = __ballot_sync(0xffffffffu, fine) >> (lane & 28);
+          const int sh = (fines & 15u) == 15u && most > 0.f ? e : 0;
+          const float down = pow2i(-sh);
+          qs[x] = p.scale_log2 * pow2i(sh);
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk) {
+            qf[kk][x] = pack_f16x2(__uint_as_float(raw[kk].x << 16) * down, __uint_as_float(raw[kk].x & 0xffff0000u) * down);
+            qf[kk][x + 2] = pack_f16x2(__uint_as_float(raw[kk].y << 16) * down, __uint_as_float(raw[kk].y & 0xffff0000u) * down);
+          }
+        }
+      }
+    }
+
+    const bool idle = rt * 16 * WR + wr * 16 >= p.R;  // none of the warp's rows exists
+    const uint32_t ks = ring + stage * X::STAGE, vs = ks + X::KT * X::RB;
+    const uint32_t ss = ring + X::STAGES * X::STAGE + stage * X::SCALE_STAGE;
+#pragma unroll 1
+    for (int s0 = wk * KW; s0 < (wk + 1) * KW; s0 += NS) {
+      const int key0 = cons.tile * X::KT + s0;
+      if (key0 >= cons.len || idle) break;  // the same for the whole warp
+      // scores
+      float sc[NT][4];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.f;
+      if constexpr (!Q8) {
+#pragma unroll
+        for (int n2 = 0; n2 < NT / 2; ++n2) {
+          const int row = s0 + n2 * 16 + (lane & 7) + ((lane >> 4) << 3);
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk) {
+            uint32_t b[4];
+            ldsm_x4(ks + chunk_at<X::RB>(row, kk * 2 + ((lane >> 3) & 1)), b);
+            mma_bf16(sc[n2 * 2], qf[kk], b[0], b[1]);
+            mma_bf16(sc[n2 * 2 + 1], qf[kk], b[2], b[3]);
+          }
+        }
+      } else {
+        constexpr int CH = D / 64;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          const int row = s0 + n * 8 + (lane >> 2);
+#pragma unroll
+          for (int ch = 0; ch < CH; ++ch) {
+            const uint4 w = lds128(ks + chunk_at<X::RB>(row, CH * quad + ch));
+            const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+            for (int s = 0; s < 4; ++s) mma_f16(sc[n], qf[ch * 4 + s], widen2(u[s]), widen2(u[s] >> 16));
+          }
+        }
+      }
+      // to log2 units; e4m3: with the rows' scales
+      uint32_t ex[NT];  // e4m3: biased exponents (K, V) of the thread's two keys
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        if constexpr (Q8) {
+          ex[n] = lds32(ss + (s0 + n * 8 + quad * 2) * 2);
+          const float k0 = __uint_as_float((ex[n] & 0xffu) << 23), k1 = __uint_as_float((ex[n] & 0xff0000u) << 7);
+          sc[n][0] *= k0 * qs[0];
+          sc[n][1] *= k1 * qs[0];
+          sc[n][2] *= k0 * qs[1];
+          sc[n][3] *= k1 * qs[1];
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sc[n][e] *= qs[0];
+        }
+      }
+      const bool edge = key0 + NS > see_all;  // some row does not see some of these keys
+      if (edge) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (key0 + n * 8 + quad * 2 + (e & 1) >= limit[e >> 1]) sc[n][e] = -INFINITY;
+      }
+      // running maximum and sum; weights
+      float alpha[2];
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        float mx = st.m[x], tx = st.mt[x];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          mx = fmaxf(mx, fmaxf(sc[n][2 * x], sc[n][2 * x + 1]));
+          if constexpr (Q8) {
+            const float e0 = (float)((int)((ex[n] >> 8) & 0xffu) - 127), e1 = (float)((int)(ex[n] >> 24) - 127);
+            tx = fmaxf(tx, fmaxf(sc[n][2 * x] + e0, sc[n][2 * x + 1] + e1));
+          }
+        }
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        const float mu = mx == -INFINITY ? 0.f : mx;
+        float add = 0.f;
+        if constexpr (Q8) {
+          tx = fmaxf(tx, __shfl_xor_sync(0xffffffffu, tx, 1));
+          tx = fmaxf(tx, __shfl_xor_sync(0xffffffffu, tx, 2));
+          const float tu = tx == -INFINITY ? 0.f : tx - 15.f;  // weights up to 2^15
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            const float e0 = (float)((int)((ex[n] >> 8) & 0xffu) - 127), e1 = (float)((int)(ex[n] >> 24) - 127);
+            const float s0v = sc[n][2 * x], s1v = sc[n][2 * x + 1];
+            add += fast_exp2(s0v - mu) + fast_exp2(s1v - mu);
+            sc[n][2 * x] = fast_exp2(s0v + e0 - tu);
+            sc[n][2 * x + 1] = fast_exp2(s1v + e1 - tu);
+          }
+          alpha[x] = fast_exp2(st.mt[x] - (tx == -INFINITY ? 0.f : tx));
+          st.l[x] = st.l[x] * fast_exp2(st.m[x] - mu) + add;
+          st.mt[x] = tx;
+        } else {
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            sc[n][2 * x] = fast_exp2(sc[n][2 * x] - mu);
+            sc[n][2 * x + 1] = fast_exp2(sc[n][2 * x + 1] - mu);
+            add += sc[n][2 * x] + sc[n][2 * x + 1];
+          }
+          alpha[x] = fast_exp2(st.m[x] - mu);
+          st.l[x] = st.l[x] * alpha[x] + add;
+        }
+        st.m[x] = mx;
+      }
+      if (__any_sync(0xffffffffu, !(alpha[0] == 1.f && alpha[1] == 1.f))) {
+#pragma unroll
+        for (int n = 0; n < D / 8; ++n) {
+          st.acc[n][0] *= alpha[0];
+          st.acc[n][1] *= alpha[0];
+          st.acc[n][2] *= alpha[1];
+          st.acc[n][3] *= alpha[1];
+        }
+      }
+      // O += P V, 16 keys at a time.  In a step that some row does not see all of, elements of V that are not finite are
+      // left out here and come in row by row below: a weight of zero would make NaN of them in rows that do not see them.
+      bool odd = false;
+#pragma unroll
+      for (int n2 = 0; n2 < NT / 2; ++n2) {
+        if constexpr (!Q8) {
+          const uint32_t a[4] = {pack_bf16x2(sc[2 * n2][0], sc[2 * n2][1]), pack_bf16x2(sc[2 * n2][2], sc[2 * n2][3]),
+                                 pack_bf16x2(sc[2 * n2 + 1][0], sc[2 * n2 + 1][1]),
+                                 pack_bf16x2(sc[2 * n2 + 1][2], sc[2 * n2 + 1][3])};
+          const int row = s0 + n2 * 16 + (lane & 15);
+#pragma unroll
+          for (int d2 = 0; d2 < D / 16; ++d2) {
+            uint32_t b[4];
+            ldsm_x4_t(vs + chunk_at<X::RB>(row, d2 * 2 + (lane >> 4)), b);
+            if (edge) {
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                if ((b[j] & 0x7f80u) == 0x7f80u) b[j] &= 0xffff0000u, odd = true;
+                if ((b[j] & 0x7f800000u) == 0x7f800000u) b[j] &= 0xffffu, odd = true;
+              }
+            }
+            mma_bf16(st.acc[d2 * 2], a, b[0], b[1]);
+            mma_bf16(st.acc[d2 * 2 + 1], a, b[2], b[3]);
+          }
+        } else {
+          const uint32_t a[4] = {pack_f16x2(sc[2 * n2][0], sc[2 * n2][1]), pack_f16x2(sc[2 * n2][2], sc[2 * n2][3]),
+                                 pack_f16x2(sc[2 * n2 + 1][0], sc[2 * n2 + 1][1]),
+                                 pack_f16x2(sc[2 * n2 + 1][2], sc[2 * n2 + 1][3])};
+          const int row = s0 + n2 * 16 + quad * 2;
+          constexpr int W = D / 32;  // words per thread and key: D / 8 consecutive elements, lane / 4 says which
+          uint32_t u[4][W];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int r = row + (j & 1) + (j >> 1) * 8;
+            if constexpr (D == 128) {
+              const uint4 w = lds128(vs + chunk_at<X::RB>(r, lane >> 2));
+              u[j][0] = w.x, u[j][1] = w.y, u[j][2] = w.z, u[j][3] = w.w;
+            } else {
+              const uint2 w = lds64(vs + chunk_at<X::RB>(r, lane >> 3) + ((lane >> 2) & 1) * 8);
+              u[j][0] = w.x, u[j][1] = w.y;
+            }
+            if (edge) {
+#pragma unroll
+              for (int i4 = 0; i4 < W; ++i4)
+#pragma unroll
+                for (int y = 0; y < 4; ++y)
+                  if (((u[j][i4] >> (8 * y)) & 0x7fu) == 0x7fu) u[j][i4] &= ~(0xffu << (8 * y)), odd = true;
+            }
+          }
+#pragma unroll
+          for (int i4 = 0; i4 < W; ++i4) {
+            const uint32_t lo0 = __byte_perm(u[0][i4], u[1][i4], 0x5140), hi0 = __byte_perm(u[0][i4], u[1][i4], 0x7362);
+            const uint32_t lo1 = __byte_perm(u[2][i4], u[3][i4], 0x5140), hi1 = __byte_perm(u[2][i4], u[3][i4], 0x7362);
+            mma_f16(st.acc[i4 * 4], a, widen2(lo0), widen2(lo1));
+            mma_f16(st.acc[i4 * 4 + 1], a, widen2(lo0 >> 16), widen2(lo1 >> 16));
+            mma_f16(st.acc[i4 * 4 + 2], a, widen2(hi0), widen2(hi1));
+            mma_f16(st.acc[i4 * 4 + 3], a, widen2(hi0 >> 16), widen2(hi1 >> 16));
+          }
+        }
+      }
+      if (edge && __any_sync(0xffffffffu, odd)) {
+#pragma unroll 1
+        for (int j = 0; j < NS; ++j) {
+          float w0 = 0.f, w1 = 0.f;  // this row pair's weights of key j, from the lane of the quad that holds them
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            float x0 = sc[n][0], x1 = sc[n][1], x2 = sc[n][2], x3 = sc[n][3];
+            asm volatile("" : "+f"(x0), "+f"(x1), "+f"(x2), "+f"(x3));  // a choice of registers, not of array elements
+            if (n == j >> 3) {
+              w0 = (j & 1) ? x1 : x0;
+              w1 = (j & 1) ? x3 : x2;
+            }
+          }
+          w0 = __shfl_sync(0xffffffffu, w0, (lane & 28) | ((j & 7) >> 1));
+          w1 = __shfl_sync(0xffffffffu, w1, (lane & 28) | ((j & 7) >> 1));
+#pragma unroll
+          for (int n = 0; n < D / 8; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              float val;
+              bool finite;
+              if constexpr (!Q8) {
+                const int d = n * 8 + quad * 2 + e;
+                const uint32_t at = vs + chunk_at<X::RB>(s0 + j, d >> 3) + (d & 7) * 2;
+                const uint32_t word = lds32(at & ~3u);
+                val = __uint_as_float((d & 1) ? word & 0xffff0000u : word << 16);
+                finite = fabsf(val) < INFINITY;
+              } else {
+                const int d = (quad * 2 + e) * (D / 8) + n;
+                const uint32_t at = vs + chunk_at<X::RB>(s0 + j, d >> 4) + (d & 15);
+                finite = ((lds32(at & ~3u) >> ((at & 3u) * 8)) & 0x7fu) != 0x7fu;
+                val = NAN;
+              }
+              if (!finite) {
+                if (key0 + j < limit[0]) st.acc[n][e] = fmaf(w0, val, st.acc[n][e]);
+                if (key0 + j < limit[1]) st.acc[n][e + 2] = fmaf(w1, val, st.acc[n][e + 2]);
+              }
+            }
+        }
+      }
+    }
+
+    const bool last = cons.tile == cons.ntile - 1;
+    if (last || i == nt - 1) {
+      // Join of the warps that share rows, in the stage just consumed.
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        st.l[x] += __shfl_xor_sync(0xffffffffu, st.l[x], 1);
+        st.l[x] += __shfl_xor_sync(0xffffffffu, st.l[x], 2);
+        if (quad == 0) {
+          ml[(warp * 16 + (lane >> 2) + x * 8) * 2] = st.m[x];
+          ml[(warp * 16 + (lane >> 2) + x * 8) * 2 + 1] = st.l[x];
+        }
+      }
+      __syncthreads();
+      float* buf = reinterpret_cast<float*>(smem + stage * X::STAGE);  // [warp][16][D]
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const int row = (lane >> 2) + x * 8;
+        float top = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < WK; ++w) top = fmaxf(top, ml[((w * WR + wr) * 16 + row) * 2]);
+        // an infinite maximum (an infinite score) gives NaN here, as exp(inf - inf) does
+        const float own = Q8 ? st.mt[x] - 15.f : st.m[x];
+        const float f = own == -INFINITY ? 0.f : exp2f(own - top);
+        float* dst = buf + (warp * 16 + row) * D;
+        if constexpr (!Q8) {
+#pragma unroll
+          for (int n = 0; n < D / 8; ++n)
+            *reinterpret_cast<float2*>(dst + n * 8 + quad * 2) = make_float2(st.acc[n][2 * x] * f, st.acc[n][2 * x + 1] * f);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+#pragma unroll
+            for (int n = 0; n < D / 8; n += 4)
+              *reinterpret_cast<float4*>(dst + (quad * 2 + e) * (D / 8) + n) =
+                  make_float4(st.acc[n][2 * x + e] * f, st.acc[n + 1][2 * x + e] * f, st.acc[n + 2][2 * x + e] * f,
+                              st.acc[n + 3][2 * x + e] * f);
+        }
+      }
+      __syncthreads();
+      const bool whole = last && (!first_piece || whole_first);
+      const int slot = first_piece ? 0 : 1;
+      constexpr int TPR = D / 8, RPP = kThreads / TPR;
+      const int e0 = (tid % TPR) * 8;
+      const int live = min(16 * WR, p.R - rt * 16 * WR);
+      for (int row = tid / TPR; row < live; row += RPP) {
+        const int w0 = row >> 4, r16 = row & 15;
+        float top = -INFINITY, sum = 0.f, v[8] = {};
+#pragma unroll
+        for (int w = 0; w < WK; ++w) top = fmaxf(top, ml[((w * WR + w0) * 16 + r16) * 2]);
+#pragma unroll
+        for (int w = 0; w < WK; ++w) {
+          const int at = (w * WR + w0) * 16 + r16;
+          const float mw = ml[at * 2];
+          sum += mw == -INFINITY ? 0.f : ml[at * 2 + 1] * exp2f(mw - top);
+          const float4 x = *reinterpret_cast<const float4*>(buf + at * D + e0);
+          const float4 y = *reinterpret_cast<const float4*>(buf + at * D + e0 + 4);
+          v[0] += x.x, v[1] += x.y, v[2] += x.z, v[3] += x.w;
+          v[4] += y.x, v[5] += y.y, v[6] += y.z, v[7] += y.w;
+        }
+        if (whole) {
+          const int r = rt * 16 * WR + row, t = r / p.G, head = h * p.G + r - t * p.G;
+          const float inv = top == -INFINITY ? 0.f : 1.f / sum;  // a row that sees no key gives 0
+          uint4 out;
+          out.x = pack_bf16x2(v[0] * inv, v[1] * inv);
+          out.y = pack_bf16x2(v[2] * inv, v[3] * inv);
+          out.z = pack_bf16x2(v[4] * inv, v[5] * inv);
+          out.w = pack_bf16x2(v[6] * inv, v[7] * inv);
+          *reinterpret_cast<uint4*>(p.o + cons.b * p.o_sb + head * p.o_sh + t * p.o_sl + e0) = out;
+          if (p.M && e0 == 0) {
+            const int64_t at = ((int64_t)cons.b * p.Hkv * p.G + head) * p.T + t;
+            p.M[at] = top;
+            p.L[at] = sum;
+          }
+        } else {
+          float* dst = p.part + ((int64_t)blockIdx.x * kSlotsPerCta + slot) * (16 * WR * (D + 2));
+          *reinterpret_cast<float4*>(dst + row * D + e0) = make_float4(v[0], v[1], v[2], v[3]);
+          *reinterpret_cast<float4*>(dst + row * D + e0 + 4) = make_float4(v[4], v[5], v[6], v[7]);
+          if (e0 == 0) *reinterpret_cast<float2*>(dst + 16 * WR * D + row * 2) = make_float2(top, sum);
+        }
+      }
+      first_piece = false;
+      fresh = true;
+    }
+    advance<X::KT>(p, cons);
+  }
+  cp_async_wait<0>();
+}
+
+// Joins the pieces of the item that begins in CTA x's range and goes on behind it: a warp per row, pieces in order.
+template <int D, bool Q8, int WR>
+__global__ void __launch_bounds__(kThreads) paged_join_kernel(const __grid_constant__ PagedAttnParams p, int ctas) {
+  using X = Geo<D, Q8>;
+  __shared__ int64_t scan[8];
+  const int c = blockIdx.x, lane = threadIdx.x & 31;
+  griddep_wait();
+  int64_t excl, item_start;
+  int b0, b1;
+  const Line line = line_scan<X::KT>(p, ctas, scan, excl, b0, b1);
+  if (c >= line.nc) return;
+  const int64_t start = range_start(line, c), end = range_start(line, c + 1);
+  const Cursor it = line_locate<X::KT>(p, end - 1, excl, b0, b1, scan, item_start);
+  const int64_t item_end = item_start + it.ntile;
+  if (item_start < start || item_end <= end) return;  // begins in another range, or ends in this one
+  // The last CTA of the item: the one whose range holds item_end - 1.
+  int last = (int)((item_end - 1) * line.nc / line.total);
+  while (range_start(line, last + 1) < item_end) ++last;
+  while (range_start(line, last) >= item_end) --last;
+  const int rt = it.hr % p.RT, h = it.hr / p.RT;
+  const int row = blockIdx.y * 4 + (threadIdx.x >> 5);
+  const int r = rt * 16 * WR + row;
+  if (row >= 16 * WR || r >= p.R) return;
+  const int64_t slot_floats = 16 * WR * (D + 2);
+  const int n = last - c + 1;
+  // piece 0 is slot 0 of this CTA if it is also its first piece, else slot 1; every later one is slot 0 of its CTA
+  const float* first = p.part + ((int64_t)c * kSlotsPerCta + (item_start == start ? 0 : 1)) * slot_floats;
+  const float* later = p.part + (int64_t)c * kSlotsPerCta * slot_floats;
+  float top = -INFINITY;
+  for (int i = lane; i < n; i += 32) {
+    const float* s = i == 0 ? first : later + (int64_t)i * kSlotsPerCta * slot_floats;
+    top = fmaxf(top, s[16 * WR * D + row * 2]);
+  }
+#pragma unroll
+  for (int d = 16; d >= 1; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+  constexpr int E = D / 32;
+  float acc[E] = {}, sum = 0.f;
+  for (int i0 = 0; i0 < n; i0 += 32) {
+    float f = 0.f, lsum = 0.f;
+    if (i0 + lane < n) {
+      const float* s = i0 + lane == 0 ? first : later + (int64_t)(i0 + lane) * kSlotsPerCta * slot_floats;
+      const float2 x = *reinterpret_cast<const float2*>(s + 16 * WR * D + row * 2);
+      f = x.x == -INFINITY ? 0.f : exp2f(x.x - top);
+      lsum = x.y * f;
+    }
+    const int m = min(32, n - i0);
+#pragma unroll 8
+    for (int i = 0; i < m; ++i) {
+      const float* s = i0 + i == 0 ? first : later + (int64_t)(i0 + i) * kSlotsPerCta * slot_floats;
+      const float g = __shfl_sync(0xffffffffu, f, i);
+      sum += __shfl_sync(0xffffffffu, lsum, i);
+      const float* src = s + row * D + lane * E;
+      if constexpr (E == 4) {
+        const float4 v = *reinterpret_cast<const float4*>(src);
+        acc[0] = fmaf(g, v.x, acc[0]);
+        acc[1] = fmaf(g, v.y, acc[1]);
+        acc[2] = fmaf(g, v.z, acc[2]);
+        acc[3] = fmaf(g, v.w, acc[3]);
+      } else {
+        const float2 v = *reinterpret_cast<const float2*>(src);
+        acc[0] = fmaf(g, v.x, acc[0]);
+        acc[1] = fmaf(g, v.y, acc[1]);
+      }
+    }
+  }
+  const float inv = top == -INFINITY ? 0.f : 1.f / sum;
+  const int t = r / p.G, head = h * p.G + r - t * p.G;
+  __nv_bfloat16* dst = p.o + it.b * p.o_sb + head * p.o_sh + t * p.o_sl + lane * E;
+  if constexpr (E == 4) {
+    *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16x2(acc[0] * inv, acc[1] * inv), pack_bf16x2(acc[2] * inv, acc[3] * inv));
+  } else {
+    *reinterpret_cast<uint32_t*>(dst) = pack_bf16x2(acc[0] * inv, acc[1] * inv);
+  }
+  if (p.M && lane == 0) {
+    const int64_t at = ((int64_t)it.b * p.Hkv * p.G + head) * p.T + t;
+    p.M[at] = top;
+    p.L[at] = sum;
+  }
+}
+
+// What a call launches: rows per CTA, whether items are split, the number of CTAs.
+struct Plan {
+  int wr, rt, split, ctas;
+  int64_t workspace;
+};
+
+int device_sms(int* sms) {
+  int dev = 0;
+  LVAR_CUDA_OK(cudaGetDevice(&dev));
+  LVAR_CUDA_OK(cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, dev));
+  return LVAR_OK;
+}
+
+int plan_of(int B, int Hq, int Hkv, int T, int D, bool q8, int max_len, int sms, Plan* out) {
+  const int64_t R = (int64_t)T * (Hq / Hkv);
+  out->wr = R <= 16 ? 1 : R <= 32 ? 2 : 4;
+  const int64_t rt = (R + 16 * out->wr - 1) / (16 * out->wr);
+  const int kt = q8 || D == 64 ? 128 : 64;
+  const int64_t tiles = max_len <= kt ? 1 : ((int64_t)max_len + kt - 1) / kt;
+  const int64_t items = B * (int64_t)Hkv * rt;
+  LVAR_REQUIRE(items < (1ll << 24), LVAR_ERR_LIMIT, "too many (sequence, key head, row tile) items");
+  out->rt = (int)rt;
+  out->split = tiles > 2;
+  out->ctas = out->split ? 2 * sms : (int)items;
+  out->workspace = out->split ? (int64_t)out->ctas * kSlotsPerCta * 16 * out->wr * (D + 2) * 4 : 0;
+  return LVAR_OK;
+}
+
+template <int D, bool Q8, int WR>
+int launch(const PagedAttnParams& p, const Plan& plan, cudaStream_t stream) {
+  using X = Geo<D, Q8>;
+  auto kern = paged_attn_kernel<D, Q8, WR>;
+  LVAR_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, X::SMEM));
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)plan.ctas);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = X::SMEM;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  LVAR_CUDA_OK(cudaLaunchKernelEx(&cfg, kern, p));
+  if (plan.split) {
+    const int rows = p.R < 16 * WR ? p.R : 16 * WR;
+    cfg.gridDim = dim3((unsigned)plan.ctas, (unsigned)((rows + 3) / 4));
+    cfg.dynamicSmemBytes = 0;
+    LVAR_CUDA_OK(cudaLaunchKernelEx(&cfg, paged_join_kernel<D, Q8, WR>, p, plan.ctas));
+  }
+  return LVAR_OK;
+}
+
+template <int D, bool Q8>
+int launch_wr(const PagedAttnParams& p, const Plan& plan, cudaStream_t stream) {
+  if (plan.wr == 1) return launch<D, Q8, 1>(p, plan, stream);
+  if (plan.wr == 2) return launch<D, Q8, 2>(p, plan, stream);
+  return launch<D, Q8, 4>(p, plan, stream);
+}
+
+}  // namespace
+
+int64_t paged_attn_workspace(int B, int Hq, int Hkv, int T, int D, int q8, int max_len) {
+  if (B < 1 || Hkv < 1 || Hq < Hkv || Hq % Hkv != 0 || T < 1 || max_len < 0 || max_len > 1 << 30 || (D != 64 && D != 128) ||
+      (int64_t)T * Hq >= (1ll << 31))
+    return fail(LVAR_ERR_ARG, "bad sizes");
+  int sms = 0;
+  if (int rc = device_sms(&sms)) return rc;
+  Plan plan;
+  if (int rc = plan_of(B, Hq, Hkv, T, D, q8 != 0, max_len, sms, &plan)) return rc;
+  return plan.workspace;
+}
+
+int launch_paged_attn(const lvar_paged_attn_args* a, cudaStream_t stream) {
+  LVAR_REQUIRE(a != nullptr, LVAR_ERR_ARG, "args must be non-null");
+  PagedAttnParams p{};
+  if (int rc = paged_view(&a->cache, &p.c)) return rc;
+  const lvar_paged_cache& c = a->cache;
+  LVAR_REQUIRE(a->q && a->o && a->lens, LVAR_ERR_ARG, "q, o and lens must be non-null");
+  LVAR_REQUIRE((a->M == nullptr) == (a->L == nullptr), LVAR_ERR_ARG, "M and L go together");
+  LVAR_REQUIRE(a->Hq >= 1 && a->T >= 1 && a->Hq % c.Hkv == 0, LVAR_ERR_ARG,
+               "query heads must be a multiple of the cache's heads (got %d and %d)", a->Hq, c.Hkv);
+  LVAR_REQUIRE((int64_t)a->T * a->Hq < (1ll << 31), LVAR_ERR_LIMIT, "too many query rows");
+  LVAR_REQUIRE(a->scale > 0.f && a->scale < INFINITY, LVAR_ERR_ARG, "scale must be positive and finite");
+  LVAR_REQUIRE(a->max_len >= 0 && a->max_len <= 1 << 30, LVAR_ERR_ARG, "max_len must lie in 0 .. 2^30");
+  const int64_t strides[] = {a->q_sb, a->q_sh, a->q_sl, a->o_sb, a->o_sh, a->o_sl};
+  for (int64_t s : strides)
+    LVAR_REQUIRE(s >= 0 && s % 8 == 0, LVAR_ERR_ARG, "strides of q and o must be non-negative multiples of 8 elements");
+  LVAR_REQUIRE(aligned16(a->q) && aligned16(a->o), LVAR_ERR_ARG, "q and o must be 16-byte aligned");
+  const int64_t room = (int64_t)c.max_pages * c.page_size;
+  const int max_len = (int)(a->max_len < room ? a->max_len : room);
+  int sms = 0;
+  if (int rc = device_sms(&sms)) return rc;
+  Plan plan;
+  if (int rc = plan_of(c.B, a->Hq, c.Hkv, a->T, c.D, c.scales != nullptr, a->max_len, sms, &plan)) return rc;
+  LVAR_REQUIRE(plan.workspace == 0 || (a->workspace && aligned16(a->workspace) && a->workspace_bytes >= plan.workspace),
+               LVAR_ERR_ARG, "workspace must be 16-byte aligned and hold %lld bytes (got %lld)", (long long)plan.workspace,
+               (long long)a->workspace_bytes);
+  p.lens = a->lens;
+  p.q = static_cast<const __nv_bfloat16*>(a->q);
+  p.q_sb = a->q_sb; p.q_sh = a->q_sh; p.q_sl = a->q_sl;
+  p.o = static_cast<__nv_bfloat16*>(a->o);
+  p.o_sb = a->o_sb; p.o_sh = a->o_sh; p.o_sl = a->o_sl;
+  p.M = a->M; p.L = a->L;
+  p.part = static_cast<float*>(a->workspace);
+  p.status = a->dev_status;
+  p.B = c.B; p.Hkv = c.Hkv; p.G = a->Hq / c.Hkv; p.T = a->T; p.R = a->T * p.G;
+  p.RT = plan.rt;
+  p.causal = a->causal != 0; p.max_len = max_len;
+  p.split = plan.split;
+  p.scale_log2 = a->scale * 1.4426950408889634f;
+  if (c.D == 128) return c.scales ? launch_wr<128, true>(p, plan, stream) : launch_wr<128, false>(p, plan, stream);
+  return c.scales ? launch_wr<64, true>(p, plan, stream) : launch_wr<64, false>(p, plan, stream);
+}
+
+}  // namespace lvar

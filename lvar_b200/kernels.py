@@ -12,7 +12,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib
-from ._lib import AttnArgs, check, lib
+from ._lib import AttnArgs, PagedAttnArgs, PagedCache, PagedReadArgs, PagedWriteArgs, check, lib
 
 
 _raw_stream = torch._C._cuda_getCurrentRawStream  # (device index) -> cudaStream_t of torch's current stream
@@ -671,3 +671,232 @@ def qkv_prologue(qkv: torch.Tensor, scale_mul: Optional[torch.Tensor], rope_cos:
                                 q.data_ptr(), H * L * c, L * c, c, k_cache.data_ptr(), k_sb, k_sh, k_sl,
                                 v_cache.data_ptr(), v_sb, v_sh, v_sl, int(cache_pos), B, L, H, c, _stream_ptr(dev)))
     return q
+
+
+# -- paged key/value cache -------------------------------------------------------------------------
+def _paged_cache(k_pages, v_pages, table, scales) -> PagedCache:
+    """Checks the tensors of a paged cache and describes them for the C side."""
+    want = torch.bfloat16 if scales is None else torch.float8_e4m3fn
+    dev = k_pages.device
+    if not k_pages.is_cuda:
+        raise RuntimeError("k_pages must be a CUDA tensor (lvar_b200 has no CPU path)")
+    if k_pages.dtype != want or v_pages.dtype != want:
+        raise RuntimeError(f"k_pages and v_pages must be bfloat16, or float8_e4m3fn together with scales; got "
+                           f"{k_pages.dtype}, {v_pages.dtype} and {'no ' if scales is None else ''}scales")
+    shape = k_pages.shape
+    if len(shape) != 4 or v_pages.shape != shape or v_pages.device != dev:
+        raise RuntimeError(f"k_pages and v_pages must be [pages, kv heads, page_size, D] on one device, got {tuple(shape)} "
+                           f"and {tuple(v_pages.shape)}")
+    k_sp, k_sh, k_sl, k_sd = k_pages.stride()
+    v_sp, v_sh, v_sl, v_sd = v_pages.stride()
+    if k_sd != 1 or v_sd != 1:
+        raise RuntimeError("k_pages and v_pages must have a contiguous last dimension")
+    n, H, size, D = shape
+    if table.dtype != torch.int32 or table.dim() != 2 or table.device != dev or (table.shape[1] > 1 and table.stride(1) != 1):
+        raise RuntimeError(f"table must be an int32 [B, pages per sequence] tensor on {dev} with a contiguous last dimension")
+    s_ptr, s_sp, s_sh = None, 0, 0
+    if scales is not None:
+        if scales.dtype != torch.uint8 or scales.shape != (n, H, size, 2) or scales.device != dev:
+            raise RuntimeError(f"scales must be a uint8 [{n}, {H}, {size}, 2] tensor on {dev}")
+        s_sp, s_sh, s_sl, s_sw = scales.stride()
+        if s_sl != 2 or s_sw != 1:
+            raise RuntimeError("scales must be contiguous in the last two dimensions")
+        s_ptr = scales.data_ptr()
+    return PagedCache(k_pages.data_ptr(), k_sp, k_sh, k_sl, v_pages.data_ptr(), v_sp, v_sh, v_sl, s_ptr, s_sp, s_sh,
+                      table.data_ptr(), table.stride(0), n, size, H, D, table.shape[0], table.shape[1])
+
+
+def _require_ints(name: str, t: torch.Tensor, B: int, device) -> int:
+    if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != B or t.device != device or (B > 1 and t.stride(0) != 1):
+        raise RuntimeError(f"{name} must be a contiguous int32 tensor of {B} entries on {device}")
+    return t.data_ptr()
+
+
+def _status_ptr(status: Optional[torch.Tensor], device) -> Optional[int]:
+    if status is None:
+        return None
+    if status.dtype != torch.int32 or status.device != device:
+        raise RuntimeError(f"status must be an int32 tensor on {device}")
+    return status.data_ptr()
+
+
+def _call(fn, args, device: torch.device) -> None:
+    """Launches on the current stream of the tensors' device, whichever device is current."""
+    if device.index == torch.cuda.current_device():
+        check(fn(C.byref(args), _raw_stream(device.index)))
+    else:
+        with torch.cuda.device(device):
+            check(fn(C.byref(args), _raw_stream(device.index)))
+
+
+def paged_kv_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor,
+                    start: torch.Tensor, *, scales: Optional[torch.Tensor] = None, count: Optional[torch.Tensor] = None,
+                    status: Optional[torch.Tensor] = None) -> None:
+    """Writes rows into a paged cache: row l of k, v (bf16 [B, H, L, D], any strides in multiples of 8) goes to position
+    ``start[b] + l`` of sequence b; rows l >= ``count[b]`` are padding and are left out.
+
+    The cache: ``k_pages``, ``v_pages`` [pages, H, page_size, D] (page_size a multiple of 16 up to 512, D 64 or 128),
+    bf16, or float8_e4m3fn with ``scales`` uint8 [pages, H, page_size, 2]: the biased exponents of every row's power of two,
+    K's and V's.  ``table`` int32 [B, n]: position p lies in page ``table[b, p // page_size]``.  ``start``, ``count``: int32
+    [B] on the device.  A position without a page is not written and sets ``status`` (see :func:`new_status`)."""
+    _require_cuda_bf16("k", k)
+    _require_cuda_bf16("v", v)
+    B, H, L, D = k.shape
+    c = _paged_cache(k_pages, v_pages, table, scales)
+    if v.shape != k.shape or (H, D, B) != (c.Hkv, c.D, c.B) or k.device != k_pages.device or v.device != k.device:
+        raise RuntimeError(f"k and v must be [{c.B}, {c.Hkv}, L, {c.D}] on {k_pages.device}, got {tuple(k.shape)} and {tuple(v.shape)}")
+    dev = k.device
+    start_ptr = _require_ints("start", start, B, dev)
+    count_ptr = None if count is None else _require_ints("count", count, B, dev)
+    if B == 0 or L == 0:
+        return
+    k_sb, k_sh, k_sl, _ = k.stride()
+    v_sb, v_sh, v_sl, _ = v.stride()
+    a = PagedWriteArgs(c, None, 0, 0, 0, k.data_ptr(), k_sb, k_sl, k_sh, v.data_ptr(), v_sb, v_sl, v_sh, None, 0, 0, 0,
+                       start_ptr, count_ptr, None, None, None, None, None, _status_ptr(status, dev), 0.0, 0, 0, 0, L, 0)
+    _call(lib.lvar_paged_write, a, dev)
+
+
+def paged_qkv_prologue(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
+                       table: torch.Tensor, start: torch.Tensor, *, scales: Optional[torch.Tensor] = None,
+                       scale_mul: Optional[torch.Tensor] = None, q_weight: Optional[torch.Tensor] = None,
+                       k_weight: Optional[torch.Tensor] = None, eps: Optional[float] = None,
+                       rope_cos: Optional[torch.Tensor] = None, rope_sin: Optional[torch.Tensor] = None,
+                       rope_halves: bool = False, count: Optional[torch.Tensor] = None,
+                       status: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Norms of queries and keys, position rotation and append to a paged cache in one pass; returns q bf16 [B, Hq, L, D].
+
+    q bf16 [B, L, Hq, D], k and v bf16 [B, L, Hkv, D]: views of one projection's output or separate tensors, Hq a multiple
+    of Hkv.  ``scale_mul`` fp32 [Hq]: x / max(|x|, 1e-12), q times scale_mul of its head (as :func:`qkv_prologue`).
+    ``eps`` (with optional ``q_weight``, ``k_weight`` fp32 [D]): x * rsqrt(mean x^2 + eps) * weight.  Neither: no norm.
+    ``rope_cos``, ``rope_sin`` fp32 [P, D/2]: row p rotates the token at cache position p, element pairs (2i, 2i + 1), or
+    (i, i + D/2) with ``rope_halves``.  The cache arguments, ``start``, ``count`` and ``status`` are those of
+    :func:`paged_kv_append`; q rows of padding are 0."""
+    for n, t in (("q", q), ("k", k), ("v", v)):
+        _require_cuda_bf16(n, t)
+    B, L, Hq, D = q.shape
+    c = _paged_cache(k_pages, v_pages, table, scales)
+    dev = q.device
+    if k.shape != v.shape or k.shape != (B, L, c.Hkv, D) or D != c.D or B != c.B or dev != k_pages.device or k.device != dev \
+            or v.device != dev:
+        raise RuntimeError(f"q must be [{c.B}, L, Hq, {c.D}] and k, v [{c.B}, L, {c.Hkv}, {c.D}] on {k_pages.device}, got "
+                           f"{tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
+    if Hq == 0 or Hq % c.Hkv:
+        raise RuntimeError(f"query heads must be a multiple of the cache's heads (got {Hq} and {c.Hkv})")
+    norm = 0
+    sm_ptr = qw_ptr = kw_ptr = cos_ptr = sin_ptr = None
+    if scale_mul is not None:
+        if eps is not None or q_weight is not None or k_weight is not None:
+            raise RuntimeError("scale_mul (L2 norm) excludes eps, q_weight and k_weight (root-mean-square norm)")
+        if scale_mul.dtype != torch.float32 or scale_mul.shape != (Hq,) or scale_mul.device != dev \
+                or not scale_mul.is_contiguous():
+            raise RuntimeError(f"scale_mul must be a contiguous float32 tensor of {Hq} entries on {dev}")
+        norm, sm_ptr = 1, scale_mul.data_ptr()
+    elif eps is not None:
+        norm = 2
+        for n, t in (("q_weight", q_weight), ("k_weight", k_weight)):
+            if t is not None and (t.dtype != torch.float32 or t.shape != (D,) or t.device != dev or not t.is_contiguous()):
+                raise RuntimeError(f"{n} must be a contiguous float32 tensor of {D} entries on {dev}")
+        qw_ptr = None if q_weight is None else q_weight.data_ptr()
+        kw_ptr = None if k_weight is None else k_weight.data_ptr()
+    elif q_weight is not None or k_weight is not None:
+        raise RuntimeError("q_weight and k_weight belong to the root-mean-square norm, which takes eps")
+    rope_rows = 0
+    if (rope_cos is None) != (rope_sin is None):
+        raise RuntimeError("rope_cos and rope_sin go together")
+    if rope_cos is not None:
+        for t in (rope_cos, rope_sin):
+            if t.dtype != torch.float32 or t.dim() != 2 or t.shape[1] != D // 2 or t.device != dev or not t.is_contiguous() \
+                    or t.shape[0] != rope_cos.shape[0]:
+                raise RuntimeError(f"rope tables must be contiguous float32 [P, {D // 2}] tensors on {dev}")
+        rope_rows, cos_ptr, sin_ptr = rope_cos.shape[0], rope_cos.data_ptr(), rope_sin.data_ptr()
+    start_ptr = _require_ints("start", start, B, dev)
+    count_ptr = None if count is None else _require_ints("count", count, B, dev)
+    out = torch.empty((B, Hq, L, D), dtype=torch.bfloat16, device=dev)
+    if B == 0 or L == 0:
+        return out
+    q_sb, q_sl, q_sh, _ = q.stride()
+    k_sb, k_sl, k_sh, _ = k.stride()
+    v_sb, v_sl, v_sh, _ = v.stride()
+    a = PagedWriteArgs(c, q.data_ptr(), q_sb, q_sl, q_sh, k.data_ptr(), k_sb, k_sl, k_sh, v.data_ptr(), v_sb, v_sl, v_sh,
+                       out.data_ptr(), Hq * L * D, L * D, D, start_ptr, count_ptr, sm_ptr, qw_ptr, kw_ptr, cos_ptr, sin_ptr,
+                       _status_ptr(status, dev), 0.0 if eps is None else float(eps), norm, int(rope_halves), rope_rows, L, Hq)
+    _call(lib.lvar_paged_write, a, dev)
+    return out
+
+
+def paged_kv_read(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor, lens: torch.Tensor, n: int, *,
+                  scales: Optional[torch.Tensor] = None, start: int = 0,
+                  out: Optional[Tuple[torch.Tensor, torch.Tensor]] = None,
+                  status: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Rows ``start`` .. ``start + n - 1`` of every sequence out of a paged cache as (K, V) bf16 [B, H, n, D], zeros for
+    rows at or behind ``lens[b]`` (int32 [B] on the device): the contiguous tensors that the many-query attention calls
+    take.  ``out``: an optional pair of destinations (bf16, unit stride along D, other strides in multiples of 8).  An e4m3
+    row comes back exactly as the values it stands for.  The cache arguments are those of :func:`paged_kv_append`."""
+    c = _paged_cache(k_pages, v_pages, table, scales)
+    dev = k_pages.device
+    shape = (c.B, c.Hkv, int(n), c.D)
+    if out is None:
+        out = (torch.empty(shape, dtype=torch.bfloat16, device=dev), torch.empty(shape, dtype=torch.bfloat16, device=dev))
+    else:
+        for name, t in zip(("k", "v"), out):
+            _require_cuda_bf16(name, t)
+            if t.shape != shape or t.device != dev:
+                raise RuntimeError(f"out must hold bfloat16 tensors of shape {shape} on {dev}, got {tuple(t.shape)}")
+    k, v = out
+    lens_ptr = _require_ints("lens", lens, c.B, dev)
+    if c.B == 0 or n == 0:
+        return k, v
+    k_sb, k_sh, k_sl, _ = k.stride()
+    v_sb, v_sh, v_sl, _ = v.stride()
+    a = PagedReadArgs(c, k.data_ptr(), k_sb, k_sh, k_sl, v.data_ptr(), v_sb, v_sh, v_sl, lens_ptr, _status_ptr(status, dev),
+                      int(start), int(n))
+    _call(lib.lvar_paged_read, a, dev)
+    return k, v
+
+
+def paged_attn_fwd(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor, lens: torch.Tensor,
+                   scale: Optional[float] = None, *, scales: Optional[torch.Tensor] = None, causal: bool = False,
+                   max_len: Optional[int] = None, return_stats: bool = False, out: Optional[torch.Tensor] = None,
+                   status: Optional[torch.Tensor] = None):
+    """Attention of the T newest tokens of every sequence over its paged cache: o = softmax(scale q K^T + mask) V, bf16
+    [B, Hq, T, D]; with ``return_stats`` (o, M, L), fp32 [B, Hq, T] as :func:`dense_attn_fwd` returns them.
+
+    q bf16 [B, Hq, T, D], Hq a multiple of the cache's heads (query head h reads key head h // (Hq // Hkv)); few tokens are
+    meant (a cached row is read once for up to 64 / (Hq // Hkv) of them): :func:`paged_kv_read` and the attention calls
+    above serve many.  ``lens`` int32 [B] on the device: the cached keys of each sequence, the new ones included; 0 marks
+    an empty slot.  ``causal``: token t sees the keys up to its own position, lens - T + t; else every token sees all keys.
+    A row that sees no key is 0 (M = -inf, L = 0).  ``max_len``: a bound on the lengths that shapes the launch (default: what
+    the table holds); a longer sequence is cut there and sets ``status``.  ``out``: see :func:`_output_like`.  The cache
+    arguments are those of :func:`paged_kv_append`."""
+    _require_cuda_bf16("q", q)
+    B, Hq, T, D = q.shape
+    c = _paged_cache(k_pages, v_pages, table, scales)
+    dev = q.device
+    if B != c.B or D != c.D or dev != k_pages.device:
+        raise RuntimeError(f"q must be [{c.B}, Hq, T, {c.D}] on {k_pages.device}, got {tuple(q.shape)}")
+    if Hq == 0 or Hq % c.Hkv:
+        raise RuntimeError(f"query heads must be a multiple of the cache's heads (got {Hq} and {c.Hkv})")
+    lens_ptr = _require_ints("lens", lens, B, dev)
+    room = c.max_pages * c.page_size
+    most = min(room, 1 << 30) if max_len is None else int(max_len)
+    o = _output_like(q, out)
+    M = L = None
+    m_ptr = l_ptr = None
+    if return_stats:
+        M = torch.empty((B, Hq, T), dtype=torch.float32, device=dev)
+        L = torch.empty((B, Hq, T), dtype=torch.float32, device=dev)
+        m_ptr, l_ptr = M.data_ptr(), L.data_ptr()
+    if B and T:
+        work, w_ptr = lib.lvar_paged_attn_workspace(B, Hq, c.Hkv, T, D, int(scales is not None), most), None
+        if work < 0:
+            check(int(work))
+        if work:
+            space = torch.empty(work, dtype=torch.uint8, device=dev)
+            w_ptr = space.data_ptr()
+        q_sb, q_sh, q_sl, _ = q.stride()
+        o_sb, o_sh, o_sl, _ = o.stride()
+        a = PagedAttnArgs(c, q.data_ptr(), q_sb, q_sh, q_sl, o.data_ptr(), o_sb, o_sh, o_sl, m_ptr, l_ptr, lens_ptr, w_ptr, work,
+                          _status_ptr(status, dev), float(D ** -0.5 if scale is None else scale), Hq, T, int(bool(causal)), most)
+        _call(lib.lvar_paged_attn, a, dev)
+    return (o, M, L) if return_stats else o
