@@ -106,6 +106,7 @@ class PagedAttnArgs(C.Structure):
         ("o", C.c_void_p), ("o_sb", C.c_int64), ("o_sh", C.c_int64), ("o_sl", C.c_int64),
         ("M", C.c_void_p), ("L", C.c_void_p), ("lens", C.c_void_p),
         ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64), ("dev_status", C.c_void_p),
+        ("wait_limit_ns", C.c_uint64),
         ("scale", C.c_float), ("Hq", C.c_int32), ("T", C.c_int32), ("causal", C.c_int32), ("max_len", C.c_int32),
     ]
 

@@ -76,6 +76,31 @@ int encode_rows_map(CUtensorMap* out, const void* base, int64_t rows, int64_t wi
   return LVAR_OK;
 }
 
+int encode_pages_map(CUtensorMap* out, const void* base, bool bytes, int pages, int H, int page_size, int D, int64_t sp,
+                     int64_t sh, int64_t sl, int box_rows) {
+  EncodeTiledFn fn = get_encode_fn();
+  LVAR_REQUIRE(fn != nullptr, LVAR_ERR_CUDA, "cuTensorMapEncodeTiled entry point not available (no CUDA driver?)");
+  const cuuint64_t elt = bytes ? 1 : 2, row_bytes = (cuuint64_t)D * elt;
+  cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)page_size, (cuuint64_t)H, (cuuint64_t)pages};
+  cuuint64_t st_l = (cuuint64_t)sl * elt, st_h = (cuuint64_t)sh * elt, st_p = (cuuint64_t)sp * elt;
+  // A stride of zero is not encodable; a dimension of one gets a harmless one.
+  if (H == 1 && st_h == 0) st_h = st_l;
+  if (pages == 1 && st_p == 0) st_p = st_l;
+  LVAR_REQUIRE(st_l >= row_bytes && st_h > 0 && st_p > 0, LVAR_ERR_ARG,
+               "cache strides must be positive (got page=%lld head=%lld row=%lld elements)", (long long)sp, (long long)sh,
+               (long long)sl);
+  cuuint64_t strides[3] = {st_l, st_h, st_p};
+  const bool narrow = row_bytes == 64;
+  cuuint32_t box[4] = {(cuuint32_t)((narrow ? 64 : 128) / elt), (cuuint32_t)box_rows, 1u, 1u};
+  cuuint32_t estr[4] = {1u, 1u, 1u, 1u};
+  CUresult r = fn(out, bytes ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base),
+                  dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  narrow ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  LVAR_REQUIRE(r == CUDA_SUCCESS, LVAR_ERR_CUDA, "cuTensorMapEncodeTiled failed with CUresult %d", (int)r);
+  return LVAR_OK;
+}
+
 int launch_attention(const lvar_attn_args* a, int mode, cudaStream_t stream);
 int launch_colsum(const void* q, const void* k, const float* M, const float* L, float* cs, int B, int H, int Lq,
                   int Lkv, int D, int64_t q_sb, int64_t q_sh, int64_t q_sl, int64_t k_sb, int64_t k_sh, int64_t k_sl,

@@ -36,6 +36,11 @@ int encode_bhld_map(CUtensorMap* out, const void* base, int B, int H, int L, int
 // elements and 128-byte swizzle, as the four-row TMA gather wants it.  Returns an LVAR_* code.
 int encode_rows_map(CUtensorMap* out, const void* base, int64_t rows, int64_t width, int64_t pitch);
 
+// Encodes a 4-D tensor map over cache pages [pages, H, page_size, D] (D contiguous, bf16 or bytes; strides in elements) with
+// a [1, 1, box_rows, 128 bytes] box and 128-byte swizzle, or 64 bytes and 64-byte swizzle where a row has no more.
+int encode_pages_map(CUtensorMap* out, const void* base, bool bytes, int pages, int H, int page_size, int D, int64_t sp,
+                     int64_t sh, int64_t sl, int box_rows);
+
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 // Bilinear resize between two square token grids (align_corners = False): the four source tokens and the

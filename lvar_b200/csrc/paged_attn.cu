@@ -8,11 +8,13 @@
 // through tensor memory for the running softmax of every 64 keys.  16 rows per warp leave the matrix pipe several times
 // ahead of HBM (16 flops per byte against the 250 that the chip's ratio allows), so it is not what bounds the kernel.
 //
-// A CTA of four warps streams tiles of keys through a ring in shared memory (cp.async, 16 bytes, XOR-swizzled rows; rows
-// behind the sequence's end are zero-filled, so that nothing that lies in a page behind it is ever read).  With up to 16
-// rows the four warps take a quarter of a tile's keys each and have a running maximum, sum and accumulator of their own,
-// joined once at the end of the piece; with more rows (up to 64 per CTA) two or four warps share the keys and differ in
-// their rows.
+// A CTA is four warps that compute and one that loads.  The loader follows the page table (one lane per box of 16 to 128
+// rows that lie together in a page) and streams tiles of keys through a ring in shared memory with tensor-map copies,
+// swizzled; the others wait for a tile and hand its place back, and meet only at an item's end.  Rows of a box behind the
+// sequence's end are copied too: their scores are masked, and elements of V that are not finite never meet a weight of zero
+// (see `edge`).  With up to 16 rows the four warps take a quarter of a tile's keys each and have a running maximum, sum and
+// accumulator of their own, joined once at the end of the piece; with more rows (up to 64 per CTA) two or four warps share
+// the keys and differ in their rows.
 //
 // Split over the cache's length: all tiles of all (sequence, key head, row tile) items form one line that the CTAs (two
 // per SM) share evenly, whatever the lengths are: they are read on the device.  An item that falls to several CTAs leaves
@@ -34,7 +36,8 @@ namespace lvar {
 
 namespace {
 
-constexpr int kThreads = 128;
+constexpr int kThreads = 128;               // threads that compute
+constexpr int kAllThreads = kThreads + 32;  // and the loader
 constexpr int kSlotsPerCta = 2;
 
 struct PagedAttnParams {
@@ -53,16 +56,17 @@ struct PagedAttnParams {
   int causal, max_len;
   int split;            // 0: CTA x takes item x
   float scale_log2;
+  int box;              // rows per copy
+  uint64_t wait_limit_ns;
 };
 
-__device__ __forceinline__ void cp_async_16_zfill(uint32_t dst, const void* src, bool ok) {
-  const int n = ok ? 16 : 0;
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+// An untiled copy of a multiple of 16 bytes between 16-byte aligned places.
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src),
+               "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
 }
-__device__ __forceinline__ void cp_async_4_zfill(uint32_t dst, const void* src, bool ok) {
-  const int n = ok ? 4 : 0;
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
-}
+__device__ __forceinline__ void compute_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kThreads) : "memory"); }
 __device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
@@ -96,11 +100,10 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], u
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// Two e4m3 bytes to two fp16 (exact); the low byte goes to the low half.
-__device__ __forceinline__ uint32_t widen2(uint32_t two) {
-  uint32_t r;
-  asm("{\n.reg .b16 t;\ncvt.u16.u32 t, %1;\ncvt.rn.f16x2.e4m3x2 %0, t;\n}" : "=r"(r) : "r"(two));
-  return r;
+// Four e4m3 bytes to two pairs of fp16 (exact); the lowest byte goes to the low half of `lo`.
+__device__ __forceinline__ void widen4(uint32_t four, uint32_t& lo, uint32_t& hi) {
+  asm("{\n.reg .b16 a, b;\nmov.b32 {a, b}, %2;\ncvt.rn.f16x2.e4m3x2 %0, a;\ncvt.rn.f16x2.e4m3x2 %1, b;\n}"
+      : "=r"(lo), "=r"(hi) : "r"(four));
 }
 __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
   uint32_t r;
@@ -112,26 +115,23 @@ __device__ __forceinline__ float pow2i(int e) { return __int_as_float((e + 127) 
 template <int D, bool Q8>
 struct Geo {
   static constexpr int RB = D * (Q8 ? 1 : 2);             // bytes of a cached row
+  static constexpr int RS = RB < 128 ? RB : 128;          // bytes of a row of a sub-tile, the widest that a copy swizzles
+  static constexpr int SUBS = RB / RS;                    // sub-tiles side by side
   static constexpr int KT = Q8 || D == 64 ? 128 : 64;     // keys per tile
-  static constexpr int CPR = RB / 16;                     // 16-byte chunks per row
-  static constexpr int RP = kThreads / CPR;               // rows per pass of the loaders
-  static constexpr int CPT = KT / RP;                     // passes
-  static constexpr int GROUP = RP < 16 ? 16 : RP;         // rows whose page is looked up at a time by one thread
-  static constexpr int PPG = GROUP / RP;
+  static constexpr int SUB = KT * RS;                     // bytes of a sub-tile
   static constexpr int STAGE = 2 * KT * RB;               // K and V
   static constexpr int STAGES = STAGE <= 16384 ? 6 : 3;
   static constexpr int SCALE_STAGE = Q8 ? KT * 2 : 0;
   static constexpr int RING = STAGES * (STAGE + SCALE_STAGE);
   static constexpr int ML = 4 * 16 * 2 * 4;               // maxima and sums of the four warps' rows
-  static constexpr int SMEM = RING + ML + 64;
+  static constexpr int SMEM = RING + ML + 64 + 2 * STAGES * 8 + 16 + 1024;  // and the start's alignment
   static_assert(4 * 16 * D * 4 <= STAGE, "the warps' accumulators are joined in a consumed stage");
 };
 
-// Byte offset of a 16-byte chunk inside a K or V tile.
-template <int RB>
-__device__ __forceinline__ uint32_t chunk_at(int row, int chunk) {
-  const int x = RB == 64 ? (row >> 1) & 3 : row & 7;
-  return (uint32_t)(row * RB + ((chunk ^ x) << 4));
+// The swizzle of a sub-tile's row: what its 16-byte chunk numbers are XORed with (as the copies do).
+template <int RS>
+__device__ __forceinline__ int swizzle_of(int row) {
+  return RS == 64 ? (row >> 1) & 3 : row & 7;
 }
 
 struct Cursor {
@@ -226,53 +226,6 @@ __device__ __forceinline__ void advance(const PagedAttnParams& p, Cursor& c) {
   }
 }
 
-template <int D, bool Q8>
-__device__ __forceinline__ void load_tile(const PagedAttnParams& p, const Cursor& cur, uint32_t ring, int stage) {
-  using X = Geo<D, Q8>;
-  const int tid = threadIdx.x;
-  const int chunk = tid % X::CPR, r0 = tid / X::CPR;
-  const int key0 = cur.tile * X::KT;
-  const int h = cur.hr / p.RT;
-  const int32_t* trow = p.c.table + cur.b * p.c.t_sb;
-  const uint8_t* kb = p.c.k + h * p.c.k_sh + chunk * 16;
-  const uint8_t* vb = p.c.v + h * p.c.v_sh + chunk * 16;
-  const uint32_t ks = ring + stage * X::STAGE, vs = ks + X::KT * X::RB;
-  int page[X::CPT / X::PPG];
-  uint32_t in[X::CPT / X::PPG];
-#pragma unroll
-  for (int g = 0; g < X::CPT / X::PPG; ++g) {
-    const int pos = key0 + g * X::GROUP + r0;
-    const uint32_t grp = (uint32_t)pos >> 4, pg = page_of_group(p.c, grp);
-    in[g] = (grp - pg * p.c.groups) * 16 + (pos & 15);
-    page[g] = pos < cur.len ? __ldg(trow + pg) : 0;
-  }
-#pragma unroll
-  for (int g = 0; g < X::CPT / X::PPG; ++g) {
-    if ((uint32_t)page[g] >= (uint32_t)p.c.num_pages && p.status) atomicCAS(p.status, 0, (int)DEV_BAD_INDEX);
-    const bool good = (uint32_t)page[g] < (uint32_t)p.c.num_pages;
-    const int64_t pg = good ? page[g] : 0;
-#pragma unroll
-    for (int j = 0; j < X::PPG; ++j) {
-      const int row = g * X::GROUP + j * X::RP + r0;
-      const bool ok = good && key0 + row < cur.len;
-      const int64_t r = in[g] + j * X::RP;
-      cp_async_16_zfill(ks + chunk_at<X::RB>(row, chunk), kb + pg * p.c.k_sp + r * p.c.k_sl, ok);
-      cp_async_16_zfill(vs + chunk_at<X::RB>(row, chunk), vb + pg * p.c.v_sp + r * p.c.v_sl, ok);
-    }
-  }
-  if constexpr (Q8) {
-    if (tid < X::KT / 2) {  // two rows' exponents
-      const int pos = key0 + tid * 2;
-      const uint32_t grp = (uint32_t)pos >> 4, pg = page_of_group(p.c, grp);
-      const uint32_t r = (grp - pg * p.c.groups) * 16 + (pos & 15);
-      const int page1 = pos < cur.len ? __ldg(trow + pg) : -1;
-      const bool ok = (uint32_t)page1 < (uint32_t)p.c.num_pages;
-      cp_async_4_zfill(ring + X::STAGES * X::STAGE + stage * X::SCALE_STAGE + tid * 4,
-                       p.c.scales + (ok ? page1 : 0) * p.c.s_sp + h * p.c.s_sh + r * 2, ok);
-    }
-  }
-}
-
 // One warp's running state over an item: two rows per thread (lane / 4 and + 8).
 template <int D>
 struct State {
@@ -281,20 +234,196 @@ struct State {
   float mt[2];       // e4m3: maximum of score + V exponent, which the accumulators are relative to
 };
 
+// Fetches the tiles of a CTA's range, `nt` from `cur` on, into the ring.
+template <int D, bool Q8>
+__device__ __forceinline__ void loader(const CUtensorMap& mk, const CUtensorMap& mv, const PagedAttnParams& p, Cursor cur, int nt,
+                                       uint8_t* ring, uint64_t* full, uint64_t* empty, const WaitCtx& w) {
+  using X = Geo<D, Q8>;
+  const int lane = threadIdx.x & 31;
+  const uint32_t box_bytes = (uint32_t)p.box * (2 * X::RB + (Q8 ? 2 : 0));
+  int stage = 0, issued = 0;
+  uint32_t phase = 0;
+  for (; issued < nt; ++issued) {
+    if (issued >= X::STAGES && !mbar_wait(&empty[stage], phase ^ 1, w, DEV_TIMEOUT_PRODUCER)) break;
+    const int key0 = cur.tile * X::KT;
+    const int boxes = min(X::KT / p.box, (cur.len - key0 + p.box - 1) / p.box);  // 0 for an empty sequence
+    if (lane == 0) mbar_arrive_expect_tx(&full[stage], boxes * box_bytes);
+    __syncwarp();
+    if (lane < boxes) {
+      const uint32_t grp = (uint32_t)(key0 + lane * p.box) >> 4, pg = page_of_group(p.c, grp);
+      const int row = (int)(grp - pg * p.c.groups) * 16, h = cur.hr / p.RT;
+      int page = p.c.table[cur.b * p.c.t_sb + pg];
+      if ((uint32_t)page >= (uint32_t)p.c.num_pages) {
+        if (p.status) atomicCAS(p.status, 0, (int)DEV_BAD_INDEX);
+        page = 0;
+      }
+      uint8_t* dst = ring + stage * X::STAGE + lane * p.box * X::RS;
+#pragma unroll
+      for (int s = 0; s < X::SUBS; ++s) {
+        tma_load_4d(dst + s * X::SUB, &mk, &full[stage], s * 64, row, h, page);
+        tma_load_4d(dst + X::KT * X::RB + s * X::SUB, &mv, &full[stage], s * 64, row, h, page);
+      }
+      if constexpr (Q8) {
+        bulk_load(smem_u32(ring + X::STAGES * X::STAGE + stage * X::SCALE_STAGE + lane * p.box * 2),
+                  p.c.scales + page * p.c.s_sp + h * p.c.s_sh + row * 2, p.box * 2, &full[stage]);
+      }
+    }
+    advance<X::KT>(p, cur);
+    if (++stage == X::STAGES) stage = 0, phase ^= 1;
+  }
+  // Shared memory must not go while a copy is in flight, also after a wait that ran out.
+  for (int i = issued > X::STAGES ? issued - X::STAGES : 0; i < issued; ++i) {
+    const uint64_t t0 = globaltimer_ns();
+    while (!mbar_try_wait(&full[i % X::STAGES], (i / X::STAGES) & 1)) {
+      if (globaltimer_ns() - t0 > LVAR_DEFAULT_WAIT_NS) {
+        if (p.status) atomicCAS(p.status, 0, (int)DEV_TIMEOUT_DRAIN);
+        break;
+      }
+    }
+  }
+}
+
+// O += P V of one step, 16 keys at a time.  CLEAN: elements of V that are not finite are left out.
+template <int D, bool Q8, int NT, bool CLEAN>
+__device__ __forceinline__ void weigh(State<D>& st, const float (&sc)[NT][4], uint32_t vs, int s0) {
+  using X = Geo<D, Q8>;
+  const int lane = threadIdx.x & 31, quad = lane & 3;
+#pragma unroll
+  for (int n2 = 0; n2 < NT / 2; ++n2) {
+    if constexpr (!Q8) {
+      const uint32_t a[4] = {pack_bf16x2(sc[2 * n2][0], sc[2 * n2][1]), pack_bf16x2(sc[2 * n2][2], sc[2 * n2][3]),
+                             pack_bf16x2(sc[2 * n2 + 1][0], sc[2 * n2 + 1][1]),
+                             pack_bf16x2(sc[2 * n2 + 1][2], sc[2 * n2 + 1][3])};
+      const uint32_t v0 = vs + (s0 + n2 * 16 + (lane & 15)) * X::RS + (((lane >> 4) ^ (lane & 7)) << 4);
+#pragma unroll
+      for (int d2 = 0; d2 < D / 16; ++d2) {
+        uint32_t b[4];
+        ldsm_x4_t((v0 ^ ((d2 & 3) << 5)) + (d2 >> 2) * X::SUB, b);
+        if constexpr (CLEAN) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            if ((b[j] & 0x7f80u) == 0x7f80u) b[j] &= 0xffff0000u;
+            if ((b[j] & 0x7f800000u) == 0x7f800000u) b[j] &= 0xffffu;
+          }
+        }
+        mma_bf16(st.acc[d2 * 2], a, b[0], b[1]);
+        mma_bf16(st.acc[d2 * 2 + 1], a, b[2], b[3]);
+      }
+    } else {
+      const uint32_t a[4] = {pack_f16x2(sc[2 * n2][0], sc[2 * n2][1]), pack_f16x2(sc[2 * n2][2], sc[2 * n2][3]),
+                             pack_f16x2(sc[2 * n2 + 1][0], sc[2 * n2 + 1][1]),
+                             pack_f16x2(sc[2 * n2 + 1][2], sc[2 * n2 + 1][3])};
+      constexpr int W = D / 32;  // words per thread and key: D / 8 consecutive elements, lane / 4 says which
+      const uint32_t r0 = vs + (s0 + n2 * 16 + quad * 2) * X::RS;
+      uint32_t u[4][W];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {  // keys 2 quad, 2 quad + 1, and both + 8
+        const uint32_t r = r0 + ((j & 1) + (j >> 1) * 8) * X::RS;
+        if constexpr (D == 128) {
+          const uint4 x = lds128(r + (((lane >> 2) ^ (quad * 2 + (j & 1))) << 4));
+          u[j][0] = x.x, u[j][1] = x.y, u[j][2] = x.z, u[j][3] = x.w;
+        } else {
+          const uint2 x = lds64(r + (((lane >> 3) ^ quad) << 4) + ((lane >> 2) & 1) * 8);
+          u[j][0] = x.x, u[j][1] = x.y;
+        }
+        if constexpr (CLEAN) {
+#pragma unroll
+          for (int i = 0; i < W; ++i)
+#pragma unroll
+            for (int y = 0; y < 4; ++y)
+              if (((u[j][i] >> (8 * y)) & 0x7fu) == 0x7fu) u[j][i] &= ~(0xffu << (8 * y));
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < W; ++i) {
+        uint32_t b[4][2];
+        widen4(__byte_perm(u[0][i], u[1][i], 0x5140), b[0][0], b[1][0]);
+        widen4(__byte_perm(u[0][i], u[1][i], 0x7362), b[2][0], b[3][0]);
+        widen4(__byte_perm(u[2][i], u[3][i], 0x5140), b[0][1], b[1][1]);
+        widen4(__byte_perm(u[2][i], u[3][i], 0x7362), b[2][1], b[3][1]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) mma_f16(st.acc[i * 4 + j], a, b[j][0], b[j][1]);
+      }
+    }
+  }
+}
+
+// Whether any of a step's V elements is not finite; by the whole warp.
+template <int D, bool Q8, int NS>
+__device__ __forceinline__ bool any_odd(uint32_t vs, int s0) {
+  using X = Geo<D, Q8>;
+  const int lane = threadIdx.x & 31;
+  uint32_t hit = 0;
+#pragma unroll
+  for (int s = 0; s < X::SUBS; ++s) {
+#pragma unroll
+    for (int i = 0; i < NS * X::RS / 512; ++i) {
+      const uint4 x = lds128(vs + s * X::SUB + s0 * X::RS + i * 512 + lane * 16);
+      const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        hit |= Q8 ? ((w[j] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u : ((w[j] & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
+    }
+  }
+  return __any_sync(0xffffffffu, hit != 0);
+}
+
+// The elements of V that CLEAN left out, row by row: a row takes those that it sees.
+template <int D, bool Q8, int NT>
+__device__ __noinline__ void weigh_odd(State<D>& st, const float (&sc)[NT][4], uint32_t vs, int s0, int seen0, int seen1) {
+  using X = Geo<D, Q8>;
+  const int lane = threadIdx.x & 31, quad = lane & 3;
+  for (int j = 0; j < NT * 8; ++j) {
+    const int from = (lane & 28) | ((j & 7) >> 1);  // the lane of the quad that has this row pair's weights of key j
+    const float w0 = __shfl_sync(0xffffffffu, sc[j >> 3][j & 1], from);
+    const float w1 = __shfl_sync(0xffffffffu, sc[j >> 3][2 + (j & 1)], from);
+    const int row = s0 + j;
+    for (int n = 0; n < D / 8; ++n)
+      for (int e = 0; e < 2; ++e) {
+        const int d = Q8 ? (quad * 2 + e) * (D / 8) + n : n * 8 + quad * 2 + e;
+        const int byte = d * (Q8 ? 1 : 2), chunk = (byte % X::RS) >> 4;
+        const uint32_t at = vs + byte / X::RS * X::SUB + row * X::RS + ((chunk ^ swizzle_of<X::RS>(row)) << 4) + (byte & 15);
+        const uint32_t bits = lds32(at & ~3u) >> ((at & 3u) * 8);
+        const float val = Q8 ? NAN : __uint_as_float(bits << 16);
+        const bool odd = Q8 ? (bits & 0x7fu) == 0x7fu : (bits & 0x7f80u) == 0x7f80u;
+        if (odd && j < seen0) st.acc[n][e] = fmaf(w0, val, st.acc[n][e]);
+        if (odd && j < seen1) st.acc[n][e + 2] = fmaf(w1, val, st.acc[n][e + 2]);
+      }
+  }
+}
+
 template <int D, bool Q8, int WR>
-__global__ void __launch_bounds__(kThreads, 2) paged_attn_kernel(const __grid_constant__ PagedAttnParams p) {
+__global__ void __launch_bounds__(kAllThreads, 2)
+    paged_attn_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
+                      const __grid_constant__ PagedAttnParams p) {
   using X = Geo<D, Q8>;
   constexpr int WK = 4 / WR;              // warps that share a row tile and differ in their keys
   constexpr int KW = X::KT / WK;          // keys of a tile per warp
   constexpr int NS = KW < 32 ? KW : 32;   // keys per step
   constexpr int NT = NS / 8;
-  extern __shared__ __align__(1024) uint8_t smem[];
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const uint32_t ring = smem_u32(smem);
   float* ml = reinterpret_cast<float*>(smem + X::RING);
   int64_t* scan = reinterpret_cast<int64_t*>(smem + X::RING + X::ML);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + X::RING + X::ML + 64);
+  uint64_t* empty = full + X::STAGES;
+  int* abort_flag = reinterpret_cast<int*>(empty + X::STAGES);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int wr = warp % WR, wk = warp / WR, quad = lane & 3;
+  const WaitCtx wait{p.status, abort_flag, p.wait_limit_ns};
 
+  if (tid == 0) {
+    for (int i = 0; i < X::STAGES; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 4);
+    }
+    *abort_flag = 0;
+    mbar_fence_init();
+    tma_prefetch_desc(&mk);
+    tma_prefetch_desc(&mv);
+  }
+  __syncthreads();
   griddep_wait();
   Cursor cons;
   int nt;
@@ -318,15 +447,9 @@ __global__ void __launch_bounds__(kThreads, 2) paged_attn_kernel(const __grid_co
     cons.len = length_of(p, cons.b);
     cons.ntile = nt = tiles_of<X::KT>(cons.len);
   }
-
-  Cursor prod = cons;
-#pragma unroll
-  for (int i = 0; i < X::STAGES - 1; ++i) {
-    if (i < nt) {
-      load_tile<D, Q8>(p, prod, ring, i);
-      advance<X::KT>(p, prod);
-    }
-    cp_async_commit();
+  if (warp == 4) {
+    loader<D, Q8>(mk, mv, p, cons, nt, smem, full, empty, wait);
+    return;
   }
 
   State<D> st;
@@ -334,18 +457,11 @@ __global__ void __launch_bounds__(kThreads, 2) paged_attn_kernel(const __grid_co
   float qs[2];      // factor from the raw product to log2 units, per row
   int limit[2];     // keys that the row sees
   int see_all = 0;  // keys that every row of the item sees
-  bool first_piece = true, fresh = true;
+  bool first_piece = true, fresh = true, alive = true;
+  int stage = 0;
+  uint32_t phase = 0;
 
   for (int i = 0; i < nt; ++i) {
-    const int stage = i % X::STAGES;
-    cp_async_wait<X::STAGES - 2>();
-    __syncthreads();
-    if (i + X::STAGES - 1 < nt) {
-      load_tile<D, Q8>(p, prod, ring, (i + X::STAGES - 1) % X::STAGES);
-      advance<X::KT>(p, prod);
-    }
-    cp_async_commit();
-
     const int rt = cons.hr % p.RT, h = cons.hr / p.RT;
     if (fresh) {
       fresh = false;
@@ -375,13 +491,8 @@ __global__ void __launch_bounds__(kThreads, 2) paged_attn_kernel(const __grid_co
           float most = 0.f;
           bool fine = true;
 #pragma unroll
-          for (int ch = 0; ch < CH; ++ch) {
-#pragma unroll
-            for (int s = 0; s < 4; ++s) {
-              const int e = 16 * (CH * quad + ch) + 4 * s;
-              raw[ch * 4 + s] = live ? *reinterpret_cast<const uint2*>(src + e) : make_uint2(0u, 0u);
-            }
-          }
+          for (int kk = 0; kk < D / 16; ++kk)
+            raw[kk] = live ? *reinterpret_cast<const uint2*>(src + 16 * (CH * quad + kk / 4) + 4 * (kk % 4)) : make_uint2(0u, 0u);
 #pragma unroll
           for (int kk = 0; kk < D / 16; ++kk) {
             const uint32_t w[2] = {raw[kk].x, raw[kk].y};
@@ -407,8 +518,9 @@ __global__ void __launch_bounds__(kThreads, 2) paged_attn_kernel(const __grid_co
         }
       }
     }
+    alive = alive && mbar_wait(&full[stage], phase, wait, DEV_TIMEOUT_SOFTMAX);
 
-    const bool idle = rt * 16 * WR + wr * 16 >= p.R;  // none of the warp's rows exists
+    const bool idle = rt * 16 * WR + wr * 16 >= p.R || !alive;  // none of the warp's rows exists
     const uint32_t ks = ring + stage * X::STAGE, vs = ks + X::KT * X::RB;
     const uint32_t ss = ring + X::STAGES * X::STAGE + stage * X::SCALE_STAGE;
 #pragma unroll 1
@@ -422,43 +534,48 @@ __global__ void __launch_bounds__(kThreads, 2) paged_attn_kernel(const __grid_co
       if constexpr (!Q8) {
 #pragma unroll
         for (int n2 = 0; n2 < NT / 2; ++n2) {
-          const int row = s0 + n2 * 16 + (lane & 7) + ((lane >> 4) << 3);
+          const uint32_t k0 = ks + (s0 + n2 * 16 + (lane & 7) + ((lane >> 4) << 3)) * X::RS + ((((lane >> 3) & 1) ^ (lane & 7)) << 4);
 #pragma unroll
           for (int kk = 0; kk < D / 16; ++kk) {
             uint32_t b[4];
-            ldsm_x4(ks + chunk_at<X::RB>(row, kk * 2 + ((lane >> 3) & 1)), b);
+            ldsm_x4((k0 ^ ((kk & 3) << 5)) + (kk >> 2) * X::SUB, b);
             mma_bf16(sc[n2 * 2], qf[kk], b[0], b[1]);
             mma_bf16(sc[n2 * 2 + 1], qf[kk], b[2], b[3]);
           }
         }
       } else {
         constexpr int CH = D / 64;
+        const uint32_t k0 = ks + (s0 + (lane >> 2)) * X::RS + (((CH * quad) ^ swizzle_of<X::RS>(lane >> 2)) << 4);
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          const int row = s0 + n * 8 + (lane >> 2);
+        for (int ch = 0; ch < CH; ++ch) {
+          uint4 w[NT];
 #pragma unroll
-          for (int ch = 0; ch < CH; ++ch) {
-            const uint4 w = lds128(ks + chunk_at<X::RB>(row, CH * quad + ch));
-            const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+          for (int n = 0; n < NT; ++n) w[n] = lds128((k0 ^ (ch << 4)) + n * 8 * X::RS);
 #pragma unroll
-            for (int s = 0; s < 4; ++s) mma_f16(sc[n], qf[ch * 4 + s], widen2(u[s]), widen2(u[s] >> 16));
+          for (int n = 0; n < NT; ++n) {
+            const uint32_t u[4] = {w[n].x, w[n].y, w[n].z, w[n].w};
+#pragma unroll
+            for (int s = 0; s < 4; ++s) {
+              uint32_t lo, hi;
+              widen4(u[s], lo, hi);
+              mma_f16(sc[n], qf[ch * 4 + s], lo, hi);
+            }
           }
         }
       }
-      // to log2 units; e4m3: with the rows' scales
-      uint32_t ex[NT];  // e4m3: biased exponents (K, V) of the thread's two keys
+      // e4m3: scores to log2 units, with the rows' scales (bf16: one factor, taken in with the maximum below)
+      uint64_t ve[NT];  // V's exponents of the thread's two keys
+      if constexpr (Q8) {
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        if constexpr (Q8) {
-          ex[n] = lds32(ss + (s0 + n * 8 + quad * 2) * 2);
-          const float k0 = __uint_as_float((ex[n] & 0xffu) << 23), k1 = __uint_as_float((ex[n] & 0xff0000u) << 7);
-          sc[n][0] *= k0 * qs[0];
-          sc[n][1] *= k1 * qs[0];
-          sc[n][2] *= k0 * qs[1];
-          sc[n][3] *= k1 * qs[1];
-        } else {
+        for (int n = 0; n < NT; ++n) {
+          const uint32_t ex = lds32(ss + (s0 + n * 8 + quad * 2) * 2);  // K, V, K, V
+          const uint64_t kf = pack_f32x2(__uint_as_float((ex << 23) & 0x7f800000u), __uint_as_float((ex << 7) & 0x7f800000u));
+          // a byte below the exponent of 2^23 is 2^23 + byte
+          ve[n] = fadd2(pack_f32x2(__uint_as_float(__byte_perm(ex, 0x4b000000u, 0x7441)), __uint_as_float(__byte_perm(ex, 0x4b000000u, 0x7443))),
+                        pack_f32x2(-8388608.f - 127.f, -8388608.f - 127.f));
 #pragma unroll
-          for (int e = 0; e < 4; ++e) sc[n][e] *= qs[0];
+          for (int x = 0; x < 2; ++x)
+            unpack_f32x2(fmul2(pack_f32x2(sc[n][2 * x], sc[n][2 * x + 1]), fmul2(kf, pack_f32x2(qs[x], qs[x]))), sc[n][2 * x], sc[n][2 * x + 1]);
         }
       }
       const bool edge = key0 + NS > see_all;  // some row does not see some of these keys
@@ -473,154 +590,80 @@ __global__ void __launch_bounds__(kThreads, 2) paged_attn_kernel(const __grid_co
       float alpha[2];
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
-        float mx = st.m[x], tx = st.mt[x];
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          mx = fmaxf(mx, fmaxf(sc[n][2 * x], sc[n][2 * x + 1]));
-          if constexpr (Q8) {
-            const float e0 = (float)((int)((ex[n] >> 8) & 0xffu) - 127), e1 = (float)((int)(ex[n] >> 24) - 127);
-            tx = fmaxf(tx, fmaxf(sc[n][2 * x] + e0, sc[n][2 * x + 1] + e1));
-          }
-        }
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        const float mu = mx == -INFINITY ? 0.f : mx;
-        float add = 0.f;
         if constexpr (Q8) {
-          tx = fmaxf(tx, __shfl_xor_sync(0xffffffffu, tx, 1));
-          tx = fmaxf(tx, __shfl_xor_sync(0xffffffffu, tx, 2));
-          const float tu = tx == -INFINITY ? 0.f : tx - 15.f;  // weights up to 2^15
+          float mx = st.m[x], tx = st.mt[x];
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
-            const float e0 = (float)((int)((ex[n] >> 8) & 0xffu) - 127), e1 = (float)((int)(ex[n] >> 24) - 127);
-            const float s0v = sc[n][2 * x], s1v = sc[n][2 * x + 1];
-            add += fast_exp2(s0v - mu) + fast_exp2(s1v - mu);
-            sc[n][2 * x] = fast_exp2(s0v + e0 - tu);
-            sc[n][2 * x + 1] = fast_exp2(s1v + e1 - tu);
+            float t0, t1;
+            unpack_f32x2(fadd2(pack_f32x2(sc[n][2 * x], sc[n][2 * x + 1]), ve[n]), t0, t1);
+            mx = fmax3(mx, sc[n][2 * x], sc[n][2 * x + 1]);
+            tx = fmax3(tx, t0, t1);
+          }
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+          tx = fmaxf(tx, __shfl_xor_sync(0xffffffffu, tx, 1));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+          tx = fmaxf(tx, __shfl_xor_sync(0xffffffffu, tx, 2));
+          const float mu = mx == -INFINITY ? 0.f : -mx;
+          const float tu = tx == -INFINITY ? 0.f : 15.f - tx;  // weights up to 2^15
+          float add = 0.f;
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            const uint64_t s = pack_f32x2(sc[n][2 * x], sc[n][2 * x + 1]);
+            float a, b, c, d;
+            unpack_f32x2(fadd2(s, pack_f32x2(mu, mu)), a, b);
+            unpack_f32x2(fadd2(fadd2(s, ve[n]), pack_f32x2(tu, tu)), c, d);
+            add += fast_exp2(a) + fast_exp2(b);
+            sc[n][2 * x] = fast_exp2(c);
+            sc[n][2 * x + 1] = fast_exp2(d);
           }
           alpha[x] = fast_exp2(st.mt[x] - (tx == -INFINITY ? 0.f : tx));
-          st.l[x] = st.l[x] * fast_exp2(st.m[x] - mu) + add;
+          st.l[x] = st.l[x] * fast_exp2(st.m[x] + mu) + add;
+          st.m[x] = mx;
           st.mt[x] = tx;
         } else {
+          float raw = -INFINITY;
+#pragma unroll
+          for (int n = 0; n < NT; ++n) raw = fmax3(raw, sc[n][2 * x], sc[n][2 * x + 1]);
+          raw = fmaxf(raw, __shfl_xor_sync(0xffffffffu, raw, 1));
+          raw = fmaxf(raw, __shfl_xor_sync(0xffffffffu, raw, 2));
+          const float mx = fmaxf(st.m[x], raw * qs[x]);
+          const float mu = mx == -INFINITY ? 0.f : -mx;
+          float add = 0.f;
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
-            sc[n][2 * x] = fast_exp2(sc[n][2 * x] - mu);
-            sc[n][2 * x + 1] = fast_exp2(sc[n][2 * x + 1] - mu);
+            float a, b;
+            unpack_f32x2(ffma2(pack_f32x2(sc[n][2 * x], sc[n][2 * x + 1]), pack_f32x2(qs[x], qs[x]), pack_f32x2(mu, mu)), a, b);
+            sc[n][2 * x] = fast_exp2(a);
+            sc[n][2 * x + 1] = fast_exp2(b);
             add += sc[n][2 * x] + sc[n][2 * x + 1];
           }
-          alpha[x] = fast_exp2(st.m[x] - mu);
+          alpha[x] = fast_exp2(st.m[x] + mu);
           st.l[x] = st.l[x] * alpha[x] + add;
+          st.m[x] = mx;
         }
-        st.m[x] = mx;
       }
       if (__any_sync(0xffffffffu, !(alpha[0] == 1.f && alpha[1] == 1.f))) {
 #pragma unroll
-        for (int n = 0; n < D / 8; ++n) {
-          st.acc[n][0] *= alpha[0];
-          st.acc[n][1] *= alpha[0];
-          st.acc[n][2] *= alpha[1];
-          st.acc[n][3] *= alpha[1];
-        }
+        for (int n = 0; n < D / 8; ++n)
+#pragma unroll
+          for (int x = 0; x < 2; ++x)
+            unpack_f32x2(fmul2(pack_f32x2(st.acc[n][2 * x], st.acc[n][2 * x + 1]), pack_f32x2(alpha[x], alpha[x])), st.acc[n][2 * x],
+                         st.acc[n][2 * x + 1]);
       }
-      // O += P V, 16 keys at a time.  In a step that some row does not see all of, elements of V that are not finite are
-      // left out here and come in row by row below: a weight of zero would make NaN of them in rows that do not see them.
-      bool odd = false;
+      // In a step that some row does not see all of, elements of V that are not finite come in row by row: a weight of zero
+      // would make NaN of them in rows that do not see them.
+      if (edge && any_odd<D, Q8, NS>(vs, s0)) {
+        weigh<D, Q8, NT, true>(st, sc, vs, s0);
+        State<D> st2 = st;
+        float w[NT][4];
 #pragma unroll
-      for (int n2 = 0; n2 < NT / 2; ++n2) {
-        if constexpr (!Q8) {
-          const uint32_t a[4] = {pack_bf16x2(sc[2 * n2][0], sc[2 * n2][1]), pack_bf16x2(sc[2 * n2][2], sc[2 * n2][3]),
-                                 pack_bf16x2(sc[2 * n2 + 1][0], sc[2 * n2 + 1][1]),
-                                 pack_bf16x2(sc[2 * n2 + 1][2], sc[2 * n2 + 1][3])};
-          const int row = s0 + n2 * 16 + (lane & 15);
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int d2 = 0; d2 < D / 16; ++d2) {
-            uint32_t b[4];
-            ldsm_x4_t(vs + chunk_at<X::RB>(row, d2 * 2 + (lane >> 4)), b);
-            if (edge) {
-#pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                if ((b[j] & 0x7f80u) == 0x7f80u) b[j] &= 0xffff0000u, odd = true;
-                if ((b[j] & 0x7f800000u) == 0x7f800000u) b[j] &= 0xffffu, odd = true;
-              }
-            }
-            mma_bf16(st.acc[d2 * 2], a, b[0], b[1]);
-            mma_bf16(st.acc[d2 * 2 + 1], a, b[2], b[3]);
-          }
-        } else {
-          const uint32_t a[4] = {pack_f16x2(sc[2 * n2][0], sc[2 * n2][1]), pack_f16x2(sc[2 * n2][2], sc[2 * n2][3]),
-                                 pack_f16x2(sc[2 * n2 + 1][0], sc[2 * n2 + 1][1]),
-                                 pack_f16x2(sc[2 * n2 + 1][2], sc[2 * n2 + 1][3])};
-          const int row = s0 + n2 * 16 + quad * 2;
-          constexpr int W = D / 32;  // words per thread and key: D / 8 consecutive elements, lane / 4 says which
-          uint32_t u[4][W];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int r = row + (j & 1) + (j >> 1) * 8;
-            if constexpr (D == 128) {
-              const uint4 w = lds128(vs + chunk_at<X::RB>(r, lane >> 2));
-              u[j][0] = w.x, u[j][1] = w.y, u[j][2] = w.z, u[j][3] = w.w;
-            } else {
-              const uint2 w = lds64(vs + chunk_at<X::RB>(r, lane >> 3) + ((lane >> 2) & 1) * 8);
-              u[j][0] = w.x, u[j][1] = w.y;
-            }
-            if (edge) {
-#pragma unroll
-              for (int i4 = 0; i4 < W; ++i4)
-#pragma unroll
-                for (int y = 0; y < 4; ++y)
-                  if (((u[j][i4] >> (8 * y)) & 0x7fu) == 0x7fu) u[j][i4] &= ~(0xffu << (8 * y)), odd = true;
-            }
-          }
-#pragma unroll
-          for (int i4 = 0; i4 < W; ++i4) {
-            const uint32_t lo0 = __byte_perm(u[0][i4], u[1][i4], 0x5140), hi0 = __byte_perm(u[0][i4], u[1][i4], 0x7362);
-            const uint32_t lo1 = __byte_perm(u[2][i4], u[3][i4], 0x5140), hi1 = __byte_perm(u[2][i4], u[3][i4], 0x7362);
-            mma_f16(st.acc[i4 * 4], a, widen2(lo0), widen2(lo1));
-            mma_f16(st.acc[i4 * 4 + 1], a, widen2(lo0 >> 16), widen2(lo1 >> 16));
-            mma_f16(st.acc[i4 * 4 + 2], a, widen2(hi0), widen2(hi1));
-            mma_f16(st.acc[i4 * 4 + 3], a, widen2(hi0 >> 16), widen2(hi1 >> 16));
-          }
-        }
-      }
-      if (edge && __any_sync(0xffffffffu, odd)) {
-#pragma unroll 1
-        for (int j = 0; j < NS; ++j) {
-          float w0 = 0.f, w1 = 0.f;  // this row pair's weights of key j, from the lane of the quad that holds them
-#pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            float x0 = sc[n][0], x1 = sc[n][1], x2 = sc[n][2], x3 = sc[n][3];
-            asm volatile("" : "+f"(x0), "+f"(x1), "+f"(x2), "+f"(x3));  // a choice of registers, not of array elements
-            if (n == j >> 3) {
-              w0 = (j & 1) ? x1 : x0;
-              w1 = (j & 1) ? x3 : x2;
-            }
-          }
-          w0 = __shfl_sync(0xffffffffu, w0, (lane & 28) | ((j & 7) >> 1));
-          w1 = __shfl_sync(0xffffffffu, w1, (lane & 28) | ((j & 7) >> 1));
-#pragma unroll
-          for (int n = 0; n < D / 8; ++n)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              float val;
-              bool finite;
-              if constexpr (!Q8) {
-                const int d = n * 8 + quad * 2 + e;
-                const uint32_t at = vs + chunk_at<X::RB>(s0 + j, d >> 3) + (d & 7) * 2;
-                const uint32_t word = lds32(at & ~3u);
-                val = __uint_as_float((d & 1) ? word & 0xffff0000u : word << 16);
-                finite = fabsf(val) < INFINITY;
-              } else {
-                const int d = (quad * 2 + e) * (D / 8) + n;
-                const uint32_t at = vs + chunk_at<X::RB>(s0 + j, d >> 4) + (d & 15);
-                finite = ((lds32(at & ~3u) >> ((at & 3u) * 8)) & 0x7fu) != 0x7fu;
-                val = NAN;
-              }
-              if (!finite) {
-                if (key0 + j < limit[0]) st.acc[n][e] = fmaf(w0, val, st.acc[n][e]);
-                if (key0 + j < limit[1]) st.acc[n][e + 2] = fmaf(w1, val, st.acc[n][e + 2]);
-              }
-            }
-        }
+          for (int e = 0; e < 4; ++e) w[n][e] = sc[n][e];
+        weigh_odd<D, Q8, NT>(st2, w, vs, s0, limit[0] - key0, limit[1] - key0);
+        st = st2;
+      } else {
+        weigh<D, Q8, NT, false>(st, sc, vs, s0);
       }
     }
 
@@ -636,7 +679,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_attn_kernel(const __grid_co
           ml[(warp * 16 + (lane >> 2) + x * 8) * 2 + 1] = st.l[x];
         }
       }
-      __syncthreads();
+      compute_sync();
       float* buf = reinterpret_cast<float*>(smem + stage * X::STAGE);  // [warp][16][D]
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
@@ -662,7 +705,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_attn_kernel(const __grid_co
                               st.acc[n + 3][2 * x + e] * f);
         }
       }
-      __syncthreads();
+      compute_sync();
       const bool whole = last && (!first_piece || whole_first);
       const int slot = first_piece ? 0 : 1;
       constexpr int TPR = D / 8, RPP = kThreads / TPR;
@@ -706,10 +749,14 @@ __global__ void __launch_bounds__(kThreads, 2) paged_attn_kernel(const __grid_co
       }
       first_piece = false;
       fresh = true;
+      compute_sync();            // the maxima and sums are read before the next item's are written
+      fence_proxy_async_smem();  // and the stage is written before the next copy into it
     }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&empty[stage]);
+    if (++stage == X::STAGES) stage = 0, phase ^= 1;
     advance<X::KT>(p, cons);
   }
-  cp_async_wait<0>();
 }
 
 // Joins the pieces of the item that begins in CTA x's range and goes on behind it: a warp per row, pieces in order.
@@ -821,13 +868,13 @@ int plan_of(int B, int Hq, int Hkv, int T, int D, bool q8, int max_len, int sms,
 }
 
 template <int D, bool Q8, int WR>
-int launch(const PagedAttnParams& p, const Plan& plan, cudaStream_t stream) {
+int launch(const PagedAttnParams& p, const CUtensorMap& mk, const CUtensorMap& mv, const Plan& plan, cudaStream_t stream) {
   using X = Geo<D, Q8>;
   auto kern = paged_attn_kernel<D, Q8, WR>;
   LVAR_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, X::SMEM));
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)plan.ctas);
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3(kAllThreads);
   cfg.dynamicSmemBytes = X::SMEM;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
@@ -835,10 +882,11 @@ int launch(const PagedAttnParams& p, const Plan& plan, cudaStream_t stream) {
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  LVAR_CUDA_OK(cudaLaunchKernelEx(&cfg, kern, p));
+  LVAR_CUDA_OK(cudaLaunchKernelEx(&cfg, kern, mk, mv, p));
   if (plan.split) {
     const int rows = p.R < 16 * WR ? p.R : 16 * WR;
     cfg.gridDim = dim3((unsigned)plan.ctas, (unsigned)((rows + 3) / 4));
+    cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = 0;
     LVAR_CUDA_OK(cudaLaunchKernelEx(&cfg, paged_join_kernel<D, Q8, WR>, p, plan.ctas));
   }
@@ -846,10 +894,19 @@ int launch(const PagedAttnParams& p, const Plan& plan, cudaStream_t stream) {
 }
 
 template <int D, bool Q8>
-int launch_wr(const PagedAttnParams& p, const Plan& plan, cudaStream_t stream) {
-  if (plan.wr == 1) return launch<D, Q8, 1>(p, plan, stream);
-  if (plan.wr == 2) return launch<D, Q8, 2>(p, plan, stream);
-  return launch<D, Q8, 4>(p, plan, stream);
+int launch_wr(PagedAttnParams& p, const lvar_paged_cache& c, const Plan& plan, cudaStream_t stream) {
+  using X = Geo<D, Q8>;
+  // Rows per copy: what page and tile have in common, and not far more than the longest sequence has.
+  int box = X::KT;
+  while (c.page_size % box != 0 || X::KT % box != 0) box -= 16;
+  while (box % 32 == 0 && box / 2 >= p.max_len) box /= 2;
+  p.box = box;
+  CUtensorMap mk, mv;
+  if (int rc = encode_pages_map(&mk, c.k, Q8, c.num_pages, c.Hkv, c.page_size, D, c.k_sp, c.k_sh, c.k_sl, box)) return rc;
+  if (int rc = encode_pages_map(&mv, c.v, Q8, c.num_pages, c.Hkv, c.page_size, D, c.v_sp, c.v_sh, c.v_sl, box)) return rc;
+  if (plan.wr == 1) return launch<D, Q8, 1>(p, mk, mv, plan, stream);
+  if (plan.wr == 2) return launch<D, Q8, 2>(p, mk, mv, plan, stream);
+  return launch<D, Q8, 4>(p, mk, mv, plan, stream);
 }
 
 }  // namespace
@@ -903,8 +960,9 @@ int launch_paged_attn(const lvar_paged_attn_args* a, cudaStream_t stream) {
   p.causal = a->causal != 0; p.max_len = max_len;
   p.split = plan.split;
   p.scale_log2 = a->scale * 1.4426950408889634f;
-  if (c.D == 128) return c.scales ? launch_wr<128, true>(p, plan, stream) : launch_wr<128, false>(p, plan, stream);
-  return c.scales ? launch_wr<64, true>(p, plan, stream) : launch_wr<64, false>(p, plan, stream);
+  p.wait_limit_ns = a->wait_limit_ns;
+  if (c.D == 128) return c.scales ? launch_wr<128, true>(p, c, plan, stream) : launch_wr<128, false>(p, c, plan, stream);
+  return c.scales ? launch_wr<64, true>(p, c, plan, stream) : launch_wr<64, false>(p, c, plan, stream);
 }
 
 }  // namespace lvar

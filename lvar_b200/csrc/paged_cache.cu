@@ -36,9 +36,8 @@ int paged_view(const lvar_paged_cache* c, PagedView* out) {
     LVAR_REQUIRE(s >= 0 && s % mult == 0, LVAR_ERR_ARG, "cache strides must be non-negative multiples of %d elements", mult);
   LVAR_REQUIRE(aligned16(c->k) && aligned16(c->v), LVAR_ERR_ARG, "cache tensors must be 16-byte aligned");
   if (c->scales) {
-    LVAR_REQUIRE(c->s_sp >= 0 && c->s_sh >= 0 && c->s_sp % 4 == 0 && c->s_sh % 4 == 0 &&
-                     (reinterpret_cast<uintptr_t>(c->scales) & 3) == 0,
-                 LVAR_ERR_ARG, "scales must be 4-byte aligned with page and head strides in multiples of 4");
+    LVAR_REQUIRE(c->s_sp >= 0 && c->s_sh >= 0 && c->s_sp % 16 == 0 && c->s_sh % 16 == 0 && aligned16(c->scales), LVAR_ERR_ARG,
+                 "scales must be 16-byte aligned with page and head strides in multiples of 16");
   }
   LVAR_REQUIRE(c->t_sb >= 0, LVAR_ERR_ARG, "the table's stride must not be negative");
   PagedView v{};

@@ -858,7 +858,7 @@ def paged_kv_read(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Ten
 def paged_attn_fwd(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor, lens: torch.Tensor,
                    scale: Optional[float] = None, *, scales: Optional[torch.Tensor] = None, causal: bool = False,
                    max_len: Optional[int] = None, return_stats: bool = False, out: Optional[torch.Tensor] = None,
-                   status: Optional[torch.Tensor] = None):
+                   status: Optional[torch.Tensor] = None, wait_limit_ns: Optional[int] = None):
     """Attention of the T newest tokens of every sequence over its paged cache: o = softmax(scale q K^T + mask) V, bf16
     [B, Hq, T, D]; with ``return_stats`` (o, M, L), fp32 [B, Hq, T] as :func:`dense_attn_fwd` returns them.
 
@@ -897,6 +897,7 @@ def paged_attn_fwd(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
         q_sb, q_sh, q_sl, _ = q.stride()
         o_sb, o_sh, o_sl, _ = o.stride()
         a = PagedAttnArgs(c, q.data_ptr(), q_sb, q_sh, q_sl, o.data_ptr(), o_sb, o_sh, o_sl, m_ptr, l_ptr, lens_ptr, w_ptr, work,
-                          _status_ptr(status, dev), float(D ** -0.5 if scale is None else scale), Hq, T, int(bool(causal)), most)
+                          _status_ptr(status, dev), _lib.DEFAULT_WAIT_NS if wait_limit_ns is None else int(wait_limit_ns),
+                          float(D ** -0.5 if scale is None else scale), Hq, T, int(bool(causal)), most)
         _call(lib.lvar_paged_attn, a, dev)
     return (o, M, L) if return_stats else o

@@ -58,7 +58,7 @@ def test_struct_mirrors_follow_the_header(name, mirror):
     text = (ROOT / "include" / "lvar_b200.h").read_text()
     start = text.index(f"typedef struct {name} {{") + len(f"typedef struct {name} {{")
     body = re.sub(r"/\*.*?\*/", "", text[start:text.index(f"}} {name};")], flags=re.S)
-    kinds = {"int64_t": C.c_int64, "int32_t": C.c_int32, "float": C.c_float, "lvar_paged_cache": _lib.PagedCache}
+    kinds = {"uint64_t": C.c_uint64, "int64_t": C.c_int64, "int32_t": C.c_int32, "float": C.c_float, "lvar_paged_cache": _lib.PagedCache}
     want = []
     for decl in filter(None, (d.strip() for d in body.split(";"))):
         first, *rest = decl.split(",")
