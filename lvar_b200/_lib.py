@@ -8,6 +8,7 @@ from __future__ import annotations
 import ctypes as C
 import os
 from pathlib import Path
+from struct import Struct
 
 LIB_PATH = Path(__file__).resolve().parent / "liblvar_b200.so"
 
@@ -111,6 +112,18 @@ class PagedAttnArgs(C.Structure):
     ]
 
 
+def packer(struct: type):
+    """The struct's fields in order (nested ones in place; 0 for a null pointer) -> its bytes, in one call.  A call takes the
+    bytes where it takes a pointer to the struct; they cost a quarter of filling a ``Structure``."""
+    codes = {C.c_void_p: "P", C.c_int64: "q", C.c_uint64: "Q", C.c_int32: "i", C.c_float: "f"}
+
+    def fmt(s):
+        return "".join(fmt(kind) if issubclass(kind, C.Structure) else codes[kind] for _, kind in s._fields_)
+    packed = Struct("@" + fmt(struct) + "0q")  # native alignment, whole multiples of 8 as in C
+    assert packed.size == C.sizeof(struct)
+    return packed.pack
+
+
 # name -> (restype, argtypes); every symbol the header declares is listed here and checked at load.
 _SIGNATURES = {
     "lvar_dense_attn": (C.c_int, [C.POINTER(AttnArgs), C.c_void_p]),
@@ -144,9 +157,9 @@ _SIGNATURES = {
                           [C.c_int32] * 5 + [C.c_void_p]),
     "lvar_upsample_ocache": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int64, C.c_int32, C.c_int32, C.c_int32] +
                              [C.c_int64] * 4 + [C.c_void_p]),
-    "lvar_paged_write": (C.c_int, [C.POINTER(PagedWriteArgs), C.c_void_p]),
-    "lvar_paged_read": (C.c_int, [C.POINTER(PagedReadArgs), C.c_void_p]),
-    "lvar_paged_attn": (C.c_int, [C.POINTER(PagedAttnArgs), C.c_void_p]),
+    "lvar_paged_write": (C.c_int, [C.c_void_p, C.c_void_p]),
+    "lvar_paged_read": (C.c_int, [C.c_void_p, C.c_void_p]),
+    "lvar_paged_attn": (C.c_int, [C.c_void_p, C.c_void_p]),
     "lvar_paged_attn_workspace": (C.c_int64, [C.c_int32] * 7),
     "lvar_last_error": (C.c_char_p, []),
     "lvar_version": (C.c_char_p, []),

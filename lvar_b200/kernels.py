@@ -6,13 +6,14 @@ launches on the current CUDA stream and returns without synchronising.  Nothing 
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import math
 from typing import Optional, Tuple
 
 import torch
 
 from . import _lib
-from ._lib import AttnArgs, PagedAttnArgs, PagedCache, PagedReadArgs, PagedWriteArgs, check, lib
+from ._lib import AttnArgs, check, lib
 
 
 _raw_stream = torch._C._cuda_getCurrentRawStream  # (device index) -> cudaStream_t of torch's current stream
@@ -674,59 +675,100 @@ def qkv_prologue(qkv: torch.Tensor, scale_mul: Optional[torch.Tensor], rope_cos:
 
 
 # -- paged key/value cache -------------------------------------------------------------------------
-def _paged_cache(k_pages, v_pages, table, scales) -> PagedCache:
-    """Checks the tensors of a paged cache and describes them for the C side."""
-    want = torch.bfloat16 if scales is None else torch.float8_e4m3fn
-    dev = k_pages.device
+# These calls serve steps of one token, where the host's share counts: a call makes one pass of cheap comparisons and packs
+# the C structure in one go; what it refuses is worked out in detail only then.
+_BF16, _E4M3, _I32, _F32, _U8 = torch.bfloat16, torch.float8_e4m3fn, torch.int32, torch.float32, torch.uint8
+_current_device = torch._C._cuda_getDevice
+_PACK_WRITE, _PACK_READ, _PACK_ATTN = _lib.packer(_lib.PagedWriteArgs), _lib.packer(_lib.PagedReadArgs), _lib.packer(_lib.PagedAttnArgs)
+
+
+def _refuse_cache(k_pages, v_pages, table, scales):
+    """Says what is wrong with a paged cache's tensors."""
     if not k_pages.is_cuda:
         raise RuntimeError("k_pages must be a CUDA tensor (lvar_b200 has no CPU path)")
+    want = _BF16 if scales is None else _E4M3
     if k_pages.dtype != want or v_pages.dtype != want:
         raise RuntimeError(f"k_pages and v_pages must be bfloat16, or float8_e4m3fn together with scales; got "
                            f"{k_pages.dtype}, {v_pages.dtype} and {'no ' if scales is None else ''}scales")
+    dev = k_pages.device
+    if k_pages.dim() != 4 or v_pages.shape != k_pages.shape or v_pages.device != dev:
+        raise RuntimeError(f"k_pages and v_pages must be [pages, kv heads, page_size, D] on one device, got "
+                           f"{tuple(k_pages.shape)} on {dev} and {tuple(v_pages.shape)} on {v_pages.device}")
+    if k_pages.stride(-1) != 1 or v_pages.stride(-1) != 1:
+        raise RuntimeError("k_pages and v_pages must have a contiguous last dimension")
+    if scales is not None and (scales.dtype != _U8 or scales.shape != (*k_pages.shape[:3], 2) or scales.device != dev or
+                               scales.stride(2) != 2 or scales.stride(3) != 1):
+        raise RuntimeError(f"scales must be a uint8 {[*k_pages.shape[:3], 2]} tensor on {dev}, contiguous in the last two "
+                           f"dimensions")
+    raise RuntimeError(f"table must be an int32 [B, pages per sequence] tensor on {dev} with a contiguous last dimension")
+
+
+def _paged_cache(k_pages, v_pages, table, scales):
+    """Checks the tensors of a paged cache: (fields of ``lvar_paged_cache`` in order, device index)."""
+    want = _BF16 if scales is None else _E4M3
+    dev = k_pages.get_device()  # -1: not a CUDA tensor
     shape = k_pages.shape
-    if len(shape) != 4 or v_pages.shape != shape or v_pages.device != dev:
-        raise RuntimeError(f"k_pages and v_pages must be [pages, kv heads, page_size, D] on one device, got {tuple(shape)} "
-                           f"and {tuple(v_pages.shape)}")
+    if (dev < 0 or len(shape) != 4 or k_pages.dtype is not want or v_pages.dtype is not want or v_pages.shape != shape or
+            v_pages.get_device() != dev or table.dtype is not _I32 or table.dim() != 2 or table.get_device() != dev):
+        _refuse_cache(k_pages, v_pages, table, scales)
+    n, H, size, D = shape
     k_sp, k_sh, k_sl, k_sd = k_pages.stride()
     v_sp, v_sh, v_sl, v_sd = v_pages.stride()
-    if k_sd != 1 or v_sd != 1:
-        raise RuntimeError("k_pages and v_pages must have a contiguous last dimension")
-    n, H, size, D = shape
-    if table.dtype != torch.int32 or table.dim() != 2 or table.device != dev or (table.shape[1] > 1 and table.stride(1) != 1):
-        raise RuntimeError(f"table must be an int32 [B, pages per sequence] tensor on {dev} with a contiguous last dimension")
-    s_ptr, s_sp, s_sh = None, 0, 0
+    B, per = table.shape
+    t_sb, t_sp = table.stride()
+    s_ptr = s_sp = s_sh = 0
+    ok = k_sd == 1 and v_sd == 1 and (t_sp == 1 or per <= 1)
     if scales is not None:
-        if scales.dtype != torch.uint8 or scales.shape != (n, H, size, 2) or scales.device != dev:
-            raise RuntimeError(f"scales must be a uint8 [{n}, {H}, {size}, 2] tensor on {dev}")
-        s_sp, s_sh, s_sl, s_sw = scales.stride()
-        if s_sl != 2 or s_sw != 1:
-            raise RuntimeError("scales must be contiguous in the last two dimensions")
+        ok = ok and scales.dtype is _U8 and scales.shape == (n, H, size, 2) and scales.get_device() == dev
+        if ok:
+            s_sp, s_sh, s_sl, s_sw = scales.stride()
+            ok = s_sl == 2 and s_sw == 1
         s_ptr = scales.data_ptr()
-    return PagedCache(k_pages.data_ptr(), k_sp, k_sh, k_sl, v_pages.data_ptr(), v_sp, v_sh, v_sl, s_ptr, s_sp, s_sh,
-                      table.data_ptr(), table.stride(0), n, size, H, D, table.shape[0], table.shape[1])
+    if not ok:
+        _refuse_cache(k_pages, v_pages, table, scales)
+    return (k_pages.data_ptr(), k_sp, k_sh, k_sl, v_pages.data_ptr(), v_sp, v_sh, v_sl, s_ptr, s_sp, s_sh, table.data_ptr(), t_sb,
+            n, size, H, D, B, per), dev
 
 
-def _require_ints(name: str, t: torch.Tensor, B: int, device) -> int:
-    if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != B or t.device != device or (B > 1 and t.stride(0) != 1):
-        raise RuntimeError(f"{name} must be a contiguous int32 tensor of {B} entries on {device}")
+def _paged_ints(name: str, t: torch.Tensor, B: int, dev: int) -> int:
+    if t.dtype is not _I32 or t.get_device() != dev or t.dim() != 1 or t.shape[0] != B or (B > 1 and t.stride(0) != 1):
+        raise RuntimeError(f"{name} must be a contiguous int32 tensor of {B} entries on cuda:{dev}")
     return t.data_ptr()
 
 
-def _status_ptr(status: Optional[torch.Tensor], device) -> Optional[int]:
+def _paged_floats(name: str, t: torch.Tensor, n: int, dev: int) -> int:
+    if t.dtype is not _F32 or t.get_device() != dev or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():
+        raise RuntimeError(f"{name} must be a contiguous float32 tensor of {n} entries on cuda:{dev}")
+    return t.data_ptr()
+
+
+def _paged_status(status: Optional[torch.Tensor], dev: int) -> int:
     if status is None:
-        return None
-    if status.dtype != torch.int32 or status.device != device:
-        raise RuntimeError(f"status must be an int32 tensor on {device}")
+        return 0
+    if status.dtype is not _I32 or status.get_device() != dev or status.numel() < 1:
+        raise RuntimeError(f"status must be an int32 tensor on cuda:{dev}")
     return status.data_ptr()
 
 
-def _call(fn, args, device: torch.device) -> None:
+def _paged_call(fn, args: bytes, dev: int) -> None:
     """Launches on the current stream of the tensors' device, whichever device is current."""
-    if device.index == torch.cuda.current_device():
-        check(fn(C.byref(args), _raw_stream(device.index)))
+    if dev == _current_device():
+        rc = fn(args, _raw_stream(dev))
     else:
-        with torch.cuda.device(device):
-            check(fn(C.byref(args), _raw_stream(device.index)))
+        with torch.cuda.device(dev):
+            rc = fn(args, _raw_stream(dev))
+    if rc:
+        check(rc)
+
+
+@functools.lru_cache(maxsize=4096)
+def _paged_workspace(dev: int, B: int, Hq: int, H: int, T: int, D: int, e4m3: bool, max_len: int) -> int:
+    """Workspace bytes of an attention call: a function of sizes and device."""
+    with torch.cuda.device(dev):
+        work = lib.lvar_paged_attn_workspace(B, Hq, H, T, D, int(e4m3), max_len)
+    if work < 0:
+        check(int(work))
+    return work
 
 
 def paged_kv_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor,
@@ -739,22 +781,24 @@ def paged_kv_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_p
     bf16, or float8_e4m3fn with ``scales`` uint8 [pages, H, page_size, 2]: the biased exponents of every row's power of two,
     K's and V's.  ``table`` int32 [B, n]: position p lies in page ``table[b, p // page_size]``.  ``start``, ``count``: int32
     [B] on the device.  A position without a page is not written and sets ``status`` (see :func:`new_status`)."""
-    _require_cuda_bf16("k", k)
-    _require_cuda_bf16("v", v)
-    B, H, L, D = k.shape
-    c = _paged_cache(k_pages, v_pages, table, scales)
-    if v.shape != k.shape or (H, D, B) != (c.Hkv, c.D, c.B) or k.device != k_pages.device or v.device != k.device:
-        raise RuntimeError(f"k and v must be [{c.B}, {c.Hkv}, L, {c.D}] on {k_pages.device}, got {tuple(k.shape)} and {tuple(v.shape)}")
-    dev = k.device
-    start_ptr = _require_ints("start", start, B, dev)
-    count_ptr = None if count is None else _require_ints("count", count, B, dev)
-    if B == 0 or L == 0:
-        return
-    k_sb, k_sh, k_sl, _ = k.stride()
-    v_sb, v_sh, v_sl, _ = v.stride()
-    a = PagedWriteArgs(c, None, 0, 0, 0, k.data_ptr(), k_sb, k_sl, k_sh, v.data_ptr(), v_sb, v_sl, v_sh, None, 0, 0, 0,
-                       start_ptr, count_ptr, None, None, None, None, None, _status_ptr(status, dev), 0.0, 0, 0, 0, L, 0)
-    _call(lib.lvar_paged_write, a, dev)
+    c, dev = _paged_cache(k_pages, v_pages, table, scales)
+    shape = k.shape
+    if (len(shape) != 4 or k.dtype is not _BF16 or v.dtype is not _BF16 or v.shape != shape or shape[0] != c[17] or
+            shape[1] != c[15] or shape[3] != c[16] or k.get_device() != dev or v.get_device() != dev):
+        raise RuntimeError(f"k and v must be bfloat16 [{c[17]}, {c[15]}, L, {c[16]}] tensors on cuda:{dev}, got {tuple(shape)} "
+                           f"and {tuple(v.shape)}")
+    B, _, L, _ = shape
+    k_sb, k_sh, k_sl, k_sd = k.stride()
+    v_sb, v_sh, v_sl, v_sd = v.stride()
+    if k_sd != 1 or v_sd != 1:
+        raise RuntimeError("k and v must have a contiguous last dimension")
+    start_ptr = _paged_ints("start", start, B, dev)
+    count_ptr = 0 if count is None else _paged_ints("count", count, B, dev)
+    st = _paged_status(status, dev)
+    if B and L:
+        _paged_call(lib.lvar_paged_write,
+                    _PACK_WRITE(*c, 0, 0, 0, 0, k.data_ptr(), k_sb, k_sl, k_sh, v.data_ptr(), v_sb, v_sl, v_sh, 0, 0, 0, 0,
+                                start_ptr, count_ptr, 0, 0, 0, 0, 0, st, 0.0, 0, 0, 0, L, 0), dev)
 
 
 def paged_qkv_prologue(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
@@ -772,56 +816,53 @@ def paged_qkv_prologue(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_page
     ``rope_cos``, ``rope_sin`` fp32 [P, D/2]: row p rotates the token at cache position p, element pairs (2i, 2i + 1), or
     (i, i + D/2) with ``rope_halves``.  The cache arguments, ``start``, ``count`` and ``status`` are those of
     :func:`paged_kv_append`; q rows of padding are 0."""
-    for n, t in (("q", q), ("k", k), ("v", v)):
-        _require_cuda_bf16(n, t)
-    B, L, Hq, D = q.shape
-    c = _paged_cache(k_pages, v_pages, table, scales)
-    dev = q.device
-    if k.shape != v.shape or k.shape != (B, L, c.Hkv, D) or D != c.D or B != c.B or dev != k_pages.device or k.device != dev \
-            or v.device != dev:
-        raise RuntimeError(f"q must be [{c.B}, L, Hq, {c.D}] and k, v [{c.B}, L, {c.Hkv}, {c.D}] on {k_pages.device}, got "
-                           f"{tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
-    if Hq == 0 or Hq % c.Hkv:
-        raise RuntimeError(f"query heads must be a multiple of the cache's heads (got {Hq} and {c.Hkv})")
-    norm = 0
-    sm_ptr = qw_ptr = kw_ptr = cos_ptr = sin_ptr = None
+    c, dev = _paged_cache(k_pages, v_pages, table, scales)
+    shape, kshape = q.shape, k.shape
+    if (len(shape) != 4 or q.dtype is not _BF16 or k.dtype is not _BF16 or v.dtype is not _BF16 or v.shape != kshape or
+            len(kshape) != 4 or shape[0] != c[17] or shape[3] != c[16] or kshape[0] != c[17] or kshape[1] != shape[1] or
+            kshape[2] != c[15] or kshape[3] != c[16] or q.get_device() != dev or k.get_device() != dev or v.get_device() != dev):
+        raise RuntimeError(f"q must be a bfloat16 [{c[17]}, L, Hq, {c[16]}] tensor and k, v bfloat16 [{c[17]}, L, {c[15]}, {c[16]}] "
+                           f"tensors on cuda:{dev}, got {tuple(shape)}, {tuple(kshape)} and {tuple(v.shape)}")
+    B, L, Hq, D = shape
+    if Hq == 0 or Hq % c[15]:
+        raise RuntimeError(f"query heads must be a multiple of the cache's heads (got {Hq} and {c[15]})")
+    q_sb, q_sl, q_sh, q_sd = q.stride()
+    k_sb, k_sl, k_sh, k_sd = k.stride()
+    v_sb, v_sl, v_sh, v_sd = v.stride()
+    if q_sd != 1 or k_sd != 1 or v_sd != 1:
+        raise RuntimeError("q, k and v must have a contiguous last dimension")
+    norm = sm_ptr = qw_ptr = kw_ptr = cos_ptr = sin_ptr = rope_rows = 0
     if scale_mul is not None:
         if eps is not None or q_weight is not None or k_weight is not None:
             raise RuntimeError("scale_mul (L2 norm) excludes eps, q_weight and k_weight (root-mean-square norm)")
-        if scale_mul.dtype != torch.float32 or scale_mul.shape != (Hq,) or scale_mul.device != dev \
-                or not scale_mul.is_contiguous():
-            raise RuntimeError(f"scale_mul must be a contiguous float32 tensor of {Hq} entries on {dev}")
-        norm, sm_ptr = 1, scale_mul.data_ptr()
+        norm, sm_ptr = 1, _paged_floats("scale_mul", scale_mul, Hq, dev)
     elif eps is not None:
         norm = 2
-        for n, t in (("q_weight", q_weight), ("k_weight", k_weight)):
-            if t is not None and (t.dtype != torch.float32 or t.shape != (D,) or t.device != dev or not t.is_contiguous()):
-                raise RuntimeError(f"{n} must be a contiguous float32 tensor of {D} entries on {dev}")
-        qw_ptr = None if q_weight is None else q_weight.data_ptr()
-        kw_ptr = None if k_weight is None else k_weight.data_ptr()
+        if q_weight is not None:
+            qw_ptr = _paged_floats("q_weight", q_weight, D, dev)
+        if k_weight is not None:
+            kw_ptr = _paged_floats("k_weight", k_weight, D, dev)
     elif q_weight is not None or k_weight is not None:
         raise RuntimeError("q_weight and k_weight belong to the root-mean-square norm, which takes eps")
-    rope_rows = 0
-    if (rope_cos is None) != (rope_sin is None):
+    if rope_cos is not None and rope_sin is not None:
+        tables = rope_cos.shape
+        if (len(tables) != 2 or tables[1] != D // 2 or rope_sin.shape != tables or rope_cos.dtype is not _F32 or
+                rope_sin.dtype is not _F32 or rope_cos.get_device() != dev or rope_sin.get_device() != dev or
+                not rope_cos.is_contiguous() or not rope_sin.is_contiguous()):
+            raise RuntimeError(f"rope_cos and rope_sin must be contiguous float32 [P, {D // 2}] tensors on cuda:{dev}")
+        rope_rows, cos_ptr, sin_ptr = tables[0], rope_cos.data_ptr(), rope_sin.data_ptr()
+    elif rope_cos is not None or rope_sin is not None:
         raise RuntimeError("rope_cos and rope_sin go together")
-    if rope_cos is not None:
-        for t in (rope_cos, rope_sin):
-            if t.dtype != torch.float32 or t.dim() != 2 or t.shape[1] != D // 2 or t.device != dev or not t.is_contiguous() \
-                    or t.shape[0] != rope_cos.shape[0]:
-                raise RuntimeError(f"rope tables must be contiguous float32 [P, {D // 2}] tensors on {dev}")
-        rope_rows, cos_ptr, sin_ptr = rope_cos.shape[0], rope_cos.data_ptr(), rope_sin.data_ptr()
-    start_ptr = _require_ints("start", start, B, dev)
-    count_ptr = None if count is None else _require_ints("count", count, B, dev)
-    out = torch.empty((B, Hq, L, D), dtype=torch.bfloat16, device=dev)
-    if B == 0 or L == 0:
-        return out
-    q_sb, q_sl, q_sh, _ = q.stride()
-    k_sb, k_sl, k_sh, _ = k.stride()
-    v_sb, v_sl, v_sh, _ = v.stride()
-    a = PagedWriteArgs(c, q.data_ptr(), q_sb, q_sl, q_sh, k.data_ptr(), k_sb, k_sl, k_sh, v.data_ptr(), v_sb, v_sl, v_sh,
-                       out.data_ptr(), Hq * L * D, L * D, D, start_ptr, count_ptr, sm_ptr, qw_ptr, kw_ptr, cos_ptr, sin_ptr,
-                       _status_ptr(status, dev), 0.0 if eps is None else float(eps), norm, int(rope_halves), rope_rows, L, Hq)
-    _call(lib.lvar_paged_write, a, dev)
+    start_ptr = _paged_ints("start", start, B, dev)
+    count_ptr = 0 if count is None else _paged_ints("count", count, B, dev)
+    st = _paged_status(status, dev)
+    out = torch.empty((B, Hq, L, D), dtype=_BF16, device=q.device)
+    if B and L:
+        _paged_call(lib.lvar_paged_write,
+                    _PACK_WRITE(*c, q.data_ptr(), q_sb, q_sl, q_sh, k.data_ptr(), k_sb, k_sl, k_sh, v.data_ptr(), v_sb, v_sl,
+                                v_sh, out.data_ptr(), Hq * L * D, L * D, D, start_ptr, count_ptr, sm_ptr, qw_ptr, kw_ptr,
+                                cos_ptr, sin_ptr, st, 0.0 if eps is None else eps, norm, 1 if rope_halves else 0, rope_rows, L,
+                                Hq), dev)
     return out
 
 
@@ -833,25 +874,25 @@ def paged_kv_read(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Ten
     rows at or behind ``lens[b]`` (int32 [B] on the device): the contiguous tensors that the many-query attention calls
     take.  ``out``: an optional pair of destinations (bf16, unit stride along D, other strides in multiples of 8).  An e4m3
     row comes back exactly as the values it stands for.  The cache arguments are those of :func:`paged_kv_append`."""
-    c = _paged_cache(k_pages, v_pages, table, scales)
-    dev = k_pages.device
-    shape = (c.B, c.Hkv, int(n), c.D)
+    c, dev = _paged_cache(k_pages, v_pages, table, scales)
+    B, n = c[17], int(n)
+    shape = (B, c[15], n, c[16])
+    lens_ptr = _paged_ints("lens", lens, B, dev)
+    st = _paged_status(status, dev)
     if out is None:
-        out = (torch.empty(shape, dtype=torch.bfloat16, device=dev), torch.empty(shape, dtype=torch.bfloat16, device=dev))
+        k = torch.empty(shape, dtype=_BF16, device=k_pages.device)
+        v = torch.empty_like(k)
     else:
-        for name, t in zip(("k", "v"), out):
-            _require_cuda_bf16(name, t)
-            if t.shape != shape or t.device != dev:
-                raise RuntimeError(f"out must hold bfloat16 tensors of shape {shape} on {dev}, got {tuple(t.shape)}")
-    k, v = out
-    lens_ptr = _require_ints("lens", lens, c.B, dev)
-    if c.B == 0 or n == 0:
-        return k, v
-    k_sb, k_sh, k_sl, _ = k.stride()
-    v_sb, v_sh, v_sl, _ = v.stride()
-    a = PagedReadArgs(c, k.data_ptr(), k_sb, k_sh, k_sl, v.data_ptr(), v_sb, v_sh, v_sl, lens_ptr, _status_ptr(status, dev),
-                      int(start), int(n))
-    _call(lib.lvar_paged_read, a, dev)
+        k, v = out
+        for t in out:
+            if t.shape != shape or t.dtype is not _BF16 or t.get_device() != dev or t.stride(-1) != 1:
+                raise RuntimeError(f"out must hold bfloat16 tensors of shape {shape} on cuda:{dev} with a contiguous last "
+                                   f"dimension, got {tuple(t.shape)}")
+    if B and n:
+        k_sb, k_sh, k_sl, _ = k.stride()
+        v_sb, v_sh, v_sl, _ = v.stride()
+        _paged_call(lib.lvar_paged_read, _PACK_READ(*c, k.data_ptr(), k_sb, k_sh, k_sl, v.data_ptr(), v_sb, v_sh, v_sl, lens_ptr,
+                                                    st, int(start), n), dev)
     return k, v
 
 
@@ -869,35 +910,39 @@ def paged_attn_fwd(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
     A row that sees no key is 0 (M = -inf, L = 0).  ``max_len``: a bound on the lengths that shapes the launch (default: what
     the table holds); a longer sequence is cut there and sets ``status``.  ``out``: see :func:`_output_like`.  The cache
     arguments are those of :func:`paged_kv_append`."""
-    _require_cuda_bf16("q", q)
-    B, Hq, T, D = q.shape
-    c = _paged_cache(k_pages, v_pages, table, scales)
-    dev = q.device
-    if B != c.B or D != c.D or dev != k_pages.device:
-        raise RuntimeError(f"q must be [{c.B}, Hq, T, {c.D}] on {k_pages.device}, got {tuple(q.shape)}")
-    if Hq == 0 or Hq % c.Hkv:
-        raise RuntimeError(f"query heads must be a multiple of the cache's heads (got {Hq} and {c.Hkv})")
-    lens_ptr = _require_ints("lens", lens, B, dev)
-    room = c.max_pages * c.page_size
-    most = min(room, 1 << 30) if max_len is None else int(max_len)
-    o = _output_like(q, out)
+    c, dev = _paged_cache(k_pages, v_pages, table, scales)
+    shape = q.shape
+    if (len(shape) != 4 or q.dtype is not _BF16 or shape[0] != c[17] or shape[3] != c[16] or q.get_device() != dev):
+        raise RuntimeError(f"q must be a bfloat16 [{c[17]}, Hq, T, {c[16]}] tensor on cuda:{dev}, got {tuple(shape)}")
+    B, Hq, T, D = shape
+    H = c[15]
+    if Hq == 0 or Hq % H:
+        raise RuntimeError(f"query heads must be a multiple of the cache's heads (got {Hq} and {H})")
+    q_sb, q_sh, q_sl, q_sd = q.stride()
+    if q_sd != 1:
+        raise RuntimeError("q must have a contiguous last dimension")
+    lens_ptr = _paged_ints("lens", lens, B, dev)
+    st = _paged_status(status, dev)
+    most = min(c[18] * c[14], 1 << 30) if max_len is None else int(max_len)
+    if out is None:
+        o = torch.empty((B, Hq, T, D), dtype=_BF16, device=q.device)
+        o_sb, o_sh, o_sl = Hq * T * D, T * D, D
+    else:
+        o = _output_like(q, out)
+        o_sb, o_sh, o_sl, _ = o.stride()
     M = L = None
-    m_ptr = l_ptr = None
+    m_ptr = l_ptr = w_ptr = 0
     if return_stats:
-        M = torch.empty((B, Hq, T), dtype=torch.float32, device=dev)
-        L = torch.empty((B, Hq, T), dtype=torch.float32, device=dev)
+        M = torch.empty((B, Hq, T), dtype=_F32, device=q.device)
+        L = torch.empty_like(M)
         m_ptr, l_ptr = M.data_ptr(), L.data_ptr()
     if B and T:
-        work, w_ptr = lib.lvar_paged_attn_workspace(B, Hq, c.Hkv, T, D, int(scales is not None), most), None
-        if work < 0:
-            check(int(work))
+        work = _paged_workspace(dev, B, Hq, H, T, D, scales is not None, most)
         if work:
-            space = torch.empty(work, dtype=torch.uint8, device=dev)
+            space = torch.empty(work, dtype=_U8, device=q.device)
             w_ptr = space.data_ptr()
-        q_sb, q_sh, q_sl, _ = q.stride()
-        o_sb, o_sh, o_sl, _ = o.stride()
-        a = PagedAttnArgs(c, q.data_ptr(), q_sb, q_sh, q_sl, o.data_ptr(), o_sb, o_sh, o_sl, m_ptr, l_ptr, lens_ptr, w_ptr, work,
-                          _status_ptr(status, dev), _lib.DEFAULT_WAIT_NS if wait_limit_ns is None else int(wait_limit_ns),
-                          float(D ** -0.5 if scale is None else scale), Hq, T, int(bool(causal)), most)
-        _call(lib.lvar_paged_attn, a, dev)
+        _paged_call(lib.lvar_paged_attn,
+                    _PACK_ATTN(*c, q.data_ptr(), q_sb, q_sh, q_sl, o.data_ptr(), o_sb, o_sh, o_sl, m_ptr, l_ptr, lens_ptr, w_ptr,
+                               work, st, _lib.DEFAULT_WAIT_NS if wait_limit_ns is None else int(wait_limit_ns),
+                               D ** -0.5 if scale is None else scale, Hq, T, 1 if causal else 0, most), dev)
     return (o, M, L) if return_stats else o

@@ -67,6 +67,26 @@ def test_struct_mirrors_follow_the_header(name, mirror):
     assert want == [tuple(f) for f in getattr(_lib, mirror)._fields_]
 
 
+@pytest.mark.parametrize("mirror", ["PagedWriteArgs", "PagedReadArgs", "PagedAttnArgs"])
+def test_packed_bytes_are_the_struct(mirror):
+    from lvar_b200 import _lib
+    kind = getattr(_lib, mirror)
+
+    def leaves(s):
+        for name, k in s._fields_:
+            yield from leaves(k) if issubclass(k, C.Structure) else [k]
+    kinds = list(leaves(kind))
+    values = [0.5 * i if k is C.c_float else i + 1 for i, k in enumerate(kinds)]
+    data = _lib.packer(kind)(*values)
+    back = kind.from_buffer_copy(data)
+
+    def read(s):
+        for name, k in s._fields_:
+            x = getattr(s, name)
+            yield from read(x) if isinstance(x, C.Structure) else [x]
+    assert list(read(back)) == values
+
+
 def test_page_division_is_exact():
     """The kernels divide a group of 16 rows by the groups per page with one multiplication."""
     g = torch.Generator().manual_seed(2)
