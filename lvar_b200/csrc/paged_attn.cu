@@ -36,8 +36,8 @@ namespace lvar {
 
 namespace {
 
-constexpr int kThreads = 128;               // threads that compute
-constexpr int kAllThreads = kThreads + 32;  // and the loader
+constexpr int kThreads = 128;     // threads that compute: a warpgroup
+constexpr int kAllThreads = 256;  // and one whose first warp loads; its registers go to the first
 constexpr int kSlotsPerCta = 2;
 
 struct PagedAttnParams {
@@ -80,9 +80,17 @@ __device__ __forceinline__ uint4 lds128(uint32_t addr) {
   asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
   return v;
 }
+__device__ __forceinline__ void sts128(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
 __device__ __forceinline__ uint2 lds64(uint32_t addr) {
   uint2 v;
   asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr));
+  return v;
+}
+__device__ __forceinline__ uint32_t lds16(uint32_t addr) {
+  uint16_t v;
+  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(addr));
   return v;
 }
 __device__ __forceinline__ uint32_t lds32(uint32_t addr) {
@@ -105,6 +113,12 @@ __device__ __forceinline__ void widen4(uint32_t four, uint32_t& lo, uint32_t& hi
   asm("{\n.reg .b16 a, b;\nmov.b32 {a, b}, %2;\ncvt.rn.f16x2.e4m3x2 %0, a;\ncvt.rn.f16x2.e4m3x2 %1, b;\n}"
       : "=r"(lo), "=r"(hi) : "r"(four));
 }
+// Transposes an 8 x 8 matrix of 16-bit elements held as an accumulator's rows.
+__device__ __forceinline__ uint32_t transpose8(uint32_t a) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(a));
+  return r;
+}
 __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
   uint32_t r;
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
@@ -112,20 +126,33 @@ __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
 }
 __device__ __forceinline__ float pow2i(int e) { return __int_as_float((e + 127) << 23); }  // -126 <= e <= 127
 
-template <int D, bool Q8>
+// CTAs per SM: two; three of smaller tiles' worth where a warp's state is small and a key's bytes are few.
+__host__ __device__ constexpr int ctas_per_sm(int D, bool q8, int nb) { return D == 64 && q8 && nb == 1 ? 3 : 2; }
+__host__ __device__ constexpr int keys_per_tile(int D, bool q8, int wr) { return D == 64 || (q8 && wr == 1) ? 128 : 64; }
+
+template <int D, bool Q8, int NB, int WR>
 struct Geo {
+  static constexpr bool WIDE = Q8 && WR > 1;              // tiles are widened to fp16 once for the warps that share them
   static constexpr int RB = D * (Q8 ? 1 : 2);             // bytes of a cached row
   static constexpr int RS = RB < 128 ? RB : 128;          // bytes of a row of a sub-tile, the widest that a copy swizzles
   static constexpr int SUBS = RB / RS;                    // sub-tiles side by side
-  static constexpr int KT = Q8 || D == 64 ? 128 : 64;     // keys per tile
+  static constexpr int KT = keys_per_tile(D, Q8, WR);     // keys per tile
   static constexpr int SUB = KT * RS;                     // bytes of a sub-tile
   static constexpr int STAGE = 2 * KT * RB;               // K and V
-  static constexpr int STAGES = STAGE <= 16384 ? 6 : 3;
+  static constexpr int CTAS = ctas_per_sm(D, Q8, NB);     // per SM
+  static constexpr int LAUNCH_REGS = CTAS == 3 ? 80 : 128;
+  static constexpr int COMPUTE_REGS = 2 * LAUNCH_REGS - 24;
+  static constexpr int STAGES = WIDE ? 65536 / STAGE : (CTAS == 3 ? 65536 : 98304) / STAGE;
   static constexpr int SCALE_STAGE = Q8 ? KT * 2 : 0;
-  static constexpr int RING = STAGES * (STAGE + SCALE_STAGE);
-  static constexpr int ML = 4 * 16 * 2 * 4;               // maxima and sums of the four warps' rows
+  static constexpr int WIDE_BYTES = WIDE ? 2 * KT * D * 2 : 0;
+  static constexpr int RING = STAGES * (STAGE + SCALE_STAGE) + WIDE_BYTES;
+  // what the matrix instructions' operands are read from: rows of 16-bit elements in sub-tiles of 128 bytes, or the stage
+  static constexpr int OS = WIDE ? 128 : RS, OSUB = KT * OS;
+  static constexpr int RW = 8 * NB;                       // rows per warp
+  static constexpr int RC = RW * WR;                      // rows per CTA
+  static constexpr int ML = 4 * RW * 2 * 4;               // maxima and sums of the four warps' rows
   static constexpr int SMEM = RING + ML + 64 + 2 * STAGES * 8 + 16 + 1024;  // and the start's alignment
-  static_assert(4 * 16 * D * 4 <= STAGE, "the warps' accumulators are joined in a consumed stage");
+  static_assert(4 * RW * D * 4 <= (WIDE ? WIDE_BYTES : STAGE), "the warps' accumulators are joined in a consumed tile");
 };
 
 // The swizzle of a sub-tile's row: what its 16-byte chunk numbers are XORed with (as the copies do).
@@ -226,19 +253,24 @@ __device__ __forceinline__ void advance(const PagedAttnParams& p, Cursor& c) {
   }
 }
 
-// One warp's running state over an item: two rows per thread (lane / 4 and + 8).
-template <int D>
+// One warp's running state over an item.  Rows lie along the matrix instruction's 8 columns: a thread has the two rows
+// 2 (lane mod 4) + {0, 1} of every block of 8, and of D the elements that element_of() gives.
+template <int D, int NB>
 struct State {
-  float acc[D / 8][4];
-  float m[2], l[2];  // maximum of the scores (log2 units) and sum of exp2(s - m), per thread
-  float mt[2];       // e4m3: maximum of score + V exponent, which the accumulators are relative to
+  float acc[D / 16][NB][4];  // [0], [1]: the two rows at a tile's first element of D, [2], [3]: at its second
+  float m[NB][2], l[NB][2];  // maximum of the scores (log2 units) and this thread's part of the sum of exp2(s - m)
+  float mt[NB][2];           // e4m3: maximum of score + V exponent, which the accumulators are relative to
 };
+template <int D, bool RAW8>
+__device__ __forceinline__ int element_of(int tile, int second) {
+  const int g = (threadIdx.x & 31) >> 2;
+  return RAW8 ? g * (D / 8) + 2 * tile + second : tile * 16 + 8 * second + g;
+}
 
 // Fetches the tiles of a CTA's range, `nt` from `cur` on, into the ring.
-template <int D, bool Q8>
+template <class X, int D, bool Q8>
 __device__ __forceinline__ void loader(const CUtensorMap& mk, const CUtensorMap& mv, const PagedAttnParams& p, Cursor cur, int nt,
                                        uint8_t* ring, uint64_t* full, uint64_t* empty, const WaitCtx& w) {
-  using X = Geo<D, Q8>;
   const int lane = threadIdx.x & 31;
   const uint32_t box_bytes = (uint32_t)p.box * (2 * X::RB + (Q8 ? 2 : 0));
   int stage = 0, issued = 0;
@@ -283,38 +315,41 @@ __device__ __forceinline__ void loader(const CUtensorMap& mk, const CUtensorMap&
   }
 }
 
-// O += P V of one step, 16 keys at a time.  CLEAN: elements of V that are not finite are left out.
-template <int D, bool Q8, int NT, bool CLEAN>
-__device__ __forceinline__ void weigh(State<D>& st, const float (&sc)[NT][4], uint32_t vs, int s0) {
-  using X = Geo<D, Q8>;
+// O^T += V^T P^T of one step, 16 keys at a time.  CLEAN: elements of V that are not finite are left out.
+template <class X, int D, bool Q8, int NB, int NK, bool CLEAN>
+__device__ __forceinline__ void weigh(State<D, NB>& st, const float (&sc)[NK][NB][4], uint32_t vs, int s0) {
   const int lane = threadIdx.x & 31, quad = lane & 3;
 #pragma unroll
-  for (int n2 = 0; n2 < NT / 2; ++n2) {
-    if constexpr (!Q8) {
-      const uint32_t a[4] = {pack_bf16x2(sc[2 * n2][0], sc[2 * n2][1]), pack_bf16x2(sc[2 * n2][2], sc[2 * n2][3]),
-                             pack_bf16x2(sc[2 * n2 + 1][0], sc[2 * n2 + 1][1]),
-                             pack_bf16x2(sc[2 * n2 + 1][2], sc[2 * n2 + 1][3])};
-      const uint32_t v0 = vs + (s0 + n2 * 16 + (lane & 15)) * X::RS + (((lane >> 4) ^ (lane & 7)) << 4);
+  for (int k = 0; k < NK; ++k) {
+    uint32_t b[NB][2];
 #pragma unroll
-      for (int d2 = 0; d2 < D / 16; ++d2) {
-        uint32_t b[4];
-        ldsm_x4_t((v0 ^ ((d2 & 3) << 5)) + (d2 >> 2) * X::SUB, b);
+    for (int nb = 0; nb < NB; ++nb) {
+      b[nb][0] = transpose8(Q8 ? pack_f16x2(sc[k][nb][0], sc[k][nb][1]) : pack_bf16x2(sc[k][nb][0], sc[k][nb][1]));
+      b[nb][1] = transpose8(Q8 ? pack_f16x2(sc[k][nb][2], sc[k][nb][3]) : pack_bf16x2(sc[k][nb][2], sc[k][nb][3]));
+    }
+    if constexpr (!Q8 || X::WIDE) {
+      const uint32_t v0 = vs + (s0 + k * 16 + (lane & 7) + ((lane >> 4) << 3)) * X::OS + ((((lane >> 3) & 1) ^ (lane & 7)) << 4);
+      constexpr uint32_t kOdd = Q8 ? 0x7c00u : 0x7f80u;  // the exponent of an element that is not finite
+#pragma unroll
+      for (int t = 0; t < D / 16; ++t) {
+        uint32_t a[4];
+        ldsm_x4_t((v0 ^ ((t & 3) << 5)) + (t >> 2) * X::OSUB, a);
         if constexpr (CLEAN) {
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            if ((b[j] & 0x7f80u) == 0x7f80u) b[j] &= 0xffff0000u;
-            if ((b[j] & 0x7f800000u) == 0x7f800000u) b[j] &= 0xffffu;
+            if ((a[j] & kOdd) == kOdd) a[j] &= 0xffff0000u;
+            if ((a[j] & (kOdd << 16)) == kOdd << 16) a[j] &= 0xffffu;
           }
         }
-        mma_bf16(st.acc[d2 * 2], a, b[0], b[1]);
-        mma_bf16(st.acc[d2 * 2 + 1], a, b[2], b[3]);
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+          if constexpr (Q8) mma_f16(st.acc[t][nb], a, b[nb][0], b[nb][1]);
+          else mma_bf16(st.acc[t][nb], a, b[nb][0], b[nb][1]);
+        }
       }
     } else {
-      const uint32_t a[4] = {pack_f16x2(sc[2 * n2][0], sc[2 * n2][1]), pack_f16x2(sc[2 * n2][2], sc[2 * n2][3]),
-                             pack_f16x2(sc[2 * n2 + 1][0], sc[2 * n2 + 1][1]),
-                             pack_f16x2(sc[2 * n2 + 1][2], sc[2 * n2 + 1][3])};
       constexpr int W = D / 32;  // words per thread and key: D / 8 consecutive elements, lane / 4 says which
-      const uint32_t r0 = vs + (s0 + n2 * 16 + quad * 2) * X::RS;
+      const uint32_t r0 = vs + (s0 + k * 16 + quad * 2) * X::RS;
       uint32_t u[4][W];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {  // keys 2 quad, 2 quad + 1, and both + 8
@@ -336,22 +371,23 @@ __device__ __forceinline__ void weigh(State<D>& st, const float (&sc)[NT][4], ui
       }
 #pragma unroll
       for (int i = 0; i < W; ++i) {
-        uint32_t b[4][2];
-        widen4(__byte_perm(u[0][i], u[1][i], 0x5140), b[0][0], b[1][0]);
-        widen4(__byte_perm(u[0][i], u[1][i], 0x7362), b[2][0], b[3][0]);
-        widen4(__byte_perm(u[2][i], u[3][i], 0x5140), b[0][1], b[1][1]);
-        widen4(__byte_perm(u[2][i], u[3][i], 0x7362), b[2][1], b[3][1]);
+        uint32_t a[2][4];
+        widen4(__byte_perm(u[0][i], u[1][i], 0x5140), a[0][0], a[0][1]);
+        widen4(__byte_perm(u[0][i], u[1][i], 0x7362), a[1][0], a[1][1]);
+        widen4(__byte_perm(u[2][i], u[3][i], 0x5140), a[0][2], a[0][3]);
+        widen4(__byte_perm(u[2][i], u[3][i], 0x7362), a[1][2], a[1][3]);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) mma_f16(st.acc[i * 4 + j], a, b[j][0], b[j][1]);
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb) mma_f16(st.acc[i * 2 + j][nb], a[j], b[nb][0], b[nb][1]);
       }
     }
   }
 }
 
 // Whether any of a step's V elements is not finite; by the whole warp.
-template <int D, bool Q8, int NS>
+template <class X, bool Q8, int NS>
 __device__ __forceinline__ bool any_odd(uint32_t vs, int s0) {
-  using X = Geo<D, Q8>;
   const int lane = threadIdx.x & 31;
   uint32_t hit = 0;
 #pragma unroll
@@ -369,38 +405,49 @@ __device__ __forceinline__ bool any_odd(uint32_t vs, int s0) {
 }
 
 // The elements of V that CLEAN left out, row by row: a row takes those that it sees.
-template <int D, bool Q8, int NT>
-__device__ __noinline__ void weigh_odd(State<D>& st, const float (&sc)[NT][4], uint32_t vs, int s0, int seen0, int seen1) {
-  using X = Geo<D, Q8>;
-  const int lane = threadIdx.x & 31, quad = lane & 3;
-  for (int j = 0; j < NT * 8; ++j) {
-    const int from = (lane & 28) | ((j & 7) >> 1);  // the lane of the quad that has this row pair's weights of key j
-    const float w0 = __shfl_sync(0xffffffffu, sc[j >> 3][j & 1], from);
-    const float w1 = __shfl_sync(0xffffffffu, sc[j >> 3][2 + (j & 1)], from);
-    const int row = s0 + j;
-    for (int n = 0; n < D / 8; ++n)
+template <class X, int D, bool Q8, int NB, int NK>
+__device__ __noinline__ void weigh_odd(State<D, NB>& st, const float (&sc)[NK][NB][4], const int (&seen)[NB][2], uint32_t vs,
+                                       int s0) {
+  const int quad = threadIdx.x & 3;
+  for (int j = 0; j < NK * 16; ++j) {
+    const int row = s0 + j, from = ((j & 7) << 2) | quad;  // the lane that has these rows' weights of key j
+    for (int nb = 0; nb < NB; ++nb)
       for (int e = 0; e < 2; ++e) {
-        const int d = Q8 ? (quad * 2 + e) * (D / 8) + n : n * 8 + quad * 2 + e;
-        const int byte = d * (Q8 ? 1 : 2), chunk = (byte % X::RS) >> 4;
-        const uint32_t at = vs + byte / X::RS * X::SUB + row * X::RS + ((chunk ^ swizzle_of<X::RS>(row)) << 4) + (byte & 15);
-        const uint32_t bits = lds32(at & ~3u) >> ((at & 3u) * 8);
-        const float val = Q8 ? NAN : __uint_as_float(bits << 16);
-        const bool odd = Q8 ? (bits & 0x7fu) == 0x7fu : (bits & 0x7f80u) == 0x7f80u;
-        if (odd && j < seen0) st.acc[n][e] = fmaf(w0, val, st.acc[n][e]);
-        if (odd && j < seen1) st.acc[n][e + 2] = fmaf(w1, val, st.acc[n][e + 2]);
+        const float w = __shfl_sync(0xffffffffu, sc[j >> 4][nb][((j >> 3) & 1) * 2 + e], from);
+        for (int t = 0; t < D / 16; ++t)
+          for (int second = 0; second < 2; ++second) {
+            const int byte = element_of<D, Q8 && !X::WIDE>(t, second) * (Q8 ? 1 : 2), chunk = (byte % X::RS) >> 4;
+            const uint32_t at = vs + byte / X::RS * X::SUB + row * X::RS + ((chunk ^ swizzle_of<X::RS>(row)) << 4) + (byte & 15);
+            const uint32_t bits = lds32(at & ~3u) >> ((at & 3u) * 8);
+            const float val = Q8 ? NAN : __uint_as_float(bits << 16);
+            const bool odd = Q8 ? (bits & 0x7fu) == 0x7fu : (bits & 0x7f80u) == 0x7f80u;
+            float& acc = st.acc[t][nb][second * 2 + e];
+            if (odd && j < seen[nb][e]) acc = fmaf(w, val, acc);
+          }
       }
   }
 }
 
-template <int D, bool Q8, int WR>
-__global__ void __launch_bounds__(kAllThreads, 2)
+__device__ __forceinline__ float max_of_keys(float x) {  // over the eight lanes that have the same rows
+  x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+  x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+  return fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+}
+__device__ __forceinline__ float sum_of_keys(float x) {
+  x += __shfl_xor_sync(0xffffffffu, x, 4);
+  x += __shfl_xor_sync(0xffffffffu, x, 8);
+  return x + __shfl_xor_sync(0xffffffffu, x, 16);
+}
+
+template <int D, bool Q8, int NB, int WR>
+__global__ void __launch_bounds__(kAllThreads, (Geo<D, Q8, NB, WR>::CTAS))
     paged_attn_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
                       const __grid_constant__ PagedAttnParams p) {
-  using X = Geo<D, Q8>;
+  using X = Geo<D, Q8, NB, WR>;
   constexpr int WK = 4 / WR;              // warps that share a row tile and differ in their keys
   constexpr int KW = X::KT / WK;          // keys of a tile per warp
   constexpr int NS = KW < 32 ? KW : 32;   // keys per step
-  constexpr int NT = NS / 8;
+  constexpr int NK = NS / 16;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const uint32_t ring = smem_u32(smem);
@@ -410,7 +457,7 @@ __global__ void __launch_bounds__(kAllThreads, 2)
   uint64_t* empty = full + X::STAGES;
   int* abort_flag = reinterpret_cast<int*>(empty + X::STAGES);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int wr = warp % WR, wk = warp / WR, quad = lane & 3;
+  const int wr = warp % WR, wk = warp / WR, quad = lane & 3, g8 = lane >> 2;
   const WaitCtx wait{p.status, abort_flag, p.wait_limit_ns};
 
   if (tid == 0) {
@@ -447,16 +494,18 @@ __global__ void __launch_bounds__(kAllThreads, 2)
     cons.len = length_of(p, cons.b);
     cons.ntile = nt = tiles_of<X::KT>(cons.len);
   }
-  if (warp == 4) {
-    loader<D, Q8>(mk, mv, p, cons, nt, smem, full, empty, wait);
+  if (warp >= 4) {
+    setmaxnreg_dec<24>();
+    if (warp == 4) loader<X, D, Q8>(mk, mv, p, cons, nt, smem, full, empty, wait);
     return;
   }
+  setmaxnreg_inc<X::COMPUTE_REGS>();
 
-  State<D> st;
-  uint32_t qf[D / 16][4];
-  float qs[2];      // factor from the raw product to log2 units, per row
-  int limit[2];     // keys that the row sees
-  int see_all = 0;  // keys that every row of the item sees
+  State<D, NB> st;
+  uint32_t qf[D / 16][NB][2];
+  float qs[NB][2];      // factor from the raw product to log2 units, per row
+  int limit[NB][2];     // keys that the row sees
+  int see_all = 0;      // keys that every row of the item sees
   bool first_piece = true, fresh = true, alive = true;
   int stage = 0;
   uint32_t phase = 0;
@@ -465,34 +514,46 @@ __global__ void __launch_bounds__(kAllThreads, 2)
     const int rt = cons.hr % p.RT, h = cons.hr / p.RT;
     if (fresh) {
       fresh = false;
-#pragma unroll
-      for (int n = 0; n < D / 8; ++n) st.acc[n][0] = st.acc[n][1] = st.acc[n][2] = st.acc[n][3] = 0.f;
       see_all = p.causal ? cons.len - p.T + 1 : cons.len;
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        st.m[x] = st.mt[x] = -INFINITY;
-        st.l[x] = 0.f;
-        const int r = rt * 16 * WR + wr * 16 + (lane >> 2) + x * 8;
+      for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+        for (int t = 0; t < D / 16; ++t) st.acc[t][nb][0] = st.acc[t][nb][1] = st.acc[t][nb][2] = st.acc[t][nb][3] = 0.f;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          st.m[nb][e] = st.mt[nb][e] = -INFINITY;
+          st.l[nb][e] = 0.f;
+          const int r = rt * X::RC + wr * X::RW + nb * 8 + quad * 2 + e;
+          limit[nb][e] = r >= p.R ? 0 : p.causal ? cons.len - p.T + r / p.G + 1 : cons.len;
+          qs[nb][e] = p.scale_log2;
+        }
+        // the queries as the instruction's second operand: row lane / 4
+        const int r = rt * X::RC + wr * X::RW + nb * 8 + g8;
         const bool live = r < p.R;
         const int t = live ? r / p.G : 0, g = live ? r - t * p.G : 0;
-        limit[x] = !live ? 0 : p.causal ? cons.len - p.T + t + 1 : cons.len;
         const __nv_bfloat16* src = p.q + cons.b * p.q_sb + (int64_t)(h * p.G + g) * p.q_sh + t * p.q_sl;
-        qs[x] = p.scale_log2;
         if constexpr (!Q8) {
 #pragma unroll
           for (int kk = 0; kk < D / 16; ++kk) {
-            qf[kk][x] = live ? *reinterpret_cast<const uint32_t*>(src + kk * 16 + quad * 2) : 0u;
-            qf[kk][x + 2] = live ? *reinterpret_cast<const uint32_t*>(src + kk * 16 + quad * 2 + 8) : 0u;
+            qf[kk][nb][0] = live ? *reinterpret_cast<const uint32_t*>(src + kk * 16 + quad * 2) : 0u;
+            qf[kk][nb][1] = live ? *reinterpret_cast<const uint32_t*>(src + kk * 16 + quad * 2 + 8) : 0u;
           }
         } else {
-          // matrix step 4 i + s takes elements 16 (2 quad + i) + 4 s + {0..3} (D = 64: 16 quad + 4 s) from this thread
+          // operands widened in registers: matrix step 4 i + s takes elements 16 (2 quad + i) + 4 s + {0..3} (D = 64:
+          // 16 quad + 4 s) from this thread; else 16 kk + 2 quad + {0, 1} and + 8
           constexpr int CH = D / 64;
           uint2 raw[D / 16];
           float most = 0.f;
           bool fine = true;
 #pragma unroll
-          for (int kk = 0; kk < D / 16; ++kk)
-            raw[kk] = live ? *reinterpret_cast<const uint2*>(src + 16 * (CH * quad + kk / 4) + 4 * (kk % 4)) : make_uint2(0u, 0u);
+          for (int kk = 0; kk < D / 16; ++kk) {
+            if constexpr (X::WIDE) {
+              raw[kk].x = live ? *reinterpret_cast<const uint32_t*>(src + kk * 16 + quad * 2) : 0u;
+              raw[kk].y = live ? *reinterpret_cast<const uint32_t*>(src + kk * 16 + quad * 2 + 8) : 0u;
+            } else {
+              raw[kk] = live ? *reinterpret_cast<const uint2*>(src + 16 * (CH * quad + kk / 4) + 4 * (kk % 4)) : make_uint2(0u, 0u);
+            }
+          }
 #pragma unroll
           for (int kk = 0; kk < D / 16; ++kk) {
             const uint32_t w[2] = {raw[kk].x, raw[kk].y};
@@ -505,165 +566,204 @@ __global__ void __launch_bounds__(kAllThreads, 2)
           }
           most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
           most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
-          const int e = min(max((int)(__float_as_uint(most) >> 23) - 127, -126), 126);
+          const int ex = min(max((int)(__float_as_uint(most) >> 23) - 127, -126), 126);
           const unsigned fines = __ballot_sync(0xffffffffu, fine) >> (lane & 28);
-          const int sh = (fines & 15u) == 15u && most > 0.f ? e : 0;
+          const int sh = (fines & 15u) == 15u && most > 0.f ? ex : 0;
           const float down = pow2i(-sh);
-          qs[x] = p.scale_log2 * pow2i(sh);
 #pragma unroll
           for (int kk = 0; kk < D / 16; ++kk) {
-            qf[kk][x] = pack_f16x2(__uint_as_float(raw[kk].x << 16) * down, __uint_as_float(raw[kk].x & 0xffff0000u) * down);
-            qf[kk][x + 2] = pack_f16x2(__uint_as_float(raw[kk].y << 16) * down, __uint_as_float(raw[kk].y & 0xffff0000u) * down);
+            qf[kk][nb][0] = pack_f16x2(__uint_as_float(raw[kk].x << 16) * down, __uint_as_float(raw[kk].x & 0xffff0000u) * down);
+            qf[kk][nb][1] = pack_f16x2(__uint_as_float(raw[kk].y << 16) * down, __uint_as_float(raw[kk].y & 0xffff0000u) * down);
           }
+          // this thread's scores are those of rows 2 quad + e, scaled by lane 4 (2 quad + e)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) qs[nb][e] *= pow2i(__shfl_sync(0xffffffffu, sh, (quad * 2 + e) * 4));
         }
       }
     }
     alive = alive && mbar_wait(&full[stage], phase, wait, DEV_TIMEOUT_SOFTMAX);
 
-    const bool idle = rt * 16 * WR + wr * 16 >= p.R || !alive;  // none of the warp's rows exists
-    const uint32_t ks = ring + stage * X::STAGE, vs = ks + X::KT * X::RB;
+    const bool idle = rt * X::RC + wr * X::RW >= p.R || !alive;  // none of the warp's rows exists
+    const uint32_t raw_v = ring + stage * X::STAGE + X::KT * X::RB;
     const uint32_t ss = ring + X::STAGES * X::STAGE + stage * X::SCALE_STAGE;
+    const uint32_t ks = X::WIDE ? ring + X::STAGES * (X::STAGE + X::SCALE_STAGE) : ring + stage * X::STAGE;
+    const uint32_t vs = ks + X::SUBS * X::KT * (X::WIDE ? D * 2 : X::RS);
+    if constexpr (X::WIDE) {
+      constexpr int CPR = X::RB / 16;
+      compute_sync();  // the last tile's readers are done
+#pragma unroll
+      for (int j = 0; j < 2 * X::KT * CPR / kThreads; ++j) {
+        const int at = j * kThreads + tid, row = at / CPR % X::KT, c = at % CPR, v = at / (CPR * X::KT);
+        const uint4 w = lds128(ring + stage * X::STAGE + v * X::KT * X::RB + row * X::RB + ((c ^ swizzle_of<X::RS>(row)) << 4));
+        uint32_t o[8];
+        widen4(w.x, o[0], o[1]);
+        widen4(w.y, o[2], o[3]);
+        widen4(w.z, o[4], o[5]);
+        widen4(w.w, o[6], o[7]);
+        const uint32_t dst = (v ? vs : ks) + (c >> 2) * X::OSUB + row * 128;
+        sts128(dst + (((2 * c & 7) ^ (row & 7)) << 4), o[0], o[1], o[2], o[3]);
+        sts128(dst + (((2 * c & 7) + 1 ^ (row & 7)) << 4), o[4], o[5], o[6], o[7]);
+      }
+      compute_sync();
+    }
 #pragma unroll 1
     for (int s0 = wk * KW; s0 < (wk + 1) * KW; s0 += NS) {
       const int key0 = cons.tile * X::KT + s0;
       if (key0 >= cons.len || idle) break;  // the same for the whole warp
-      // scores
-      float sc[NT][4];
+      // scores, transposed: a thread has keys lane / 4 and + 8 of every 16, two rows of every 8
+      float sc[NK][NB][4];
 #pragma unroll
-      for (int n = 0; n < NT; ++n) sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.f;
-      if constexpr (!Q8) {
+      for (int k = 0; k < NK; ++k)
 #pragma unroll
-        for (int n2 = 0; n2 < NT / 2; ++n2) {
-          const uint32_t k0 = ks + (s0 + n2 * 16 + (lane & 7) + ((lane >> 4) << 3)) * X::RS + ((((lane >> 3) & 1) ^ (lane & 7)) << 4);
+        for (int nb = 0; nb < NB; ++nb) sc[k][nb][0] = sc[k][nb][1] = sc[k][nb][2] = sc[k][nb][3] = 0.f;
+      if constexpr (!Q8 || X::WIDE) {
+        const uint32_t k0 = ks + (s0 + (lane & 15)) * X::OS + (((lane >> 4) ^ (lane & 7)) << 4);
 #pragma unroll
-          for (int kk = 0; kk < D / 16; ++kk) {
-            uint32_t b[4];
-            ldsm_x4((k0 ^ ((kk & 3) << 5)) + (kk >> 2) * X::SUB, b);
-            mma_bf16(sc[n2 * 2], qf[kk], b[0], b[1]);
-            mma_bf16(sc[n2 * 2 + 1], qf[kk], b[2], b[3]);
+        for (int kk = 0; kk < D / 16; ++kk) {
+#pragma unroll
+          for (int k = 0; k < NK; ++k) {
+            uint32_t a[4];
+            ldsm_x4((k0 ^ ((kk & 3) << 5)) + (kk >> 2) * X::OSUB + k * 16 * X::OS, a);
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) {
+              if constexpr (Q8) mma_f16(sc[k][nb], a, qf[kk][nb][0], qf[kk][nb][1]);
+              else mma_bf16(sc[k][nb], a, qf[kk][nb][0], qf[kk][nb][1]);
+            }
           }
         }
       } else {
         constexpr int CH = D / 64;
-        const uint32_t k0 = ks + (s0 + (lane >> 2)) * X::RS + (((CH * quad) ^ swizzle_of<X::RS>(lane >> 2)) << 4);
+        const uint32_t k0 = ks + (s0 + g8) * X::RS + (((CH * quad) ^ swizzle_of<X::RS>(g8)) << 4);
 #pragma unroll
         for (int ch = 0; ch < CH; ++ch) {
-          uint4 w[NT];
 #pragma unroll
-          for (int n = 0; n < NT; ++n) w[n] = lds128((k0 ^ (ch << 4)) + n * 8 * X::RS);
-#pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            const uint32_t u[4] = {w[n].x, w[n].y, w[n].z, w[n].w};
+          for (int k = 0; k < NK; ++k) {
+            const uint4 w0 = lds128((k0 ^ (ch << 4)) + k * 16 * X::RS), w1 = lds128((k0 ^ (ch << 4)) + (k * 16 + 8) * X::RS);
+            const uint32_t u0[4] = {w0.x, w0.y, w0.z, w0.w}, u1[4] = {w1.x, w1.y, w1.z, w1.w};
 #pragma unroll
             for (int s = 0; s < 4; ++s) {
-              uint32_t lo, hi;
-              widen4(u[s], lo, hi);
-              mma_f16(sc[n], qf[ch * 4 + s], lo, hi);
+              uint32_t a[4];
+              widen4(u0[s], a[0], a[2]);
+              widen4(u1[s], a[1], a[3]);
+#pragma unroll
+              for (int nb = 0; nb < NB; ++nb) mma_f16(sc[k][nb], a, qf[ch * 4 + s][nb][0], qf[ch * 4 + s][nb][1]);
             }
           }
         }
       }
       // e4m3: scores to log2 units, with the rows' scales (bf16: one factor, taken in with the maximum below)
-      uint64_t ve[NT];  // V's exponents of the thread's two keys
+      float ve[NK][2];  // V's exponents of the thread's keys
       if constexpr (Q8) {
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-          const uint32_t ex = lds32(ss + (s0 + n * 8 + quad * 2) * 2);  // K, V, K, V
-          const uint64_t kf = pack_f32x2(__uint_as_float((ex << 23) & 0x7f800000u), __uint_as_float((ex << 7) & 0x7f800000u));
-          // a byte below the exponent of 2^23 is 2^23 + byte
-          ve[n] = fadd2(pack_f32x2(__uint_as_float(__byte_perm(ex, 0x4b000000u, 0x7441)), __uint_as_float(__byte_perm(ex, 0x4b000000u, 0x7443))),
-                        pack_f32x2(-8388608.f - 127.f, -8388608.f - 127.f));
+        for (int k = 0; k < NK; ++k)
 #pragma unroll
-          for (int x = 0; x < 2; ++x)
-            unpack_f32x2(fmul2(pack_f32x2(sc[n][2 * x], sc[n][2 * x + 1]), fmul2(kf, pack_f32x2(qs[x], qs[x]))), sc[n][2 * x], sc[n][2 * x + 1]);
-        }
+          for (int y = 0; y < 2; ++y) {
+            const uint32_t ex = lds16(ss + (s0 + k * 16 + y * 8 + g8) * 2);  // K's, V's
+            const float kf = __uint_as_float((ex << 23) & 0x7f800000u);
+            ve[k][y] = __uint_as_float(0x4b000000u | (ex >> 8)) - (8388608.f + 127.f);  // 2^23 + byte, exact
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb)
+              unpack_f32x2(fmul2(pack_f32x2(sc[k][nb][2 * y], sc[k][nb][2 * y + 1]),
+                                 fmul2(pack_f32x2(kf, kf), pack_f32x2(qs[nb][0], qs[nb][1]))),
+                           sc[k][nb][2 * y], sc[k][nb][2 * y + 1]);
+          }
       }
       const bool edge = key0 + NS > see_all;  // some row does not see some of these keys
       if (edge) {
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+        for (int k = 0; k < NK; ++k)
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (key0 + n * 8 + quad * 2 + (e & 1) >= limit[e >> 1]) sc[n][e] = -INFINITY;
+          for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (key0 + k * 16 + (e >> 1) * 8 + g8 >= limit[nb][e & 1]) sc[k][nb][e] = -INFINITY;
       }
       // running maximum and sum; weights
-      float alpha[2];
+      float alpha[NB][2];
+      bool moved = false;
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        if constexpr (Q8) {
-          float mx = st.m[x], tx = st.mt[x];
+      for (int nb = 0; nb < NB; ++nb) {
+        float mx[2] = {-INFINITY, -INFINITY}, tx[2] = {-INFINITY, -INFINITY}, mu[2], tu[2];
 #pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            float t0, t1;
-            unpack_f32x2(fadd2(pack_f32x2(sc[n][2 * x], sc[n][2 * x + 1]), ve[n]), t0, t1);
-            mx = fmax3(mx, sc[n][2 * x], sc[n][2 * x + 1]);
-            tx = fmax3(tx, t0, t1);
+        for (int k = 0; k < NK; ++k) {
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            mx[e] = fmax3(mx[e], sc[k][nb][e], sc[k][nb][2 + e]);
+            if constexpr (Q8) tx[e] = fmax3(tx[e], sc[k][nb][e] + ve[k][0], sc[k][nb][2 + e] + ve[k][1]);
           }
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-          tx = fmaxf(tx, __shfl_xor_sync(0xffffffffu, tx, 1));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-          tx = fmaxf(tx, __shfl_xor_sync(0xffffffffu, tx, 2));
-          const float mu = mx == -INFINITY ? 0.f : -mx;
-          const float tu = tx == -INFINITY ? 0.f : 15.f - tx;  // weights up to 2^15
-          float add = 0.f;
+        }
 #pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            const uint64_t s = pack_f32x2(sc[n][2 * x], sc[n][2 * x + 1]);
-            float a, b, c, d;
-            unpack_f32x2(fadd2(s, pack_f32x2(mu, mu)), a, b);
-            unpack_f32x2(fadd2(fadd2(s, ve[n]), pack_f32x2(tu, tu)), c, d);
-            add += fast_exp2(a) + fast_exp2(b);
-            sc[n][2 * x] = fast_exp2(c);
-            sc[n][2 * x + 1] = fast_exp2(d);
+        for (int e = 0; e < 2; ++e) {
+          mx[e] = max_of_keys(mx[e]);
+          mx[e] = fmaxf(st.m[nb][e], Q8 ? mx[e] : mx[e] * qs[nb][e]);
+          mu[e] = mx[e] == -INFINITY ? 0.f : -mx[e];
+          if constexpr (Q8) {
+            tx[e] = fmaxf(st.mt[nb][e], max_of_keys(tx[e]));
+            tu[e] = tx[e] == -INFINITY ? 0.f : 15.f - tx[e];  // weights up to 2^15
           }
-          alpha[x] = fast_exp2(st.mt[x] - (tx == -INFINITY ? 0.f : tx));
-          st.l[x] = st.l[x] * fast_exp2(st.m[x] + mu) + add;
-          st.m[x] = mx;
-          st.mt[x] = tx;
-        } else {
-          float raw = -INFINITY;
+        }
+        uint64_t add = 0;
 #pragma unroll
-          for (int n = 0; n < NT; ++n) raw = fmax3(raw, sc[n][2 * x], sc[n][2 * x + 1]);
-          raw = fmaxf(raw, __shfl_xor_sync(0xffffffffu, raw, 1));
-          raw = fmaxf(raw, __shfl_xor_sync(0xffffffffu, raw, 2));
-          const float mx = fmaxf(st.m[x], raw * qs[x]);
-          const float mu = mx == -INFINITY ? 0.f : -mx;
-          float add = 0.f;
+        for (int k = 0; k < NK; ++k)
 #pragma unroll
-          for (int n = 0; n < NT; ++n) {
+          for (int y = 0; y < 2; ++y) {
+            const uint64_t s = pack_f32x2(sc[k][nb][2 * y], sc[k][nb][2 * y + 1]);
             float a, b;
-            unpack_f32x2(ffma2(pack_f32x2(sc[n][2 * x], sc[n][2 * x + 1]), pack_f32x2(qs[x], qs[x]), pack_f32x2(mu, mu)), a, b);
-            sc[n][2 * x] = fast_exp2(a);
-            sc[n][2 * x + 1] = fast_exp2(b);
-            add += sc[n][2 * x] + sc[n][2 * x + 1];
+            if constexpr (Q8) {
+              unpack_f32x2(fadd2(s, pack_f32x2(mu[0], mu[1])), a, b);
+              add = fadd2(add, pack_f32x2(fast_exp2(a), fast_exp2(b)));
+              unpack_f32x2(fadd2(fadd2(s, pack_f32x2(ve[k][y], ve[k][y])), pack_f32x2(tu[0], tu[1])), a, b);
+              sc[k][nb][2 * y] = fast_exp2(a);
+              sc[k][nb][2 * y + 1] = fast_exp2(b);
+            } else {
+              unpack_f32x2(ffma2(s, pack_f32x2(qs[nb][0], qs[nb][1]), pack_f32x2(mu[0], mu[1])), a, b);
+              sc[k][nb][2 * y] = fast_exp2(a);
+              sc[k][nb][2 * y + 1] = fast_exp2(b);
+              add = fadd2(add, pack_f32x2(sc[k][nb][2 * y], sc[k][nb][2 * y + 1]));
+            }
           }
-          alpha[x] = fast_exp2(st.m[x] + mu);
-          st.l[x] = st.l[x] * alpha[x] + add;
-          st.m[x] = mx;
+        float part[2];
+        unpack_f32x2(add, part[0], part[1]);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float f = fast_exp2(st.m[nb][e] + mu[e]);
+          alpha[nb][e] = Q8 ? fast_exp2(st.mt[nb][e] - (tx[e] == -INFINITY ? 0.f : tx[e])) : f;
+          moved = moved || alpha[nb][e] != 1.f;  // a NaN counts
+          st.l[nb][e] = fmaf(st.l[nb][e], f, part[e]);
+          st.m[nb][e] = mx[e];
+          if constexpr (Q8) st.mt[nb][e] = tx[e];
         }
       }
-      if (__any_sync(0xffffffffu, !(alpha[0] == 1.f && alpha[1] == 1.f))) {
+      if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
-        for (int n = 0; n < D / 8; ++n)
+        for (int t = 0; t < D / 16; ++t)
 #pragma unroll
-          for (int x = 0; x < 2; ++x)
-            unpack_f32x2(fmul2(pack_f32x2(st.acc[n][2 * x], st.acc[n][2 * x + 1]), pack_f32x2(alpha[x], alpha[x])), st.acc[n][2 * x],
-                         st.acc[n][2 * x + 1]);
+          for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+            for (int y = 0; y < 2; ++y)
+              unpack_f32x2(fmul2(pack_f32x2(st.acc[t][nb][2 * y], st.acc[t][nb][2 * y + 1]), pack_f32x2(alpha[nb][0], alpha[nb][1])),
+                           st.acc[t][nb][2 * y], st.acc[t][nb][2 * y + 1]);
       }
       // In a step that some row does not see all of, elements of V that are not finite come in row by row: a weight of zero
       // would make NaN of them in rows that do not see them.
-      if (edge && any_odd<D, Q8, NS>(vs, s0)) {
-        weigh<D, Q8, NT, true>(st, sc, vs, s0);
-        State<D> st2 = st;
-        float w[NT][4];
+      if (edge && any_odd<X, Q8, NS>(raw_v, s0)) {
+        weigh<X, D, Q8, NB, NK, true>(st, sc, vs, s0);
+        State<D, NB> st2 = st;
+        float w[NK][NB][4];
+        int seen[NB][2];
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+        for (int nb = 0; nb < NB; ++nb) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) w[n][e] = sc[n][e];
-        weigh_odd<D, Q8, NT>(st2, w, vs, s0, limit[0] - key0, limit[1] - key0);
+          for (int k = 0; k < NK; ++k)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w[k][nb][e] = sc[k][nb][e];
+          seen[nb][0] = limit[nb][0] - key0;
+          seen[nb][1] = limit[nb][1] - key0;
+        }
+        weigh_odd<X, D, Q8, NB, NK>(st2, w, seen, raw_v, s0);
         st = st2;
       } else {
-        weigh<D, Q8, NT, false>(st, sc, vs, s0);
+        weigh<X, D, Q8, NB, NK, false>(st, sc, vs, s0);
       }
     }
 
@@ -671,63 +771,64 @@ __global__ void __launch_bounds__(kAllThreads, 2)
     if (last || i == nt - 1) {
       // Join of the warps that share rows, in the stage just consumed.
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        st.l[x] += __shfl_xor_sync(0xffffffffu, st.l[x], 1);
-        st.l[x] += __shfl_xor_sync(0xffffffffu, st.l[x], 2);
-        if (quad == 0) {
-          ml[(warp * 16 + (lane >> 2) + x * 8) * 2] = st.m[x];
-          ml[(warp * 16 + (lane >> 2) + x * 8) * 2 + 1] = st.l[x];
+      for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          st.l[nb][e] = sum_of_keys(st.l[nb][e]);
+          if (g8 == 0)
+            *reinterpret_cast<float2*>(ml + (warp * X::RW + nb * 8 + quad * 2 + e) * 2) = make_float2(st.m[nb][e], st.l[nb][e]);
         }
-      }
       compute_sync();
-      float* buf = reinterpret_cast<float*>(smem + stage * X::STAGE);  // [warp][16][D]
+      // [warp][row][D]; elements are XORed with 8 times bits 1 and 2 of the row, so that a warp's rows differ in their banks
+      float* buf = reinterpret_cast<float*>(smem + (X::WIDE ? X::STAGES * (X::STAGE + X::SCALE_STAGE) : stage * X::STAGE));
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        const int row = (lane >> 2) + x * 8;
-        float top = -INFINITY;
+      for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-        for (int w = 0; w < WK; ++w) top = fmaxf(top, ml[((w * WR + wr) * 16 + row) * 2]);
-        // an infinite maximum (an infinite score) gives NaN here, as exp(inf - inf) does
-        const float own = Q8 ? st.mt[x] - 15.f : st.m[x];
-        const float f = own == -INFINITY ? 0.f : exp2f(own - top);
-        float* dst = buf + (warp * 16 + row) * D;
-        if constexpr (!Q8) {
+        for (int e = 0; e < 2; ++e) {
+          const int row = nb * 8 + quad * 2 + e;
+          float top = -INFINITY;
 #pragma unroll
-          for (int n = 0; n < D / 8; ++n)
-            *reinterpret_cast<float2*>(dst + n * 8 + quad * 2) = make_float2(st.acc[n][2 * x] * f, st.acc[n][2 * x + 1] * f);
-        } else {
+          for (int w = 0; w < WK; ++w) top = fmaxf(top, ml[((w * WR + wr) * X::RW + row) * 2]);
+          // an infinite maximum (an infinite score) gives NaN here, as exp(inf - inf) does
+          const float own = Q8 ? st.mt[nb][e] - 15.f : st.m[nb][e];
+          const float f = own == -INFINITY ? 0.f : exp2f(own - top);
+          float* dst = buf + (warp * X::RW + row) * D;
+          if constexpr (!Q8 || X::WIDE) {
 #pragma unroll
-          for (int e = 0; e < 2; ++e)
+            for (int t = 0; t < D / 16; ++t) {
+              dst[element_of<D, false>(t, 0) ^ (quad * 8)] = st.acc[t][nb][e] * f;
+              dst[element_of<D, false>(t, 1) ^ (quad * 8)] = st.acc[t][nb][2 + e] * f;
+            }
+          } else {
 #pragma unroll
-            for (int n = 0; n < D / 8; n += 4)
-              *reinterpret_cast<float4*>(dst + (quad * 2 + e) * (D / 8) + n) =
-                  make_float4(st.acc[n][2 * x + e] * f, st.acc[n + 1][2 * x + e] * f, st.acc[n + 2][2 * x + e] * f,
-                              st.acc[n + 3][2 * x + e] * f);
+            for (int t = 0; t < D / 16; t += 2)
+              *reinterpret_cast<float4*>(dst + (element_of<D, true>(t, 0) ^ (quad * 8))) = make_float4(
+                  st.acc[t][nb][e] * f, st.acc[t][nb][2 + e] * f, st.acc[t + 1][nb][e] * f, st.acc[t + 1][nb][2 + e] * f);
+          }
         }
-      }
       compute_sync();
       const bool whole = last && (!first_piece || whole_first);
       const int slot = first_piece ? 0 : 1;
       constexpr int TPR = D / 8, RPP = kThreads / TPR;
       const int e0 = (tid % TPR) * 8;
-      const int live = min(16 * WR, p.R - rt * 16 * WR);
+      const int live = min(X::RC, p.R - rt * X::RC);
       for (int row = tid / TPR; row < live; row += RPP) {
-        const int w0 = row >> 4, r16 = row & 15;
+        const int w0 = row / X::RW, in = row % X::RW, ex = e0 ^ ((in >> 1 & 3) * 8);
         float top = -INFINITY, sum = 0.f, v[8] = {};
 #pragma unroll
-        for (int w = 0; w < WK; ++w) top = fmaxf(top, ml[((w * WR + w0) * 16 + r16) * 2]);
+        for (int w = 0; w < WK; ++w) top = fmaxf(top, ml[((w * WR + w0) * X::RW + in) * 2]);
 #pragma unroll
         for (int w = 0; w < WK; ++w) {
-          const int at = (w * WR + w0) * 16 + r16;
+          const int at = (w * WR + w0) * X::RW + in;
           const float mw = ml[at * 2];
           sum += mw == -INFINITY ? 0.f : ml[at * 2 + 1] * exp2f(mw - top);
-          const float4 x = *reinterpret_cast<const float4*>(buf + at * D + e0);
-          const float4 y = *reinterpret_cast<const float4*>(buf + at * D + e0 + 4);
+          const float4 x = *reinterpret_cast<const float4*>(buf + at * D + ex);
+          const float4 y = *reinterpret_cast<const float4*>(buf + at * D + ex + 4);
           v[0] += x.x, v[1] += x.y, v[2] += x.z, v[3] += x.w;
           v[4] += y.x, v[5] += y.y, v[6] += y.z, v[7] += y.w;
         }
         if (whole) {
-          const int r = rt * 16 * WR + row, t = r / p.G, head = h * p.G + r - t * p.G;
+          const int r = rt * X::RC + row, t = r / p.G, head = h * p.G + r - t * p.G;
           const float inv = top == -INFINITY ? 0.f : 1.f / sum;  // a row that sees no key gives 0
           uint4 out;
           out.x = pack_bf16x2(v[0] * inv, v[1] * inv);
@@ -741,10 +842,10 @@ __global__ void __launch_bounds__(kAllThreads, 2)
             p.L[at] = sum;
           }
         } else {
-          float* dst = p.part + ((int64_t)blockIdx.x * kSlotsPerCta + slot) * (16 * WR * (D + 2));
+          float* dst = p.part + ((int64_t)blockIdx.x * kSlotsPerCta + slot) * (X::RC * (D + 2));
           *reinterpret_cast<float4*>(dst + row * D + e0) = make_float4(v[0], v[1], v[2], v[3]);
           *reinterpret_cast<float4*>(dst + row * D + e0 + 4) = make_float4(v[4], v[5], v[6], v[7]);
-          if (e0 == 0) *reinterpret_cast<float2*>(dst + 16 * WR * D + row * 2) = make_float2(top, sum);
+          if (e0 == 0) *reinterpret_cast<float2*>(dst + X::RC * D + row * 2) = make_float2(top, sum);
         }
       }
       first_piece = false;
@@ -760,29 +861,29 @@ __global__ void __launch_bounds__(kAllThreads, 2)
 }
 
 // Joins the pieces of the item that begins in CTA x's range and goes on behind it: a warp per row, pieces in order.
-template <int D, bool Q8, int WR>
-__global__ void __launch_bounds__(kThreads) paged_join_kernel(const __grid_constant__ PagedAttnParams p, int ctas) {
-  using X = Geo<D, Q8>;
+template <int D, int KT>
+__global__ void __launch_bounds__(kThreads) paged_join_kernel(const __grid_constant__ PagedAttnParams p, int ctas, int rc) {
   __shared__ int64_t scan[8];
   const int c = blockIdx.x, lane = threadIdx.x & 31;
-  griddep_wait();
+  // The lengths were there before the pieces' kernel began; only the pieces have to be waited for.
   int64_t excl, item_start;
   int b0, b1;
-  const Line line = line_scan<X::KT>(p, ctas, scan, excl, b0, b1);
+  const Line line = line_scan<KT>(p, ctas, scan, excl, b0, b1);
   if (c >= line.nc) return;
   const int64_t start = range_start(line, c), end = range_start(line, c + 1);
-  const Cursor it = line_locate<X::KT>(p, end - 1, excl, b0, b1, scan, item_start);
+  const Cursor it = line_locate<KT>(p, end - 1, excl, b0, b1, scan, item_start);
   const int64_t item_end = item_start + it.ntile;
   if (item_start < start || item_end <= end) return;  // begins in another range, or ends in this one
   // The last CTA of the item: the one whose range holds item_end - 1.
   int last = (int)((item_end - 1) * line.nc / line.total);
   while (range_start(line, last + 1) < item_end) ++last;
   while (range_start(line, last) >= item_end) --last;
+  griddep_wait();
   const int rt = it.hr % p.RT, h = it.hr / p.RT;
   const int row = blockIdx.y * 4 + (threadIdx.x >> 5);
-  const int r = rt * 16 * WR + row;
-  if (row >= 16 * WR || r >= p.R) return;
-  const int64_t slot_floats = 16 * WR * (D + 2);
+  const int r = rt * rc + row;
+  if (row >= rc || r >= p.R) return;
+  const int64_t slot_floats = rc * (D + 2);
   const int n = last - c + 1;
   // piece 0 is slot 0 of this CTA if it is also its first piece, else slot 1; every later one is slot 0 of its CTA
   const float* first = p.part + ((int64_t)c * kSlotsPerCta + (item_start == start ? 0 : 1)) * slot_floats;
@@ -790,7 +891,7 @@ __global__ void __launch_bounds__(kThreads) paged_join_kernel(const __grid_const
   float top = -INFINITY;
   for (int i = lane; i < n; i += 32) {
     const float* s = i == 0 ? first : later + (int64_t)i * kSlotsPerCta * slot_floats;
-    top = fmaxf(top, s[16 * WR * D + row * 2]);
+    top = fmaxf(top, s[rc * D + row * 2]);
   }
 #pragma unroll
   for (int d = 16; d >= 1; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
@@ -800,7 +901,7 @@ __global__ void __launch_bounds__(kThreads) paged_join_kernel(const __grid_const
     float f = 0.f, lsum = 0.f;
     if (i0 + lane < n) {
       const float* s = i0 + lane == 0 ? first : later + (int64_t)(i0 + lane) * kSlotsPerCta * slot_floats;
-      const float2 x = *reinterpret_cast<const float2*>(s + 16 * WR * D + row * 2);
+      const float2 x = *reinterpret_cast<const float2*>(s + rc * D + row * 2);
       f = x.x == -INFINITY ? 0.f : exp2f(x.x - top);
       lsum = x.y * f;
     }
@@ -839,9 +940,10 @@ __global__ void __launch_bounds__(kThreads) paged_join_kernel(const __grid_const
   }
 }
 
-// What a call launches: rows per CTA, whether items are split, the number of CTAs.
+// What a call launches: blocks of 8 rows per warp, warps that differ in their rows, row tiles, whether items are split, the
+// number of CTAs.
 struct Plan {
-  int wr, rt, split, ctas;
+  int nb, wr, rt, split, ctas;
   int64_t workspace;
 };
 
@@ -854,23 +956,25 @@ int device_sms(int* sms) {
 
 int plan_of(int B, int Hq, int Hkv, int T, int D, bool q8, int max_len, int sms, Plan* out) {
   const int64_t R = (int64_t)T * (Hq / Hkv);
+  out->nb = R <= 8 ? 1 : 2;
   out->wr = R <= 16 ? 1 : R <= 32 ? 2 : 4;
-  const int64_t rt = (R + 16 * out->wr - 1) / (16 * out->wr);
-  const int kt = q8 || D == 64 ? 128 : 64;
+  const int rc = 8 * out->nb * out->wr;
+  const int64_t rt = (R + rc - 1) / rc;
+  const int kt = keys_per_tile(D, q8, out->wr);
   const int64_t tiles = max_len <= kt ? 1 : ((int64_t)max_len + kt - 1) / kt;
   const int64_t items = B * (int64_t)Hkv * rt;
   LVAR_REQUIRE(items < (1ll << 24), LVAR_ERR_LIMIT, "too many (sequence, key head, row tile) items");
   out->rt = (int)rt;
   out->split = tiles > 2;
-  out->ctas = out->split ? 2 * sms : (int)items;
-  out->workspace = out->split ? (int64_t)out->ctas * kSlotsPerCta * 16 * out->wr * (D + 2) * 4 : 0;
+  out->ctas = out->split ? ctas_per_sm(D, q8, out->nb) * sms : (int)items;
+  out->workspace = out->split ? (int64_t)out->ctas * kSlotsPerCta * rc * (D + 2) * 4 : 0;
   return LVAR_OK;
 }
 
-template <int D, bool Q8, int WR>
+template <int D, bool Q8, int NB, int WR>
 int launch(const PagedAttnParams& p, const CUtensorMap& mk, const CUtensorMap& mv, const Plan& plan, cudaStream_t stream) {
-  using X = Geo<D, Q8>;
-  auto kern = paged_attn_kernel<D, Q8, WR>;
+  using X = Geo<D, Q8, NB, WR>;
+  auto kern = paged_attn_kernel<D, Q8, NB, WR>;
   LVAR_CUDA_OK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, X::SMEM));
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)plan.ctas);
@@ -884,29 +988,30 @@ int launch(const PagedAttnParams& p, const CUtensorMap& mk, const CUtensorMap& m
   cfg.numAttrs = 1;
   LVAR_CUDA_OK(cudaLaunchKernelEx(&cfg, kern, mk, mv, p));
   if (plan.split) {
-    const int rows = p.R < 16 * WR ? p.R : 16 * WR;
+    const int rows = p.R < X::RC ? p.R : X::RC;
     cfg.gridDim = dim3((unsigned)plan.ctas, (unsigned)((rows + 3) / 4));
     cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = 0;
-    LVAR_CUDA_OK(cudaLaunchKernelEx(&cfg, paged_join_kernel<D, Q8, WR>, p, plan.ctas));
+    LVAR_CUDA_OK(cudaLaunchKernelEx(&cfg, paged_join_kernel<D, X::KT>, p, plan.ctas, X::RC));
   }
   return LVAR_OK;
 }
 
 template <int D, bool Q8>
 int launch_wr(PagedAttnParams& p, const lvar_paged_cache& c, const Plan& plan, cudaStream_t stream) {
-  using X = Geo<D, Q8>;
+  const int KT = keys_per_tile(D, Q8, plan.wr);
   // Rows per copy: what page and tile have in common, and not far more than the longest sequence has.
-  int box = X::KT;
-  while (c.page_size % box != 0 || X::KT % box != 0) box -= 16;
+  int box = KT;
+  while (c.page_size % box != 0 || KT % box != 0) box -= 16;
   while (box % 32 == 0 && box / 2 >= p.max_len) box /= 2;
   p.box = box;
   CUtensorMap mk, mv;
   if (int rc = encode_pages_map(&mk, c.k, Q8, c.num_pages, c.Hkv, c.page_size, D, c.k_sp, c.k_sh, c.k_sl, box)) return rc;
   if (int rc = encode_pages_map(&mv, c.v, Q8, c.num_pages, c.Hkv, c.page_size, D, c.v_sp, c.v_sh, c.v_sl, box)) return rc;
-  if (plan.wr == 1) return launch<D, Q8, 1>(p, mk, mv, plan, stream);
-  if (plan.wr == 2) return launch<D, Q8, 2>(p, mk, mv, plan, stream);
-  return launch<D, Q8, 4>(p, mk, mv, plan, stream);
+  if (plan.nb == 1) return launch<D, Q8, 1, 1>(p, mk, mv, plan, stream);
+  if (plan.wr == 1) return launch<D, Q8, 2, 1>(p, mk, mv, plan, stream);
+  if (plan.wr == 2) return launch<D, Q8, 2, 2>(p, mk, mv, plan, stream);
+  return launch<D, Q8, 2, 4>(p, mk, mv, plan, stream);
 }
 
 }  // namespace
