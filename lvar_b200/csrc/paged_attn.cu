@@ -11,8 +11,7 @@
 // A CTA is four warps that compute and one that loads.  The loader follows the page table (one lane per box of 16 to 128
 // rows that lie together in a page) and streams tiles of keys through a ring in shared memory with tensor-map copies,
 // swizzled; the others wait for a tile and hand its place back, and meet only at an item's end.  Rows of a box behind the
-// sequence's end are copied too: their scores are masked, and elements of V that are not finite never meet a weight of zero
-// (see `edge`).  With up to 16 rows the four warps take a quarter of a tile's keys each and have a running maximum, sum and
+// sequence's end are copied too: their scores are masked and their V rows made zeros.  With up to 16 rows the four warps take a quarter of a tile's keys each and have a running maximum, sum and
 // accumulator of their own, joined once at the end of the piece; with more rows (up to 64 per CTA) two or four warps share
 // the keys and differ in their rows.
 //
@@ -49,7 +48,8 @@ struct PagedAttnParams {
   int64_t o_sb, o_sh, o_sl;
   float* M;  // [B, Hq, T] or null
   float* L;
-  float* part;  // workspace of the split form
+  float* part;  // workspace of the split form: the CTAs' pieces,
+  int4* heads;  // and what begins in a CTA's range and goes on behind it: sequence, head and row tile, pieces (0: none), slot
   int32_t* status;
   int B, Hkv, G, T, R;  // R = T * G rows per (sequence, key head)
   int RT;               // row tiles
@@ -145,13 +145,17 @@ struct Geo {
   static constexpr int STAGES = WIDE ? 65536 / STAGE : (CTAS == 3 ? 65536 : 98304) / STAGE;
   static constexpr int SCALE_STAGE = Q8 ? KT * 2 : 0;
   static constexpr int WIDE_BYTES = WIDE ? 2 * KT * D * 2 : 0;
-  static constexpr int RING = STAGES * (STAGE + SCALE_STAGE) + WIDE_BYTES;
+  // Queries come with an item's first tile where they are few; otherwise their readers load them.
+  static constexpr int QROW = D * 2 + 16;                 // a row's bytes, padded so that eight rows differ in their banks
+  static constexpr int Q_STAGE = WR == 1 ? 8 * NB * QROW : 0;
+  static constexpr int WIDE_AT = STAGES * (STAGE + SCALE_STAGE), Q_AT = WIDE_AT + WIDE_BYTES;
+  static constexpr int RING = Q_AT + STAGES * Q_STAGE;
   // what the matrix instructions' operands are read from: rows of 16-bit elements in sub-tiles of 128 bytes, or the stage
   static constexpr int OS = WIDE ? 128 : RS, OSUB = KT * OS;
   static constexpr int RW = 8 * NB;                       // rows per warp
   static constexpr int RC = RW * WR;                      // rows per CTA
-  static constexpr int ML = 4 * RW * 2 * 4;               // maxima and sums of the four warps' rows
-  static constexpr int SMEM = RING + ML + 64 + 2 * STAGES * 8 + 16 + 1024;  // and the start's alignment
+  static constexpr int ML = 4 * RW * 2;                   // maxima and sums of the four warps' rows, floats; twice
+  static constexpr int SMEM = RING + 2 * ML * 4 + 2 * STAGES * 8 + 16 + 1024;  // and the start's alignment
   static_assert(4 * RW * D * 4 <= (WIDE ? WIDE_BYTES : STAGE), "the warps' accumulators are joined in a consumed tile");
 };
 
@@ -176,18 +180,21 @@ __device__ __forceinline__ int tiles_of(int len) {
   return max(1, (len + KT - 1) / KT);
 }
 
-// The line of all tiles, shared by the CTAs: prefix sums over the sequences, one pass by the whole CTA.
-struct Line {
-  int64_t total;
-  int nc;  // CTAs that have tiles
+// All tiles of all items lie on a line that the CTAs share evenly.  What CTA `c` takes of it, worked out by every warp for
+// itself: prefix sums over the sequences, a few of them per lane.
+struct Range {
+  int64_t total, start;
+  int nc, nt;          // CTAs that have tiles, tiles of this one (0: none)
+  int64_t item_start;  // of the item at `start`
 };
+__device__ __forceinline__ int64_t range_start(int64_t total, int nc, int c) {
+  return total < 1 << 20 ? (int64_t)((uint32_t)total * (uint32_t)c / (uint32_t)nc) : total * c / nc;  // c <= nc < 2^12
+}
 
 template <int KT>
-__device__ __forceinline__ Line line_scan(const PagedAttnParams& p, int ctas, int64_t* sm, int64_t& excl, int& b0, int& b1) {
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int per = (p.B + kThreads - 1) / kThreads;
-  b0 = min(tid * per, p.B);
-  b1 = min(b0 + per, p.B);
+__device__ __forceinline__ Range warp_range(const PagedAttnParams& p, int ctas, int c, Cursor& cur) {
+  const int lane = threadIdx.x & 31;
+  const int per = (p.B + 31) / 32, b0 = min(lane * per, p.B), b1 = min(b0 + per, p.B);
   const int HR = p.Hkv * p.RT;
   int64_t mine = 0;
   for (int b = b0; b < b1; ++b) mine += (int64_t)tiles_of<KT>(length_of(p, b)) * HR;
@@ -197,49 +204,34 @@ __device__ __forceinline__ Line line_scan(const PagedAttnParams& p, int ctas, in
     const int64_t x = __shfl_up_sync(0xffffffffu, inc, d);
     if (lane >= d) inc += x;
   }
-  if (lane == 31) sm[warp] = inc;
-  __syncthreads();
-  int64_t before = 0, total = 0;
-#pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    if (w < warp) before += sm[w];
-    total += sm[w];
-  }
-  excl = before + inc - mine;
-  Line l;
-  l.total = total;
-  l.nc = (int)(total < ctas ? total : ctas);
-  return l;
-}
-__device__ __forceinline__ int64_t range_start(const Line& l, int c) { return l.total * c / l.nc; }
-
-// The item and tile at place x of the line, and the place of the item's first tile; by the whole CTA.
-template <int KT>
-__device__ __forceinline__ Cursor line_locate(const PagedAttnParams& p, int64_t x, int64_t excl, int b0, int b1, int64_t* sm,
-                                              int64_t& item_start) {
-  const int HR = p.Hkv * p.RT;
-  int64_t at = excl;
-  __syncthreads();
-  for (int b = b0; b < b1; ++b) {
-    const int len = length_of(p, b), n = tiles_of<KT>(len);
-    const int64_t end = at + (int64_t)n * HR;
-    if (x >= at && x < end) {
-      sm[0] = b;
-      sm[1] = at;
-      sm[2] = len;
+  Range r;
+  r.total = __shfl_sync(0xffffffffu, inc, 31);
+  r.nc = (int)(r.total < ctas ? r.total : ctas);
+  r.nt = 0;
+  if (c >= r.nc) return r;
+  r.start = range_start(r.total, r.nc, c);
+  r.nt = (int)(range_start(r.total, r.nc, c + 1) - r.start);
+  int64_t at = inc - mine;
+  int b = 0, len = 0;
+  const bool here = r.start >= at && r.start < inc;
+  if (here) {
+    for (b = b0;; ++b) {
+      len = length_of(p, b);
+      const int64_t end = at + (int64_t)tiles_of<KT>(len) * HR;
+      if (r.start < end) break;
+      at = end;
     }
-    at = end;
   }
-  __syncthreads();
-  Cursor c;
-  c.b = (int)sm[0];
-  c.len = (int)sm[2];
-  c.ntile = tiles_of<KT>(c.len);
-  const int64_t in = x - sm[1];
-  c.hr = (int)(in / c.ntile);
-  c.tile = (int)(in - (int64_t)c.hr * c.ntile);
-  item_start = sm[1] + (int64_t)c.hr * c.ntile;
-  return c;
+  const int from = __ffs(__ballot_sync(0xffffffffu, here)) - 1;
+  cur.b = __shfl_sync(0xffffffffu, b, from);
+  cur.len = __shfl_sync(0xffffffffu, len, from);
+  at = __shfl_sync(0xffffffffu, at, from);
+  cur.ntile = tiles_of<KT>(cur.len);
+  const uint32_t in = (uint32_t)(r.start - at);  // below 2^24 tiles times 2^24 items in all, far below here
+  cur.hr = (int)(in / (uint32_t)cur.ntile);
+  cur.tile = (int)(in - (uint32_t)cur.hr * (uint32_t)cur.ntile);
+  r.item_start = r.start - cur.tile;
+  return r;
 }
 template <int KT>
 __device__ __forceinline__ void advance(const PagedAttnParams& p, Cursor& c) {
@@ -279,8 +271,15 @@ __device__ __forceinline__ void loader(const CUtensorMap& mk, const CUtensorMap&
     if (issued >= X::STAGES && !mbar_wait(&empty[stage], phase ^ 1, w, DEV_TIMEOUT_PRODUCER)) break;
     const int key0 = cur.tile * X::KT;
     const int boxes = min(X::KT / p.box, (cur.len - key0 + p.box - 1) / p.box);  // 0 for an empty sequence
-    if (lane == 0) mbar_arrive_expect_tx(&full[stage], boxes * box_bytes);
+    const int r0 = cur.hr % p.RT * X::RC;
+    const int queries = X::Q_STAGE && (issued == 0 || cur.tile == 0) ? min(X::RC, p.R - r0) : 0;
+    if (lane == 0) mbar_arrive_expect_tx(&full[stage], boxes * box_bytes + queries * D * 2);
     __syncwarp();
+    if (lane < queries) {
+      const int t = (r0 + lane) / p.G, head = cur.hr / p.RT * p.G + r0 + lane - t * p.G;
+      bulk_load(smem_u32(ring + X::Q_AT + stage * X::Q_STAGE + lane * X::QROW), p.q + cur.b * p.q_sb + head * p.q_sh + t * p.q_sl,
+                D * 2, &full[stage]);
+    }
     if (lane < boxes) {
       const uint32_t grp = (uint32_t)(key0 + lane * p.box) >> 4, pg = page_of_group(p.c, grp);
       const int row = (int)(grp - pg * p.c.groups) * 16, h = cur.hr / p.RT;
@@ -385,9 +384,9 @@ __device__ __forceinline__ void weigh(State<D, NB>& st, const float (&sc)[NK][NB
   }
 }
 
-// Whether any of a step's V elements is not finite; by the whole warp.
+// Whether any element of a step's first `rows` V rows is not finite; by the whole warp.
 template <class X, bool Q8, int NS>
-__device__ __forceinline__ bool any_odd(uint32_t vs, int s0) {
+__device__ __forceinline__ bool any_odd(uint32_t vs, int s0, int rows) {
   const int lane = threadIdx.x & 31;
   uint32_t hit = 0;
 #pragma unroll
@@ -397,7 +396,7 @@ __device__ __forceinline__ bool any_odd(uint32_t vs, int s0) {
       const uint4 x = lds128(vs + s * X::SUB + s0 * X::RS + i * 512 + lane * 16);
       const uint32_t w[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
+      for (int j = 0; j < 4 && (i * 512 + lane * 16) / X::RS < rows; ++j)
         hit |= Q8 ? ((w[j] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u : ((w[j] & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
     }
   }
@@ -451,9 +450,9 @@ __global__ void __launch_bounds__(kAllThreads, (Geo<D, Q8, NB, WR>::CTAS))
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const uint32_t ring = smem_u32(smem);
-  float* ml = reinterpret_cast<float*>(smem + X::RING);
-  int64_t* scan = reinterpret_cast<int64_t*>(smem + X::RING + X::ML);
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + X::RING + X::ML + 64);
+  float* const ml_first = reinterpret_cast<float*>(smem + X::RING);
+  float* ml = ml_first;
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + X::RING + 2 * X::ML * 4);
   uint64_t* empty = full + X::STAGES;
   int* abort_flag = reinterpret_cast<int*>(empty + X::STAGES);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -472,31 +471,28 @@ __global__ void __launch_bounds__(kAllThreads, (Geo<D, Q8, NB, WR>::CTAS))
   }
   __syncthreads();
   griddep_wait();
+  if (p.split) griddep_launch_dependents();
+  if (warp > 4) {
+    setmaxnreg_dec<24>();
+    return;
+  }
   Cursor cons;
-  int nt;
-  bool whole_first = true;  // whether the CTA's first piece begins at its item's start
+  Range range;
   if (p.split) {
-    griddep_launch_dependents();
-    int64_t excl, item_start;
-    int b0, b1;
-    const Line line = line_scan<X::KT>(p, (int)gridDim.x, scan, excl, b0, b1);
-    const int c = blockIdx.x;
-    if (c >= line.nc) return;
-    const int64_t start = range_start(line, c);
-    nt = (int)(range_start(line, c + 1) - start);
-    cons = line_locate<X::KT>(p, start, excl, b0, b1, scan, item_start);
-    whole_first = item_start == start;
+    range = warp_range<X::KT>(p, (int)gridDim.x, blockIdx.x, cons);
   } else {
     const int HR = p.Hkv * p.RT;
     cons.b = blockIdx.x / HR;
     cons.hr = blockIdx.x - cons.b * HR;
     cons.tile = 0;
     cons.len = length_of(p, cons.b);
-    cons.ntile = nt = tiles_of<X::KT>(cons.len);
+    cons.ntile = range.nt = tiles_of<X::KT>(cons.len);
+    range.item_start = range.start = 0;
   }
-  if (warp >= 4) {
+  const int nt = range.nt;
+  if (warp == 4) {
     setmaxnreg_dec<24>();
-    if (warp == 4) loader<X, D, Q8>(mk, mv, p, cons, nt, smem, full, empty, wait);
+    loader<X, D, Q8>(mk, mv, p, cons, nt, smem, full, empty, wait);
     return;
   }
   setmaxnreg_inc<X::COMPUTE_REGS>();
@@ -506,12 +502,15 @@ __global__ void __launch_bounds__(kAllThreads, (Geo<D, Q8, NB, WR>::CTAS))
   float qs[NB][2];      // factor from the raw product to log2 units, per row
   int limit[NB][2];     // keys that the row sees
   int see_all = 0;      // keys that every row of the item sees
+  const bool whole_first = range.item_start == range.start;  // the CTA's first piece begins at its item's start
   bool first_piece = true, fresh = true, alive = true;
+  int4 head = make_int4(0, 0, 0, 0);
   int stage = 0;
   uint32_t phase = 0;
 
   for (int i = 0; i < nt; ++i) {
     const int rt = cons.hr % p.RT, h = cons.hr / p.RT;
+    if (X::Q_STAGE) alive = alive && mbar_wait(&full[stage], phase, wait, DEV_TIMEOUT_SOFTMAX);
     if (fresh) {
       fresh = false;
       see_all = p.causal ? cons.len - p.T + 1 : cons.len;
@@ -531,7 +530,9 @@ __global__ void __launch_bounds__(kAllThreads, (Geo<D, Q8, NB, WR>::CTAS))
         const int r = rt * X::RC + wr * X::RW + nb * 8 + g8;
         const bool live = r < p.R;
         const int t = live ? r / p.G : 0, g = live ? r - t * p.G : 0;
-        const __nv_bfloat16* src = p.q + cons.b * p.q_sb + (int64_t)(h * p.G + g) * p.q_sh + t * p.q_sl;
+        const __nv_bfloat16* src =
+            X::Q_STAGE ? reinterpret_cast<const __nv_bfloat16*>(smem + X::Q_AT + stage * X::Q_STAGE + (nb * 8 + g8) * X::QROW)
+                       : p.q + cons.b * p.q_sb + (int64_t)(h * p.G + g) * p.q_sh + t * p.q_sl;
         if constexpr (!Q8) {
 #pragma unroll
           for (int kk = 0; kk < D / 16; ++kk) {
@@ -581,12 +582,12 @@ __global__ void __launch_bounds__(kAllThreads, (Geo<D, Q8, NB, WR>::CTAS))
         }
       }
     }
-    alive = alive && mbar_wait(&full[stage], phase, wait, DEV_TIMEOUT_SOFTMAX);
+    if (!X::Q_STAGE) alive = alive && mbar_wait(&full[stage], phase, wait, DEV_TIMEOUT_SOFTMAX);
 
     const bool idle = rt * X::RC + wr * X::RW >= p.R || !alive;  // none of the warp's rows exists
     const uint32_t raw_v = ring + stage * X::STAGE + X::KT * X::RB;
     const uint32_t ss = ring + X::STAGES * X::STAGE + stage * X::SCALE_STAGE;
-    const uint32_t ks = X::WIDE ? ring + X::STAGES * (X::STAGE + X::SCALE_STAGE) : ring + stage * X::STAGE;
+    const uint32_t ks = X::WIDE ? ring + X::WIDE_AT : ring + stage * X::STAGE;
     const uint32_t vs = ks + X::SUBS * X::KT * (X::WIDE ? D * 2 : X::RS);
     if constexpr (X::WIDE) {
       constexpr int CPR = X::RB / 16;
@@ -594,7 +595,8 @@ __global__ void __launch_bounds__(kAllThreads, (Geo<D, Q8, NB, WR>::CTAS))
 #pragma unroll
       for (int j = 0; j < 2 * X::KT * CPR / kThreads; ++j) {
         const int at = j * kThreads + tid, row = at / CPR % X::KT, c = at % CPR, v = at / (CPR * X::KT);
-        const uint4 w = lds128(ring + stage * X::STAGE + v * X::KT * X::RB + row * X::RB + ((c ^ swizzle_of<X::RS>(row)) << 4));
+        uint4 w = lds128(ring + stage * X::STAGE + v * X::KT * X::RB + row * X::RB + ((c ^ swizzle_of<X::RS>(row)) << 4));
+        if (v && cons.tile * X::KT + row >= cons.len) w = make_uint4(0u, 0u, 0u, 0u);  // behind the sequence's end: anything
         uint32_t o[8];
         widen4(w.x, o[0], o[1]);
         widen4(w.y, o[2], o[3]);
@@ -610,6 +612,14 @@ __global__ void __launch_bounds__(kAllThreads, (Geo<D, Q8, NB, WR>::CTAS))
     for (int s0 = wk * KW; s0 < (wk + 1) * KW; s0 += NS) {
       const int key0 = cons.tile * X::KT + s0;
       if (key0 >= cons.len || idle) break;  // the same for the whole warp
+      const int rows = cons.len - key0;  // of the step's keys
+      if (!X::WIDE && rows < NS) {
+        // V rows behind the sequence's end become zeros: what a copy brought along or an earlier tile left may be anything
+#pragma unroll
+        for (int s = 0; s < X::SUBS; ++s)
+          for (int at = rows * X::RS + lane * 16; at < NS * X::RS; at += 512) sts128(vs + s * X::SUB + s0 * X::RS + at, 0, 0, 0, 0);
+        __syncwarp();
+      }
       // scores, transposed: a thread has keys lane / 4 and + 8 of every 16, two rows of every 8
       float sc[NK][NB][4];
 #pragma unroll
@@ -746,7 +756,7 @@ __global__ void __launch_bounds__(kAllThreads, (Geo<D, Q8, NB, WR>::CTAS))
       }
       // In a step that some row does not see all of, elements of V that are not finite come in row by row: a weight of zero
       // would make NaN of them in rows that do not see them.
-      if (edge && any_odd<X, Q8, NS>(raw_v, s0)) {
+      if (edge && any_odd<X, Q8, NS>(raw_v, s0, rows)) {
         weigh<X, D, Q8, NB, NK, true>(st, sc, vs, s0);
         State<D, NB> st2 = st;
         float w[NK][NB][4];
@@ -780,7 +790,7 @@ __global__ void __launch_bounds__(kAllThreads, (Geo<D, Q8, NB, WR>::CTAS))
         }
       compute_sync();
       // [warp][row][D]; elements are XORed with 8 times bits 1 and 2 of the row, so that a warp's rows differ in their banks
-      float* buf = reinterpret_cast<float*>(smem + (X::WIDE ? X::STAGES * (X::STAGE + X::SCALE_STAGE) : stage * X::STAGE));
+      float* buf = reinterpret_cast<float*>(smem + (X::WIDE ? X::WIDE_AT : stage * X::STAGE));
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
@@ -848,95 +858,89 @@ __global__ void __launch_bounds__(kAllThreads, (Geo<D, Q8, NB, WR>::CTAS))
           if (e0 == 0) *reinterpret_cast<float2*>(dst + X::RC * D + row * 2) = make_float2(top, sum);
         }
       }
+      if (!last && (!first_piece || whole_first)) {  // the head of an item that later CTAs go on with
+        const int64_t item_end = range.start + i + 1 + (cons.ntile - 1 - cons.tile);
+        int to = (int)((item_end - 1) * range.nc / range.total);
+        while (range_start(range.total, range.nc, to + 1) < item_end) ++to;
+        while (range_start(range.total, range.nc, to) >= item_end) --to;
+        head = make_int4(cons.b, cons.hr, to - (int)blockIdx.x + 1, slot);
+      }
       first_piece = false;
       fresh = true;
-      compute_sync();            // the maxima and sums are read before the next item's are written
-      fence_proxy_async_smem();  // and the stage is written before the next copy into it
+      ml = ml_first + (ml == ml_first ? X::ML : 0);  // a slow warp may still read this item's
+      fence_proxy_async_smem();                      // the stage is written before the next copy into it
     }
     __syncwarp();
     if (lane == 0) mbar_arrive(&empty[stage]);
     if (++stage == X::STAGES) stage = 0, phase ^= 1;
     advance<X::KT>(p, cons);
   }
+  if (p.split && tid == 0) p.heads[blockIdx.x] = head;
 }
 
-// Joins the pieces of the item that begins in CTA x's range and goes on behind it: a warp per row, pieces in order.
-template <int D, int KT>
-__global__ void __launch_bounds__(kThreads) paged_join_kernel(const __grid_constant__ PagedAttnParams p, int ctas, int rc) {
-  __shared__ int64_t scan[8];
-  const int c = blockIdx.x, lane = threadIdx.x & 31;
-  // The lengths were there before the pieces' kernel began; only the pieces have to be waited for.
-  int64_t excl, item_start;
-  int b0, b1;
-  const Line line = line_scan<KT>(p, ctas, scan, excl, b0, b1);
-  if (c >= line.nc) return;
-  const int64_t start = range_start(line, c), end = range_start(line, c + 1);
-  const Cursor it = line_locate<KT>(p, end - 1, excl, b0, b1, scan, item_start);
-  const int64_t item_end = item_start + it.ntile;
-  if (item_start < start || item_end <= end) return;  // begins in another range, or ends in this one
-  // The last CTA of the item: the one whose range holds item_end - 1.
-  int last = (int)((item_end - 1) * line.nc / line.total);
-  while (range_start(line, last + 1) < item_end) ++last;
-  while (range_start(line, last) >= item_end) --last;
-  griddep_wait();
-  const int rt = it.hr % p.RT, h = it.hr / p.RT;
-  const int row = blockIdx.y * 4 + (threadIdx.x >> 5);
-  const int r = rt * rc + row;
-  if (row >= rc || r >= p.R) return;
-  const int64_t slot_floats = rc * (D + 2);
-  const int n = last - c + 1;
-  // piece 0 is slot 0 of this CTA if it is also its first piece, else slot 1; every later one is slot 0 of its CTA
-  const float* first = p.part + ((int64_t)c * kSlotsPerCta + (item_start == start ? 0 : 1)) * slot_floats;
-  const float* later = p.part + (int64_t)c * kSlotsPerCta * slot_floats;
-  float top = -INFINITY;
-  for (int i = lane; i < n; i += 32) {
-    const float* s = i == 0 ? first : later + (int64_t)i * kSlotsPerCta * slot_floats;
-    top = fmaxf(top, s[rc * D + row * 2]);
-  }
-#pragma unroll
-  for (int d = 16; d >= 1; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+// Joins the pieces of the item that begins in CTA x's range and goes on behind it: four warps share a row's pieces, each
+// adds its own in order, and the four sums are added in order.
+template <int D>
+__global__ void __launch_bounds__(kThreads) paged_join_kernel(const __grid_constant__ PagedAttnParams p, int rc) {
   constexpr int E = D / 32;
-  float acc[E] = {}, sum = 0.f;
-  for (int i0 = 0; i0 < n; i0 += 32) {
-    float f = 0.f, lsum = 0.f;
-    if (i0 + lane < n) {
-      const float* s = i0 + lane == 0 ? first : later + (int64_t)(i0 + lane) * kSlotsPerCta * slot_floats;
-      const float2 x = *reinterpret_cast<const float2*>(s + rc * D + row * 2);
-      f = x.x == -INFINITY ? 0.f : exp2f(x.x - top);
-      lsum = x.y * f;
+  __shared__ float sums[4][D];
+  const int c = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  griddep_wait();
+  const int4 it = p.heads[c];
+  const int n = it.z;
+  if (n == 0) return;
+  const int rt = it.y % p.RT, h = it.y / p.RT, rows = min(rc, p.R - rt * rc);
+  const int64_t slot_floats = rc * (D + 2);
+  // the first piece lies in the CTA's slot it.w, every later one in slot 0 of its CTA
+  const float* first = p.part + ((int64_t)c * kSlotsPerCta + it.w) * slot_floats;
+  const float* later = p.part + (int64_t)c * kSlotsPerCta * slot_floats;
+  for (int row = blockIdx.y; row < rows; row += gridDim.y) {
+    float top = -INFINITY;
+    for (int i = lane; i < n; i += 32) {
+      const float* s = i == 0 ? first : later + (int64_t)i * kSlotsPerCta * slot_floats;
+      top = fmaxf(top, s[rc * D + row * 2]);
     }
-    const int m = min(32, n - i0);
-#pragma unroll 8
-    for (int i = 0; i < m; ++i) {
-      const float* s = i0 + i == 0 ? first : later + (int64_t)(i0 + i) * kSlotsPerCta * slot_floats;
-      const float g = __shfl_sync(0xffffffffu, f, i);
-      sum += __shfl_sync(0xffffffffu, lsum, i);
+#pragma unroll
+    for (int d = 16; d >= 1; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+    float acc[E] = {}, sum = 0.f;
+#pragma unroll 4
+    for (int i = warp; i < n; i += 4) {
+      const float* s = i == 0 ? first : later + (int64_t)i * kSlotsPerCta * slot_floats;
+      const float2 x = *reinterpret_cast<const float2*>(s + rc * D + row * 2);
+      const float f = x.x == -INFINITY ? 0.f : exp2f(x.x - top);
+      sum = fmaf(x.y, f, sum);
       const float* src = s + row * D + lane * E;
       if constexpr (E == 4) {
         const float4 v = *reinterpret_cast<const float4*>(src);
-        acc[0] = fmaf(g, v.x, acc[0]);
-        acc[1] = fmaf(g, v.y, acc[1]);
-        acc[2] = fmaf(g, v.z, acc[2]);
-        acc[3] = fmaf(g, v.w, acc[3]);
+        acc[0] = fmaf(f, v.x, acc[0]);
+        acc[1] = fmaf(f, v.y, acc[1]);
+        acc[2] = fmaf(f, v.z, acc[2]);
+        acc[3] = fmaf(f, v.w, acc[3]);
       } else {
         const float2 v = *reinterpret_cast<const float2*>(src);
-        acc[0] = fmaf(g, v.x, acc[0]);
-        acc[1] = fmaf(g, v.y, acc[1]);
+        acc[0] = fmaf(f, v.x, acc[0]);
+        acc[1] = fmaf(f, v.y, acc[1]);
       }
     }
-  }
-  const float inv = top == -INFINITY ? 0.f : 1.f / sum;
-  const int t = r / p.G, head = h * p.G + r - t * p.G;
-  __nv_bfloat16* dst = p.o + it.b * p.o_sb + head * p.o_sh + t * p.o_sl + lane * E;
-  if constexpr (E == 4) {
-    *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16x2(acc[0] * inv, acc[1] * inv), pack_bf16x2(acc[2] * inv, acc[3] * inv));
-  } else {
-    *reinterpret_cast<uint32_t*>(dst) = pack_bf16x2(acc[0] * inv, acc[1] * inv);
-  }
-  if (p.M && lane == 0) {
-    const int64_t at = ((int64_t)it.b * p.Hkv * p.G + head) * p.T + t;
-    p.M[at] = top;
-    p.L[at] = sum;
+#pragma unroll
+    for (int e = 0; e < E; ++e) sums[warp][lane * E + e] = acc[e];
+    __shared__ float row_sum[4];
+    if (lane == 0) row_sum[warp] = sum;
+    __syncthreads();
+    const int r = rt * rc + row, t = r / p.G, head = h * p.G + r - t * p.G;
+    const float total = (row_sum[0] + row_sum[1]) + (row_sum[2] + row_sum[3]);
+    if (tid < D / 2) {
+      const float inv = top == -INFINITY ? 0.f : 1.f / total;  // a row that sees no key gives 0
+      const float a = (sums[0][2 * tid] + sums[1][2 * tid]) + (sums[2][2 * tid] + sums[3][2 * tid]);
+      const float b = (sums[0][2 * tid + 1] + sums[1][2 * tid + 1]) + (sums[2][2 * tid + 1] + sums[3][2 * tid + 1]);
+      *reinterpret_cast<uint32_t*>(p.o + it.x * p.o_sb + head * p.o_sh + t * p.o_sl + 2 * tid) = pack_bf16x2(a * inv, b * inv);
+    }
+    if (p.M && tid == 0) {
+      const int64_t at = ((int64_t)it.x * p.Hkv * p.G + head) * p.T + t;
+      p.M[at] = top;
+      p.L[at] = total;
+    }
+    __syncthreads();
   }
 }
 
@@ -967,7 +971,7 @@ int plan_of(int B, int Hq, int Hkv, int T, int D, bool q8, int max_len, int sms,
   out->rt = (int)rt;
   out->split = tiles > 2;
   out->ctas = out->split ? ctas_per_sm(D, q8, out->nb) * sms : (int)items;
-  out->workspace = out->split ? (int64_t)out->ctas * kSlotsPerCta * rc * (D + 2) * 4 : 0;
+  out->workspace = out->split ? (int64_t)out->ctas * (kSlotsPerCta * rc * (D + 2) * 4 + 16) : 0;
   return LVAR_OK;
 }
 
@@ -989,10 +993,10 @@ int launch(const PagedAttnParams& p, const CUtensorMap& mk, const CUtensorMap& m
   LVAR_CUDA_OK(cudaLaunchKernelEx(&cfg, kern, mk, mv, p));
   if (plan.split) {
     const int rows = p.R < X::RC ? p.R : X::RC;
-    cfg.gridDim = dim3((unsigned)plan.ctas, (unsigned)((rows + 3) / 4));
+    cfg.gridDim = dim3((unsigned)plan.ctas, (unsigned)(rows < 8 ? rows : 8));
     cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = 0;
-    LVAR_CUDA_OK(cudaLaunchKernelEx(&cfg, paged_join_kernel<D, X::KT>, p, plan.ctas, X::RC));
+    LVAR_CUDA_OK(cudaLaunchKernelEx(&cfg, paged_join_kernel<D>, p, X::RC));
   }
   return LVAR_OK;
 }
@@ -1059,6 +1063,7 @@ int launch_paged_attn(const lvar_paged_attn_args* a, cudaStream_t stream) {
   p.o_sb = a->o_sb; p.o_sh = a->o_sh; p.o_sl = a->o_sl;
   p.M = a->M; p.L = a->L;
   p.part = static_cast<float*>(a->workspace);
+  p.heads = reinterpret_cast<int4*>(p.part + (int64_t)plan.ctas * kSlotsPerCta * 8 * plan.nb * plan.wr * (c.D + 2));
   p.status = a->dev_status;
   p.B = c.B; p.Hkv = c.Hkv; p.G = a->Hq / c.Hkv; p.T = a->T; p.R = a->T * p.G;
   p.RT = plan.rt;
