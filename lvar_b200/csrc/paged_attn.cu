@@ -24,8 +24,8 @@
 // for elements 2^-24 below the row's largest).  K's row scale multiplies the score.  V's row scale 2^e joins the exponent
 // of the weight, w = exp2(s + e - running maximum of (s + e)), so that the fp16 weights are always taken relative to the
 // largest CONTRIBUTION; the row sum keeps a maximum of its own.
-// Weights are rounded once, to bf16 (bf16 cache) or fp16 scaled by 2^15 (e4m3 cache); sums, maxima and accumulators are
-// fp32.
+// Weights are rounded once, to bf16 (bf16 cache) or fp16 (e4m3 cache; scaled by 2^7, so that only weights 2^-21 of the
+// largest or less are subnormal); sums, maxima and accumulators are fp32.
 #include <math.h>
 
 #include "paged.cuh"
@@ -38,6 +38,7 @@ namespace {
 constexpr int kThreads = 128;     // threads that compute: a warpgroup
 constexpr int kAllThreads = 256;  // and one whose first warp loads; its registers go to the first
 constexpr int kSlotsPerCta = 2;
+constexpr float kUp = 7.f;  // fp16 weights are scaled by 2^7; with 2^8 above the reference they end at 2^15
 
 struct PagedAttnParams {
   PagedView c;
@@ -250,8 +251,10 @@ __device__ __forceinline__ void advance(const PagedAttnParams& p, Cursor& c) {
 template <int D, int NB>
 struct State {
   float acc[D / 16][NB][4];  // [0], [1]: the two rows at a tile's first element of D, [2], [3]: at its second
-  float m[NB][2], l[NB][2];  // maximum of the scores (log2 units) and this thread's part of the sum of exp2(s - m)
-  float mt[NB][2];           // e4m3: maximum of score + V exponent, which the accumulators are relative to
+  // scores in log2 units: this thread's maximum, the reference of its part `l` of the sum of exp2(s - ref) and, in bf16, of
+  // the accumulators; e4m3: the same of score + V exponent, the reference of the accumulators
+  float mx[NB][2], ref[NB][2], l[NB][2];
+  float tmx[NB][2], tref[NB][2];
 };
 template <int D, bool RAW8>
 __device__ __forceinline__ int element_of(int tile, int second) {
@@ -445,7 +448,7 @@ __global__ void __launch_bounds__(kAllThreads, (Geo<D, Q8, NB, WR>::CTAS))
   using X = Geo<D, Q8, NB, WR>;
   constexpr int WK = 4 / WR;              // warps that share a row tile and differ in their keys
   constexpr int KW = X::KT / WK;          // keys of a tile per warp
-  constexpr int NS = KW < 32 ? KW : 32;   // keys per step
+  constexpr int NS = WR == 1 ? (KW < 32 ? KW : 32) : KW < 64 ? KW : 64;  // keys per step
   constexpr int NK = NS / 16;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -520,7 +523,7 @@ __global__ void __launch_bounds__(kAllThreads, (Geo<D, Q8, NB, WR>::CTAS))
         for (int t = 0; t < D / 16; ++t) st.acc[t][nb][0] = st.acc[t][nb][1] = st.acc[t][nb][2] = st.acc[t][nb][3] = 0.f;
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          st.m[nb][e] = st.mt[nb][e] = -INFINITY;
+          st.mx[nb][e] = st.ref[nb][e] = st.tmx[nb][e] = st.tref[nb][e] = -INFINITY;
           st.l[nb][e] = 0.f;
           const int r = rt * X::RC + wr * X::RW + nb * 8 + quad * 2 + e;
           limit[nb][e] = r >= p.R ? 0 : p.causal ? cons.len - p.T + r / p.G + 1 : cons.len;
@@ -688,31 +691,58 @@ __global__ void __launch_bounds__(kAllThreads, (Geo<D, Q8, NB, WR>::CTAS))
             for (int e = 0; e < 4; ++e)
               if (key0 + k * 16 + (e >> 1) * 8 + g8 >= limit[nb][e & 1]) sc[k][nb][e] = -INFINITY;
       }
-      // running maximum and sum; weights
-      float alpha[NB][2];
-      bool moved = false;
+      // Weights relative to a reference that a row's scores have exceeded by at most 2^8: it moves to the maximum only when
+      // they would, which is rare after an item's first step and spares every other one the exchange between lanes.
+      bool grown = false;
 #pragma unroll
-      for (int nb = 0; nb < NB; ++nb) {
-        float mx[2] = {-INFINITY, -INFINITY}, tx[2] = {-INFINITY, -INFINITY}, mu[2], tu[2];
-#pragma unroll
-        for (int k = 0; k < NK; ++k) {
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            mx[e] = fmax3(mx[e], sc[k][nb][e], sc[k][nb][2 + e]);
-            if constexpr (Q8) tx[e] = fmax3(tx[e], sc[k][nb][e] + ve[k][0], sc[k][nb][2 + e] + ve[k][1]);
-          }
-        }
+      for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          mx[e] = max_of_keys(mx[e]);
-          mx[e] = fmaxf(st.m[nb][e], Q8 ? mx[e] : mx[e] * qs[nb][e]);
-          mu[e] = mx[e] == -INFINITY ? 0.f : -mx[e];
-          if constexpr (Q8) {
-            tx[e] = fmaxf(st.mt[nb][e], max_of_keys(tx[e]));
-            tu[e] = tx[e] == -INFINITY ? 0.f : 15.f - tx[e];  // weights up to 2^15
+          float raw = -INFINITY;
+#pragma unroll
+          for (int k = 0; k < NK; ++k) {
+            raw = fmax3(raw, sc[k][nb][e], sc[k][nb][2 + e]);
+            if constexpr (Q8) st.tmx[nb][e] = fmax3(st.tmx[nb][e], sc[k][nb][e] + ve[k][0], sc[k][nb][2 + e] + ve[k][1]);
           }
+          st.mx[nb][e] = fmaxf(st.mx[nb][e], Q8 ? raw : raw * qs[nb][e]);
+          grown = grown || st.mx[nb][e] > st.ref[nb][e] + 8.f;
+          if constexpr (Q8) grown = grown || st.tmx[nb][e] > st.tref[nb][e] + 8.f;
         }
-        uint64_t add = 0;
+      if (__any_sync(0xffffffffu, grown)) {
+        float alpha[NB][2];
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            st.mx[nb][e] = max_of_keys(st.mx[nb][e]);
+            float f = st.mx[nb][e] == -INFINITY ? 1.f : fast_exp2(st.ref[nb][e] - st.mx[nb][e]);
+            st.l[nb][e] *= f;
+            st.ref[nb][e] = st.mx[nb][e];
+            if constexpr (Q8) {
+              st.tmx[nb][e] = max_of_keys(st.tmx[nb][e]);
+              f = st.tmx[nb][e] == -INFINITY ? 1.f : fast_exp2(st.tref[nb][e] - st.tmx[nb][e]);
+              st.tref[nb][e] = st.tmx[nb][e];
+            }
+            alpha[nb][e] = f;
+          }
+#pragma unroll
+        for (int t = 0; t < D / 16; ++t)
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+            for (int y = 0; y < 2; ++y)
+              unpack_f32x2(fmul2(pack_f32x2(st.acc[t][nb][2 * y], st.acc[t][nb][2 * y + 1]), pack_f32x2(alpha[nb][0], alpha[nb][1])),
+                           st.acc[t][nb][2 * y], st.acc[t][nb][2 * y + 1]);
+      }
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
+        float mu[2], tu[2];  // nothing seen so far: scores stay -inf
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          mu[e] = st.ref[nb][e] == -INFINITY ? 0.f : -st.ref[nb][e];
+          if constexpr (Q8) tu[e] = st.tref[nb][e] == -INFINITY ? 0.f : kUp - st.tref[nb][e];
+        }
+        uint64_t add = pack_f32x2(st.l[nb][0], st.l[nb][1]);
 #pragma unroll
         for (int k = 0; k < NK; ++k)
 #pragma unroll
@@ -732,27 +762,7 @@ __global__ void __launch_bounds__(kAllThreads, (Geo<D, Q8, NB, WR>::CTAS))
               add = fadd2(add, pack_f32x2(sc[k][nb][2 * y], sc[k][nb][2 * y + 1]));
             }
           }
-        float part[2];
-        unpack_f32x2(add, part[0], part[1]);
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const float f = fast_exp2(st.m[nb][e] + mu[e]);
-          alpha[nb][e] = Q8 ? fast_exp2(st.mt[nb][e] - (tx[e] == -INFINITY ? 0.f : tx[e])) : f;
-          moved = moved || alpha[nb][e] != 1.f;  // a NaN counts
-          st.l[nb][e] = fmaf(st.l[nb][e], f, part[e]);
-          st.m[nb][e] = mx[e];
-          if constexpr (Q8) st.mt[nb][e] = tx[e];
-        }
-      }
-      if (__any_sync(0xffffffffu, moved)) {
-#pragma unroll
-        for (int t = 0; t < D / 16; ++t)
-#pragma unroll
-          for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-            for (int y = 0; y < 2; ++y)
-              unpack_f32x2(fmul2(pack_f32x2(st.acc[t][nb][2 * y], st.acc[t][nb][2 * y + 1]), pack_f32x2(alpha[nb][0], alpha[nb][1])),
-                           st.acc[t][nb][2 * y], st.acc[t][nb][2 * y + 1]);
+        unpack_f32x2(add, st.l[nb][0], st.l[nb][1]);
       }
       // In a step that some row does not see all of, elements of V that are not finite come in row by row: a weight of zero
       // would make NaN of them in rows that do not see them.
@@ -784,9 +794,10 @@ __global__ void __launch_bounds__(kAllThreads, (Geo<D, Q8, NB, WR>::CTAS))
       for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          st.l[nb][e] = sum_of_keys(st.l[nb][e]);
+          const float m = max_of_keys(st.mx[nb][e]), l = sum_of_keys(st.l[nb][e]);
           if (g8 == 0)
-            *reinterpret_cast<float2*>(ml + (warp * X::RW + nb * 8 + quad * 2 + e) * 2) = make_float2(st.m[nb][e], st.l[nb][e]);
+            *reinterpret_cast<float2*>(ml + (warp * X::RW + nb * 8 + quad * 2 + e) * 2) =
+                make_float2(m, m == -INFINITY ? 0.f : l * exp2f(st.ref[nb][e] - m));
         }
       compute_sync();
       // [warp][row][D]; elements are XORed with 8 times bits 1 and 2 of the row, so that a warp's rows differ in their banks
@@ -800,7 +811,7 @@ __global__ void __launch_bounds__(kAllThreads, (Geo<D, Q8, NB, WR>::CTAS))
 #pragma unroll
           for (int w = 0; w < WK; ++w) top = fmaxf(top, ml[((w * WR + wr) * X::RW + row) * 2]);
           // an infinite maximum (an infinite score) gives NaN here, as exp(inf - inf) does
-          const float own = Q8 ? st.mt[nb][e] - 15.f : st.m[nb][e];
+          const float own = Q8 ? st.tref[nb][e] - kUp : st.ref[nb][e];
           const float f = own == -INFINITY ? 0.f : exp2f(own - top);
           float* dst = buf + (warp * X::RW + row) * D;
           if constexpr (!Q8 || X::WIDE) {
@@ -878,12 +889,11 @@ __global__ void __launch_bounds__(kAllThreads, (Geo<D, Q8, NB, WR>::CTAS))
   if (p.split && tid == 0) p.heads[blockIdx.x] = head;
 }
 
-// Joins the pieces of the item that begins in CTA x's range and goes on behind it: four warps share a row's pieces, each
-// adds its own in order, and the four sums are added in order.
+// Joins the pieces of the item that begins in CTA x's range and goes on behind it, in a fixed order.
 template <int D>
 __global__ void __launch_bounds__(kThreads) paged_join_kernel(const __grid_constant__ PagedAttnParams p, int rc) {
   constexpr int E = D / 32;
-  __shared__ float sums[4][D];
+  __shared__ float sums[4][D], row_sum[4];
   const int c = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   griddep_wait();
   const int4 it = p.heads[c];
@@ -894,7 +904,10 @@ __global__ void __launch_bounds__(kThreads) paged_join_kernel(const __grid_const
   // the first piece lies in the CTA's slot it.w, every later one in slot 0 of its CTA
   const float* first = p.part + ((int64_t)c * kSlotsPerCta + it.w) * slot_floats;
   const float* later = p.part + (int64_t)c * kSlotsPerCta * slot_floats;
-  for (int row = blockIdx.y; row < rows; row += gridDim.y) {
+  // Few pieces: a warp takes a row by itself; many: the CTA's four warps share a row's pieces.
+  const bool shared = n > 16;
+  const int ways = shared ? 4 : 1, part = shared ? warp : 0;
+  for (int row = shared ? blockIdx.y : blockIdx.y * 4 + warp; row < rows; row += shared ? gridDim.y : gridDim.y * 4) {
     float top = -INFINITY;
     for (int i = lane; i < n; i += 32) {
       const float* s = i == 0 ? first : later + (int64_t)i * kSlotsPerCta * slot_floats;
@@ -904,43 +917,52 @@ __global__ void __launch_bounds__(kThreads) paged_join_kernel(const __grid_const
     for (int d = 16; d >= 1; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
     float acc[E] = {}, sum = 0.f;
 #pragma unroll 4
-    for (int i = warp; i < n; i += 4) {
+    for (int i = part; i < n; i += ways) {
       const float* s = i == 0 ? first : later + (int64_t)i * kSlotsPerCta * slot_floats;
       const float2 x = *reinterpret_cast<const float2*>(s + rc * D + row * 2);
       const float f = x.x == -INFINITY ? 0.f : exp2f(x.x - top);
       sum = fmaf(x.y, f, sum);
       const float* src = s + row * D + lane * E;
+      float v[E];
       if constexpr (E == 4) {
-        const float4 v = *reinterpret_cast<const float4*>(src);
-        acc[0] = fmaf(f, v.x, acc[0]);
-        acc[1] = fmaf(f, v.y, acc[1]);
-        acc[2] = fmaf(f, v.z, acc[2]);
-        acc[3] = fmaf(f, v.w, acc[3]);
+        const float4 y = *reinterpret_cast<const float4*>(src);
+        v[0] = y.x, v[1] = y.y, v[2] = y.z, v[3] = y.w;
       } else {
-        const float2 v = *reinterpret_cast<const float2*>(src);
-        acc[0] = fmaf(f, v.x, acc[0]);
-        acc[1] = fmaf(f, v.y, acc[1]);
+        const float2 y = *reinterpret_cast<const float2*>(src);
+        v[0] = y.x, v[1] = y.y;
       }
-    }
 #pragma unroll
-    for (int e = 0; e < E; ++e) sums[warp][lane * E + e] = acc[e];
-    __shared__ float row_sum[4];
-    if (lane == 0) row_sum[warp] = sum;
-    __syncthreads();
-    const int r = rt * rc + row, t = r / p.G, head = h * p.G + r - t * p.G;
-    const float total = (row_sum[0] + row_sum[1]) + (row_sum[2] + row_sum[3]);
-    if (tid < D / 2) {
-      const float inv = top == -INFINITY ? 0.f : 1.f / total;  // a row that sees no key gives 0
-      const float a = (sums[0][2 * tid] + sums[1][2 * tid]) + (sums[2][2 * tid] + sums[3][2 * tid]);
-      const float b = (sums[0][2 * tid + 1] + sums[1][2 * tid + 1]) + (sums[2][2 * tid + 1] + sums[3][2 * tid + 1]);
-      *reinterpret_cast<uint32_t*>(p.o + it.x * p.o_sb + head * p.o_sh + t * p.o_sl + 2 * tid) = pack_bf16x2(a * inv, b * inv);
+      for (int e = 0; e < E; ++e) acc[e] = fmaf(f, v[e], acc[e]);
     }
-    if (p.M && tid == 0) {
+    if (shared) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) sums[warp][lane * E + e] = acc[e];
+      if (lane == 0) row_sum[warp] = sum;
+      __syncthreads();
+      if (warp == 0) {
+        sum = (row_sum[0] + row_sum[1]) + (row_sum[2] + row_sum[3]);
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          const int at = lane * E + e;
+          acc[e] = (sums[0][at] + sums[1][at]) + (sums[2][at] + sums[3][at]);
+        }
+      }
+      __syncthreads();
+      if (warp != 0) continue;
+    }
+    const int r = rt * rc + row, t = r / p.G, head = h * p.G + r - t * p.G;
+    const float inv = top == -INFINITY ? 0.f : 1.f / sum;  // a row that sees no key gives 0
+    __nv_bfloat16* dst = p.o + it.x * p.o_sb + head * p.o_sh + t * p.o_sl + lane * E;
+    if constexpr (E == 4) {
+      *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16x2(acc[0] * inv, acc[1] * inv), pack_bf16x2(acc[2] * inv, acc[3] * inv));
+    } else {
+      *reinterpret_cast<uint32_t*>(dst) = pack_bf16x2(acc[0] * inv, acc[1] * inv);
+    }
+    if (p.M && lane == 0) {
       const int64_t at = ((int64_t)it.x * p.Hkv * p.G + head) * p.T + t;
       p.M[at] = top;
-      p.L[at] = total;
+      p.L[at] = sum;
     }
-    __syncthreads();
   }
 }
 

@@ -856,7 +856,7 @@ def paged_qkv_prologue(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_page
     start_ptr = _paged_ints("start", start, B, dev)
     count_ptr = 0 if count is None else _paged_ints("count", count, B, dev)
     st = _paged_status(status, dev)
-    out = torch.empty((B, Hq, L, D), dtype=_BF16, device=q.device)
+    out = torch.empty_strided((B, Hq, L, D), (Hq * L * D, L * D, D, 1), dtype=_BF16, device=q.device)
     if B and L:
         _paged_call(lib.lvar_paged_write,
                     _PACK_WRITE(*c, q.data_ptr(), q_sb, q_sl, q_sh, k.data_ptr(), k_sb, k_sl, k_sh, v.data_ptr(), v_sb, v_sl,
@@ -880,7 +880,7 @@ def paged_kv_read(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Ten
     lens_ptr = _paged_ints("lens", lens, B, dev)
     st = _paged_status(status, dev)
     if out is None:
-        k = torch.empty(shape, dtype=_BF16, device=k_pages.device)
+        k = torch.empty_strided(shape, (shape[1] * n * shape[3], n * shape[3], shape[3], 1), dtype=_BF16, device=k_pages.device)
         v = torch.empty_like(k)
     else:
         k, v = out
@@ -925,8 +925,8 @@ def paged_attn_fwd(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
     st = _paged_status(status, dev)
     most = min(c[18] * c[14], 1 << 30) if max_len is None else int(max_len)
     if out is None:
-        o = torch.empty((B, Hq, T, D), dtype=_BF16, device=q.device)
         o_sb, o_sh, o_sl = Hq * T * D, T * D, D
+        o = torch.empty_strided((B, Hq, T, D), (o_sb, o_sh, o_sl, 1), dtype=_BF16, device=q.device)
     else:
         o = _output_like(q, out)
         o_sb, o_sh, o_sl, _ = o.stride()
@@ -939,7 +939,7 @@ def paged_attn_fwd(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
     if B and T:
         work = _paged_workspace(dev, B, Hq, H, T, D, scales is not None, most)
         if work:
-            space = torch.empty(work, dtype=_U8, device=q.device)
+            space = torch.empty_strided((work,), (1,), dtype=_U8, device=q.device)
             w_ptr = space.data_ptr()
         _paged_call(lib.lvar_paged_attn,
                     _PACK_ATTN(*c, q.data_ptr(), q_sb, q_sh, q_sl, o.data_ptr(), o_sb, o_sh, o_sl, m_ptr, l_ptr, lens_ptr, w_ptr,
