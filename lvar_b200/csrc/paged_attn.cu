@@ -57,7 +57,7 @@ struct PagedAttnParams {
   int causal, max_len;
   int split;            // 0: CTA x takes item x
   float scale_log2;
-  int box;              // rows per copy
+  int box_log2;         // rows per copy: 16 to 128
   uint64_t wait_limit_ns;
 };
 
@@ -166,8 +166,10 @@ __device__ __forceinline__ int swizzle_of(int row) {
   return RS == 64 ? (row >> 1) & 3 : row & 7;
 }
 
+// A tile of an item: sequence, key head, row tile, tile of keys.
 struct Cursor {
-  int b, hr, tile, ntile, len;
+  int b, h, rt, tile, ntile, len;
+  int next_len;  // of the sequence behind, fetched ahead
 };
 
 // Length of a sequence as the kernel uses it: inside the caller's bound and the table's.
@@ -179,6 +181,11 @@ __device__ __forceinline__ int length_of(const PagedAttnParams& p, int b) {
 template <int KT>
 __device__ __forceinline__ int tiles_of(int len) {
   return max(1, (len + KT - 1) / KT);
+}
+
+// The length of the sequence behind `b`, for advance().
+__device__ __forceinline__ void look_ahead(const PagedAttnParams& p, Cursor& c) {
+  c.next_len = c.b + 1 < p.B ? length_of(p, c.b + 1) : 0;
 }
 
 // All tiles of all items lie on a line that the CTAs share evenly.  What CTA `c` takes of it, worked out by every warp for
@@ -209,6 +216,8 @@ __device__ __forceinline__ Range warp_range(const PagedAttnParams& p, int ctas, 
   r.total = __shfl_sync(0xffffffffu, inc, 31);
   r.nc = (int)(r.total < ctas ? r.total : ctas);
   r.nt = 0;
+  r.start = r.item_start = 0;
+  cur = Cursor{};
   if (c >= r.nc) return r;
   r.start = range_start(r.total, r.nc, c);
   r.nt = (int)(range_start(r.total, r.nc, c + 1) - r.start);
@@ -229,8 +238,11 @@ __device__ __forceinline__ Range warp_range(const PagedAttnParams& p, int ctas, 
   at = __shfl_sync(0xffffffffu, at, from);
   cur.ntile = tiles_of<KT>(cur.len);
   const uint32_t in = (uint32_t)(r.start - at);  // below 2^24 tiles times 2^24 items in all, far below here
-  cur.hr = (int)(in / (uint32_t)cur.ntile);
-  cur.tile = (int)(in - (uint32_t)cur.hr * (uint32_t)cur.ntile);
+  const uint32_t item = in / (uint32_t)cur.ntile;
+  cur.tile = (int)(in - item * (uint32_t)cur.ntile);
+  cur.h = (int)(item / (uint32_t)p.RT);
+  cur.rt = (int)(item - (uint32_t)cur.h * (uint32_t)p.RT);
+  look_ahead(p, cur);
   r.item_start = r.start - cur.tile;
   return r;
 }
@@ -238,12 +250,14 @@ template <int KT>
 __device__ __forceinline__ void advance(const PagedAttnParams& p, Cursor& c) {
   if (++c.tile < c.ntile) return;
   c.tile = 0;
-  if (++c.hr < p.Hkv * p.RT) return;
-  c.hr = 0;
-  if (++c.b < p.B) {
-    c.len = length_of(p, c.b);
-    c.ntile = tiles_of<KT>(c.len);
-  }
+  if (++c.rt < p.RT) return;
+  c.rt = 0;
+  if (++c.h < p.Hkv) return;
+  c.h = 0;
+  ++c.b;
+  c.len = c.next_len;
+  c.ntile = tiles_of<KT>(c.len);
+  look_ahead(p, c);
 }
 
 // One warp's running state over an item.  Rows lie along the matrix instruction's 8 columns: a thread has the two rows
@@ -267,42 +281,53 @@ template <class X, int D, bool Q8>
 __device__ __forceinline__ void loader(const CUtensorMap& mk, const CUtensorMap& mv, const PagedAttnParams& p, Cursor cur, int nt,
                                        uint8_t* ring, uint64_t* full, uint64_t* empty, const WaitCtx& w) {
   const int lane = threadIdx.x & 31;
-  const uint32_t box_bytes = (uint32_t)p.box * (2 * X::RB + (Q8 ? 2 : 0));
+  const int box = 1 << p.box_log2;
+  const uint32_t box_bytes = (uint32_t)box * (2 * X::RB + (Q8 ? 2 : 0));
   int stage = 0, issued = 0;
   uint32_t phase = 0;
+  // this lane's box of a tile: how many boxes the tile has, the box's row in its page, the page (fetched a tile ahead)
+  int boxes, row, page;
+  auto look_up = [&](const Cursor& c) {
+    const int key0 = c.tile * X::KT;
+    boxes = min(X::KT >> p.box_log2, (c.len - key0 + box - 1) >> p.box_log2);  // 0 for an empty sequence
+    const uint32_t grp = (uint32_t)(key0 + (lane << p.box_log2)) >> 4, pg = page_of_group(p.c, grp);
+    row = (int)(grp - pg * p.c.groups) * 16;
+    page = lane < boxes ? p.c.table[c.b * p.c.t_sb + pg] : 0;
+  };
+  if (nt > 0) look_up(cur);  // a CTA behind the line's end has no tile, and its cursor no sequence
   for (; issued < nt; ++issued) {
+    Cursor next = cur;
+    advance<X::KT>(p, next);
+    const int now = boxes, now_row = row;
+    int now_page = page;
+    if (issued + 1 < nt) look_up(next);
     if (issued >= X::STAGES && !mbar_wait(&empty[stage], phase ^ 1, w, DEV_TIMEOUT_PRODUCER)) break;
-    const int key0 = cur.tile * X::KT;
-    const int boxes = min(X::KT / p.box, (cur.len - key0 + p.box - 1) / p.box);  // 0 for an empty sequence
-    const int r0 = cur.hr % p.RT * X::RC;
+    const int r0 = cur.rt * X::RC;
     const int queries = X::Q_STAGE && (issued == 0 || cur.tile == 0) ? min(X::RC, p.R - r0) : 0;
-    if (lane == 0) mbar_arrive_expect_tx(&full[stage], boxes * box_bytes + queries * D * 2);
+    if (lane == 0) mbar_arrive_expect_tx(&full[stage], now * box_bytes + queries * D * 2);
     __syncwarp();
+    if (lane < now) {
+      if ((uint32_t)now_page >= (uint32_t)p.c.num_pages) {
+        if (p.status) atomicCAS(p.status, 0, (int)DEV_BAD_INDEX);
+        now_page = 0;
+      }
+      uint8_t* dst = ring + stage * X::STAGE + (lane << p.box_log2) * X::RS;
+#pragma unroll
+      for (int s = 0; s < X::SUBS; ++s) {
+        tma_load_4d(dst + s * X::SUB, &mk, &full[stage], s * 64, now_row, cur.h, now_page);
+        tma_load_4d(dst + X::KT * X::RB + s * X::SUB, &mv, &full[stage], s * 64, now_row, cur.h, now_page);
+      }
+      if constexpr (Q8) {
+        bulk_load(smem_u32(ring + X::STAGES * X::STAGE + stage * X::SCALE_STAGE + (lane << p.box_log2) * 2),
+                  p.c.scales + now_page * p.c.s_sp + cur.h * p.c.s_sh + now_row * 2, box * 2, &full[stage]);
+      }
+    }
     if (lane < queries) {
-      const int t = (r0 + lane) / p.G, head = cur.hr / p.RT * p.G + r0 + lane - t * p.G;
+      const uint32_t r = r0 + lane, t = r / (uint32_t)p.G, head = cur.h * p.G + r - t * p.G;
       bulk_load(smem_u32(ring + X::Q_AT + stage * X::Q_STAGE + lane * X::QROW), p.q + cur.b * p.q_sb + head * p.q_sh + t * p.q_sl,
                 D * 2, &full[stage]);
     }
-    if (lane < boxes) {
-      const uint32_t grp = (uint32_t)(key0 + lane * p.box) >> 4, pg = page_of_group(p.c, grp);
-      const int row = (int)(grp - pg * p.c.groups) * 16, h = cur.hr / p.RT;
-      int page = p.c.table[cur.b * p.c.t_sb + pg];
-      if ((uint32_t)page >= (uint32_t)p.c.num_pages) {
-        if (p.status) atomicCAS(p.status, 0, (int)DEV_BAD_INDEX);
-        page = 0;
-      }
-      uint8_t* dst = ring + stage * X::STAGE + lane * p.box * X::RS;
-#pragma unroll
-      for (int s = 0; s < X::SUBS; ++s) {
-        tma_load_4d(dst + s * X::SUB, &mk, &full[stage], s * 64, row, h, page);
-        tma_load_4d(dst + X::KT * X::RB + s * X::SUB, &mv, &full[stage], s * 64, row, h, page);
-      }
-      if constexpr (Q8) {
-        bulk_load(smem_u32(ring + X::STAGES * X::STAGE + stage * X::SCALE_STAGE + lane * p.box * 2),
-                  p.c.scales + page * p.c.s_sp + h * p.c.s_sh + row * 2, p.box * 2, &full[stage]);
-      }
-    }
-    advance<X::KT>(p, cur);
+    cur = next;
     if (++stage == X::STAGES) stage = 0, phase ^= 1;
   }
   // Shared memory must not go while a copy is in flight, also after a wait that ran out.
@@ -484,10 +509,11 @@ __global__ void __launch_bounds__(kAllThreads, (Geo<D, Q8, NB, WR>::CTAS))
   if (p.split) {
     range = warp_range<X::KT>(p, (int)gridDim.x, blockIdx.x, cons);
   } else {
-    const int HR = p.Hkv * p.RT;
-    cons.b = blockIdx.x / HR;
-    cons.hr = blockIdx.x - cons.b * HR;
-    cons.tile = 0;
+    const uint32_t HR = p.Hkv * p.RT, in = blockIdx.x % HR;
+    cons.b = (int)(blockIdx.x / HR);
+    cons.h = (int)(in / (uint32_t)p.RT);
+    cons.rt = (int)(in % (uint32_t)p.RT);
+    cons.tile = cons.next_len = 0;
     cons.len = length_of(p, cons.b);
     cons.ntile = range.nt = tiles_of<X::KT>(cons.len);
     range.item_start = range.start = 0;
@@ -512,7 +538,7 @@ __global__ void __launch_bounds__(kAllThreads, (Geo<D, Q8, NB, WR>::CTAS))
   uint32_t phase = 0;
 
   for (int i = 0; i < nt; ++i) {
-    const int rt = cons.hr % p.RT, h = cons.hr / p.RT;
+    const int rt = cons.rt, h = cons.h;
     if (X::Q_STAGE) alive = alive && mbar_wait(&full[stage], phase, wait, DEV_TIMEOUT_SOFTMAX);
     if (fresh) {
       fresh = false;
@@ -526,13 +552,13 @@ __global__ void __launch_bounds__(kAllThreads, (Geo<D, Q8, NB, WR>::CTAS))
           st.mx[nb][e] = st.ref[nb][e] = st.tmx[nb][e] = st.tref[nb][e] = -INFINITY;
           st.l[nb][e] = 0.f;
           const int r = rt * X::RC + wr * X::RW + nb * 8 + quad * 2 + e;
-          limit[nb][e] = r >= p.R ? 0 : p.causal ? cons.len - p.T + r / p.G + 1 : cons.len;
+          limit[nb][e] = r >= p.R ? 0 : p.causal ? cons.len - p.T + (int)((uint32_t)r / (uint32_t)p.G) + 1 : cons.len;
           qs[nb][e] = p.scale_log2;
         }
         // the queries as the instruction's second operand: row lane / 4
         const int r = rt * X::RC + wr * X::RW + nb * 8 + g8;
         const bool live = r < p.R;
-        const int t = live ? r / p.G : 0, g = live ? r - t * p.G : 0;
+        const int t = live ? (int)((uint32_t)r / (uint32_t)p.G) : 0, g = live ? r - t * p.G : 0;
         const __nv_bfloat16* src =
             X::Q_STAGE ? reinterpret_cast<const __nv_bfloat16*>(smem + X::Q_AT + stage * X::Q_STAGE + (nb * 8 + g8) * X::QROW)
                        : p.q + cons.b * p.q_sb + (int64_t)(h * p.G + g) * p.q_sh + t * p.q_sl;
@@ -797,7 +823,7 @@ __global__ void __launch_bounds__(kAllThreads, (Geo<D, Q8, NB, WR>::CTAS))
           const float m = max_of_keys(st.mx[nb][e]), l = sum_of_keys(st.l[nb][e]);
           if (g8 == 0)
             *reinterpret_cast<float2*>(ml + (warp * X::RW + nb * 8 + quad * 2 + e) * 2) =
-                make_float2(m, m == -INFINITY ? 0.f : l * exp2f(st.ref[nb][e] - m));
+                make_float2(m, m == -INFINITY ? 0.f : l * fast_exp2(st.ref[nb][e] - m));
         }
       compute_sync();
       // [warp][row][D]; elements are XORed with 8 times bits 1 and 2 of the row, so that a warp's rows differ in their banks
@@ -812,7 +838,7 @@ __global__ void __launch_bounds__(kAllThreads, (Geo<D, Q8, NB, WR>::CTAS))
           for (int w = 0; w < WK; ++w) top = fmaxf(top, ml[((w * WR + wr) * X::RW + row) * 2]);
           // an infinite maximum (an infinite score) gives NaN here, as exp(inf - inf) does
           const float own = Q8 ? st.tref[nb][e] - kUp : st.ref[nb][e];
-          const float f = own == -INFINITY ? 0.f : exp2f(own - top);
+          const float f = own == -INFINITY ? 0.f : fast_exp2(own - top);
           float* dst = buf + (warp * X::RW + row) * D;
           if constexpr (!Q8 || X::WIDE) {
 #pragma unroll
@@ -842,14 +868,14 @@ __global__ void __launch_bounds__(kAllThreads, (Geo<D, Q8, NB, WR>::CTAS))
         for (int w = 0; w < WK; ++w) {
           const int at = (w * WR + w0) * X::RW + in;
           const float mw = ml[at * 2];
-          sum += mw == -INFINITY ? 0.f : ml[at * 2 + 1] * exp2f(mw - top);
+          sum += mw == -INFINITY ? 0.f : ml[at * 2 + 1] * fast_exp2(mw - top);
           const float4 x = *reinterpret_cast<const float4*>(buf + at * D + ex);
           const float4 y = *reinterpret_cast<const float4*>(buf + at * D + ex + 4);
           v[0] += x.x, v[1] += x.y, v[2] += x.z, v[3] += x.w;
           v[4] += y.x, v[5] += y.y, v[6] += y.z, v[7] += y.w;
         }
         if (whole) {
-          const int r = rt * X::RC + row, t = r / p.G, head = h * p.G + r - t * p.G;
+          const int r = rt * X::RC + row, t = (int)((uint32_t)r / (uint32_t)p.G), head = h * p.G + r - t * p.G;
           const float inv = top == -INFINITY ? 0.f : 1.f / sum;  // a row that sees no key gives 0
           uint4 out;
           out.x = pack_bf16x2(v[0] * inv, v[1] * inv);
@@ -874,7 +900,7 @@ __global__ void __launch_bounds__(kAllThreads, (Geo<D, Q8, NB, WR>::CTAS))
         int to = (int)((item_end - 1) * range.nc / range.total);
         while (range_start(range.total, range.nc, to + 1) < item_end) ++to;
         while (range_start(range.total, range.nc, to) >= item_end) --to;
-        head = make_int4(cons.b, cons.hr, to - (int)blockIdx.x + 1, slot);
+        head = make_int4(cons.b, cons.h * p.RT + rt, to - (int)blockIdx.x + 1, slot);
       }
       first_piece = false;
       fresh = true;
@@ -920,7 +946,7 @@ __global__ void __launch_bounds__(kThreads) paged_join_kernel(const __grid_const
     for (int i = part; i < n; i += ways) {
       const float* s = i == 0 ? first : later + (int64_t)i * kSlotsPerCta * slot_floats;
       const float2 x = *reinterpret_cast<const float2*>(s + rc * D + row * 2);
-      const float f = x.x == -INFINITY ? 0.f : exp2f(x.x - top);
+      const float f = x.x == -INFINITY ? 0.f : fast_exp2(x.x - top);
       sum = fmaf(x.y, f, sum);
       const float* src = s + row * D + lane * E;
       float v[E];
@@ -1030,7 +1056,7 @@ int launch_wr(PagedAttnParams& p, const lvar_paged_cache& c, const Plan& plan, c
   int box = KT;
   while (c.page_size % box != 0 || KT % box != 0) box -= 16;
   while (box % 32 == 0 && box / 2 >= p.max_len) box /= 2;
-  p.box = box;
+  p.box_log2 = 31 - __builtin_clz(box);  // a divisor of 64 or 128
   CUtensorMap mk, mv;
   if (int rc = encode_pages_map(&mk, c.k, Q8, c.num_pages, c.Hkv, c.page_size, D, c.k_sp, c.k_sh, c.k_sl, box)) return rc;
   if (int rc = encode_pages_map(&mv, c.v, Q8, c.num_pages, c.Hkv, c.page_size, D, c.v_sp, c.v_sh, c.v_sl, box)) return rc;
