@@ -125,6 +125,8 @@ __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
 }
+// Token of a (token, query head) row.
+__device__ __forceinline__ int token_of(int r, int T, int G) { return T == 1 ? 0 : (int)((uint32_t)r / (uint32_t)G); }
 __device__ __forceinline__ float pow2i(int e) { return __int_as_float((e + 127) << 23); }  // -126 <= e <= 127
 
 // CTAs per SM: two; three of smaller tiles' worth where a warp's state is small and a key's bytes are few.
@@ -155,6 +157,7 @@ struct Geo {
   static constexpr int OS = WIDE ? 128 : RS, OSUB = KT * OS;
   static constexpr int RW = 8 * NB;                       // rows per warp
   static constexpr int RC = RW * WR;                      // rows per CTA
+  static constexpr int COST = WR == 1 ? 1 : 4;            // of an item beside its tiles, in tiles
   static constexpr int ML = 4 * RW * 2;                   // maxima and sums of the four warps' rows, floats; twice
   static constexpr int SMEM = RING + 2 * ML * 4 + 2 * STAGES * 8 + 16 + 1024;  // and the start's alignment
   static_assert(4 * RW * D * 4 <= (WIDE ? WIDE_BYTES : STAGE), "the warps' accumulators are joined in a consumed tile");
@@ -188,24 +191,60 @@ __device__ __forceinline__ void look_ahead(const PagedAttnParams& p, Cursor& c) 
   c.next_len = c.b + 1 < p.B ? length_of(p, c.b + 1) : 0;
 }
 
-// All tiles of all items lie on a line that the CTAs share evenly.  What CTA `c` takes of it, worked out by every warp for
-// itself: prefix sums over the sequences, a few of them per lane.
+// All items lie on a line that the CTAs share evenly, each with COST units and one unit per tile behind them: what an item
+// costs beside its tiles counts too, or a CTA over many short sequences would be the last by far (64 sequences of 0 to 2521
+// keys x 16 heads, e4m3, head dimension 64: 66 us without, 50 with one unit, 53 with four; 16 sequences of 0 to 4121 keys x
+// 35 rows x 4 heads, bf16: 37, 34 and 30 us).  A CTA takes the tiles
+// whose units lie in its range; every warp works that out for itself, by prefix sums over the sequences, a few per lane.
 struct Range {
-  int64_t total, start;
-  int nc, nt;          // CTAs that have tiles, tiles of this one (0: none)
-  int64_t item_start;  // of the item at `start`
+  int64_t total;       // units
+  int64_t item_start;  // unit of the first tile of the item at the range's start
+  int nc, nt;          // CTAs that have units, tiles of this one
 };
 __device__ __forceinline__ int64_t range_start(int64_t total, int nc, int c) {
   return total < 1 << 20 ? (int64_t)((uint32_t)total * (uint32_t)c / (uint32_t)nc) : total * c / nc;  // c <= nc < 2^12
 }
+__device__ __forceinline__ uint32_t divide(int64_t x, uint32_t d) {
+  return (uint64_t)x >> 32 ? (uint32_t)((uint64_t)x / d) : (uint32_t)x / d;
+}
 
-template <int KT>
+// The first tile at or behind unit x, the unit of its item's first tile, and the number of tiles in front of x; by a warp
+// whose lanes hold the sequences b0 .. b1 - 1 that begin at unit `at`.
+template <int KT, int COST>
+__device__ __forceinline__ int64_t locate(const PagedAttnParams& p, int64_t x, int64_t at, int64_t end, int b0, Cursor& cur,
+                                          int64_t& item_start) {
+  const int HR = p.Hkv * p.RT;
+  int b = 0, len = 0;
+  const bool here = x >= at && x < end;
+  if (here) {
+    for (b = b0;; ++b) {
+      len = length_of(p, b);
+      const int64_t next = at + (int64_t)(tiles_of<KT>(len) + COST) * HR;
+      if (x < next) break;
+      at = next;
+    }
+  }
+  const int from = __ffs(__ballot_sync(0xffffffffu, here)) - 1;
+  cur.b = __shfl_sync(0xffffffffu, b, from);
+  cur.len = __shfl_sync(0xffffffffu, len, from);
+  at = __shfl_sync(0xffffffffu, at, from);
+  cur.ntile = tiles_of<KT>(cur.len);
+  const uint32_t item = divide(x - at, (uint32_t)(cur.ntile + COST));
+  const int64_t begin = at + (int64_t)item * (cur.ntile + COST) + COST;
+  cur.tile = max((int)(x - begin), 0);
+  cur.h = (int)(item / (uint32_t)p.RT);
+  cur.rt = (int)(item - (uint32_t)cur.h * (uint32_t)p.RT);
+  item_start = begin;
+  return at - (int64_t)COST * HR * cur.b + (int64_t)item * cur.ntile + cur.tile;
+}
+
+template <int KT, int COST>
 __device__ __forceinline__ Range warp_range(const PagedAttnParams& p, int ctas, int c, Cursor& cur) {
   const int lane = threadIdx.x & 31;
   const int per = (p.B + 31) / 32, b0 = min(lane * per, p.B), b1 = min(b0 + per, p.B);
   const int HR = p.Hkv * p.RT;
   int64_t mine = 0;
-  for (int b = b0; b < b1; ++b) mine += (int64_t)tiles_of<KT>(length_of(p, b)) * HR;
+  for (int b = b0; b < b1; ++b) mine += (int64_t)(tiles_of<KT>(length_of(p, b)) + COST) * HR;
   int64_t inc = mine;
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) {
@@ -216,34 +255,14 @@ __device__ __forceinline__ Range warp_range(const PagedAttnParams& p, int ctas, 
   r.total = __shfl_sync(0xffffffffu, inc, 31);
   r.nc = (int)(r.total < ctas ? r.total : ctas);
   r.nt = 0;
-  r.start = r.item_start = 0;
+  r.item_start = 0;
   cur = Cursor{};
   if (c >= r.nc) return r;
-  r.start = range_start(r.total, r.nc, c);
-  r.nt = (int)(range_start(r.total, r.nc, c + 1) - r.start);
-  int64_t at = inc - mine;
-  int b = 0, len = 0;
-  const bool here = r.start >= at && r.start < inc;
-  if (here) {
-    for (b = b0;; ++b) {
-      len = length_of(p, b);
-      const int64_t end = at + (int64_t)tiles_of<KT>(len) * HR;
-      if (r.start < end) break;
-      at = end;
-    }
-  }
-  const int from = __ffs(__ballot_sync(0xffffffffu, here)) - 1;
-  cur.b = __shfl_sync(0xffffffffu, b, from);
-  cur.len = __shfl_sync(0xffffffffu, len, from);
-  at = __shfl_sync(0xffffffffu, at, from);
-  cur.ntile = tiles_of<KT>(cur.len);
-  const uint32_t in = (uint32_t)(r.start - at);  // below 2^24 tiles times 2^24 items in all, far below here
-  const uint32_t item = in / (uint32_t)cur.ntile;
-  cur.tile = (int)(in - item * (uint32_t)cur.ntile);
-  cur.h = (int)(item / (uint32_t)p.RT);
-  cur.rt = (int)(item - (uint32_t)cur.h * (uint32_t)p.RT);
+  const int64_t start = range_start(r.total, r.nc, c), end = range_start(r.total, r.nc, c + 1);
+  int64_t behind = r.total - (int64_t)COST * HR * p.B, unused;
+  if (end < r.total) behind = locate<KT, COST>(p, end, inc - mine, inc, b0, cur, unused);
+  r.nt = (int)(behind - locate<KT, COST>(p, start, inc - mine, inc, b0, cur, r.item_start));
   look_ahead(p, cur);
-  r.item_start = r.start - cur.tile;
   return r;
 }
 template <int KT>
@@ -323,7 +342,7 @@ __device__ __forceinline__ void loader(const CUtensorMap& mk, const CUtensorMap&
       }
     }
     if (lane < queries) {
-      const uint32_t r = r0 + lane, t = r / (uint32_t)p.G, head = cur.h * p.G + r - t * p.G;
+      const int r = r0 + lane, t = token_of(r, p.T, p.G), head = cur.h * p.G + r - t * p.G;
       bulk_load(smem_u32(ring + X::Q_AT + stage * X::Q_STAGE + lane * X::QROW), p.q + cur.b * p.q_sb + head * p.q_sh + t * p.q_sl,
                 D * 2, &full[stage]);
     }
@@ -431,10 +450,11 @@ __device__ __forceinline__ bool any_odd(uint32_t vs, int s0, int rows) {
   return __any_sync(0xffffffffu, hit != 0);
 }
 
-// The elements of V that CLEAN left out, row by row: a row takes those that it sees.
+// O^T += V^T P^T of a step with elements of V that are not finite: without them, and then row by row those that a row sees.
 template <class X, int D, bool Q8, int NB, int NK>
-__device__ __noinline__ void weigh_odd(State<D, NB>& st, const float (&sc)[NK][NB][4], const int (&seen)[NB][2], uint32_t vs,
-                                       int s0) {
+__device__ __noinline__ void weigh_odd(State<D, NB>& st, const float (&sc)[NK][NB][4], const int (&seen)[NB][2], uint32_t operand,
+                                       uint32_t vs, int s0) {
+  weigh<X, D, Q8, NB, NK, true>(st, sc, operand, s0);
   const int quad = threadIdx.x & 3;
   for (int j = 0; j < NK * 16; ++j) {
     const int row = s0 + j, from = ((j & 7) << 2) | quad;  // the lane that has these rows' weights of key j
@@ -507,7 +527,7 @@ __global__ void __launch_bounds__(kAllThreads, (Geo<D, Q8, NB, WR>::CTAS))
   Cursor cons;
   Range range;
   if (p.split) {
-    range = warp_range<X::KT>(p, (int)gridDim.x, blockIdx.x, cons);
+    range = warp_range<X::KT, X::COST>(p, (int)gridDim.x, blockIdx.x, cons);
   } else {
     const uint32_t HR = p.Hkv * p.RT, in = blockIdx.x % HR;
     cons.b = (int)(blockIdx.x / HR);
@@ -516,7 +536,7 @@ __global__ void __launch_bounds__(kAllThreads, (Geo<D, Q8, NB, WR>::CTAS))
     cons.tile = cons.next_len = 0;
     cons.len = length_of(p, cons.b);
     cons.ntile = range.nt = tiles_of<X::KT>(cons.len);
-    range.item_start = range.start = 0;
+    range.item_start = 0;
   }
   const int nt = range.nt;
   if (warp == 4) {
@@ -531,9 +551,10 @@ __global__ void __launch_bounds__(kAllThreads, (Geo<D, Q8, NB, WR>::CTAS))
   float qs[NB][2];      // factor from the raw product to log2 units, per row
   int limit[NB][2];     // keys that the row sees
   int see_all = 0;      // keys that every row of the item sees
-  const bool whole_first = range.item_start == range.start;  // the CTA's first piece begins at its item's start
+  const bool whole_first = cons.tile == 0;  // the CTA's first piece begins at its item's start
   bool first_piece = true, fresh = true, alive = true;
   int4 head = make_int4(0, 0, 0, 0);
+  int64_t item_unit = range.item_start;  // of the item's first tile, on the line
   int stage = 0;
   uint32_t phase = 0;
 
@@ -552,13 +573,13 @@ __global__ void __launch_bounds__(kAllThreads, (Geo<D, Q8, NB, WR>::CTAS))
           st.mx[nb][e] = st.ref[nb][e] = st.tmx[nb][e] = st.tref[nb][e] = -INFINITY;
           st.l[nb][e] = 0.f;
           const int r = rt * X::RC + wr * X::RW + nb * 8 + quad * 2 + e;
-          limit[nb][e] = r >= p.R ? 0 : p.causal ? cons.len - p.T + (int)((uint32_t)r / (uint32_t)p.G) + 1 : cons.len;
+          limit[nb][e] = r >= p.R ? 0 : p.causal ? cons.len - p.T + token_of(r, p.T, p.G) + 1 : cons.len;
           qs[nb][e] = p.scale_log2;
         }
         // the queries as the instruction's second operand: row lane / 4
         const int r = rt * X::RC + wr * X::RW + nb * 8 + g8;
         const bool live = r < p.R;
-        const int t = live ? (int)((uint32_t)r / (uint32_t)p.G) : 0, g = live ? r - t * p.G : 0;
+        const int t = live ? token_of(r, p.T, p.G) : 0, g = live ? r - t * p.G : 0;
         const __nv_bfloat16* src =
             X::Q_STAGE ? reinterpret_cast<const __nv_bfloat16*>(smem + X::Q_AT + stage * X::Q_STAGE + (nb * 8 + g8) * X::QROW)
                        : p.q + cons.b * p.q_sb + (int64_t)(h * p.G + g) * p.q_sh + t * p.q_sl;
@@ -793,7 +814,6 @@ __global__ void __launch_bounds__(kAllThreads, (Geo<D, Q8, NB, WR>::CTAS))
       // In a step that some row does not see all of, elements of V that are not finite come in row by row: a weight of zero
       // would make NaN of them in rows that do not see them.
       if (edge && any_odd<X, Q8, NS>(raw_v, s0, rows)) {
-        weigh<X, D, Q8, NB, NK, true>(st, sc, vs, s0);
         State<D, NB> st2 = st;
         float w[NK][NB][4];
         int seen[NB][2];
@@ -806,7 +826,7 @@ __global__ void __launch_bounds__(kAllThreads, (Geo<D, Q8, NB, WR>::CTAS))
           seen[nb][0] = limit[nb][0] - key0;
           seen[nb][1] = limit[nb][1] - key0;
         }
-        weigh_odd<X, D, Q8, NB, NK>(st2, w, seen, raw_v, s0);
+        weigh_odd<X, D, Q8, NB, NK>(st2, w, seen, vs, raw_v, s0);
         st = st2;
       } else {
         weigh<X, D, Q8, NB, NK, false>(st, sc, vs, s0);
@@ -875,7 +895,7 @@ __global__ void __launch_bounds__(kAllThreads, (Geo<D, Q8, NB, WR>::CTAS))
           v[4] += y.x, v[5] += y.y, v[6] += y.z, v[7] += y.w;
         }
         if (whole) {
-          const int r = rt * X::RC + row, t = (int)((uint32_t)r / (uint32_t)p.G), head = h * p.G + r - t * p.G;
+          const int r = rt * X::RC + row, t = token_of(r, p.T, p.G), head = h * p.G + r - t * p.G;
           const float inv = top == -INFINITY ? 0.f : 1.f / sum;  // a row that sees no key gives 0
           uint4 out;
           out.x = pack_bf16x2(v[0] * inv, v[1] * inv);
@@ -896,10 +916,11 @@ __global__ void __launch_bounds__(kAllThreads, (Geo<D, Q8, NB, WR>::CTAS))
         }
       }
       if (!last && (!first_piece || whole_first)) {  // the head of an item that later CTAs go on with
-        const int64_t item_end = range.start + i + 1 + (cons.ntile - 1 - cons.tile);
-        int to = (int)((item_end - 1) * range.nc / range.total);
-        while (range_start(range.total, range.nc, to + 1) < item_end) ++to;
-        while (range_start(range.total, range.nc, to) >= item_end) --to;
+        // the CTA whose range holds the unit of its last tile
+        const int64_t end_tile = item_unit + cons.ntile - 1;
+        int to = (int)(end_tile * range.nc / range.total);
+        while (range_start(range.total, range.nc, to + 1) <= end_tile) ++to;
+        while (range_start(range.total, range.nc, to) > end_tile) --to;
         head = make_int4(cons.b, cons.h * p.RT + rt, to - (int)blockIdx.x + 1, slot);
       }
       first_piece = false;
@@ -910,16 +931,20 @@ __global__ void __launch_bounds__(kAllThreads, (Geo<D, Q8, NB, WR>::CTAS))
     __syncwarp();
     if (lane == 0) mbar_arrive(&empty[stage]);
     if (++stage == X::STAGES) stage = 0, phase ^= 1;
+    if (last) item_unit += cons.ntile + X::COST;
     advance<X::KT>(p, cons);
   }
   if (p.split && tid == 0) p.heads[blockIdx.x] = head;
 }
 
-// Joins the pieces of the item that begins in CTA x's range and goes on behind it, in a fixed order.
+// Joins the pieces of the item that begins in CTA x's range and goes on behind it, in a fixed order.  Eight pieces of a row
+// are under way at a time: the kernel is a chain of few memory latencies.
+constexpr int kJoinWarps = 8;
+
 template <int D>
-__global__ void __launch_bounds__(kThreads) paged_join_kernel(const __grid_constant__ PagedAttnParams p, int rc) {
-  constexpr int E = D / 32;
-  __shared__ float sums[4][D], row_sum[4];
+__global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(const __grid_constant__ PagedAttnParams p, int rc) {
+  constexpr int E = D / 32, BATCH = 8;
+  __shared__ float sums[kJoinWarps][D], row_max[kJoinWarps], row_sum[kJoinWarps];
   const int c = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   griddep_wait();
   const int4 it = p.heads[c];
@@ -930,53 +955,72 @@ __global__ void __launch_bounds__(kThreads) paged_join_kernel(const __grid_const
   // the first piece lies in the CTA's slot it.w, every later one in slot 0 of its CTA
   const float* first = p.part + ((int64_t)c * kSlotsPerCta + it.w) * slot_floats;
   const float* later = p.part + (int64_t)c * kSlotsPerCta * slot_floats;
-  // Few pieces: a warp takes a row by itself; many: the CTA's four warps share a row's pieces.
-  const bool shared = n > 16;
-  const int ways = shared ? 4 : 1, part = shared ? warp : 0;
-  for (int row = shared ? blockIdx.y : blockIdx.y * 4 + warp; row < rows; row += shared ? gridDim.y : gridDim.y * 4) {
-    float top = -INFINITY;
-    for (int i = lane; i < n; i += 32) {
-      const float* s = i == 0 ? first : later + (int64_t)i * kSlotsPerCta * slot_floats;
-      top = fmaxf(top, s[rc * D + row * 2]);
-    }
+  // Few pieces: a warp takes a row by itself; many: the CTA's warps share a row's pieces.
+  const bool shared = n > 2 * BATCH;
+  const int ways = shared ? kJoinWarps : 1, step = shared ? gridDim.y : gridDim.y * kJoinWarps;
+  for (int row = shared ? blockIdx.y : blockIdx.y * kJoinWarps + warp; row < rows; row += step) {
+    float top = -INFINITY, sum = 0.f, acc[E] = {};
+    for (int i0 = shared ? warp : 0; i0 < n; i0 += ways * BATCH) {
+      float2 x[BATCH];
+      float v[BATCH][E];
 #pragma unroll
-    for (int d = 16; d >= 1; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-    float acc[E] = {}, sum = 0.f;
-#pragma unroll 4
-    for (int i = part; i < n; i += ways) {
-      const float* s = i == 0 ? first : later + (int64_t)i * kSlotsPerCta * slot_floats;
-      const float2 x = *reinterpret_cast<const float2*>(s + rc * D + row * 2);
-      const float f = x.x == -INFINITY ? 0.f : fast_exp2(x.x - top);
-      sum = fmaf(x.y, f, sum);
-      const float* src = s + row * D + lane * E;
-      float v[E];
-      if constexpr (E == 4) {
-        const float4 y = *reinterpret_cast<const float4*>(src);
-        v[0] = y.x, v[1] = y.y, v[2] = y.z, v[3] = y.w;
-      } else {
-        const float2 y = *reinterpret_cast<const float2*>(src);
-        v[0] = y.x, v[1] = y.y;
+      for (int u = 0; u < BATCH; ++u) {
+        const int i = i0 + u * ways;
+        x[u] = make_float2(-INFINITY, 0.f);
+#pragma unroll
+        for (int e = 0; e < E; ++e) v[u][e] = 0.f;
+        if (i < n) {
+          const float* s = i == 0 ? first : later + (int64_t)i * kSlotsPerCta * slot_floats;
+          x[u] = *reinterpret_cast<const float2*>(s + rc * D + row * 2);
+          if constexpr (E == 4) {
+            const float4 y = *reinterpret_cast<const float4*>(s + row * D + lane * E);
+            v[u][0] = y.x, v[u][1] = y.y, v[u][2] = y.z, v[u][3] = y.w;
+          } else {
+            const float2 y = *reinterpret_cast<const float2*>(s + row * D + lane * E);
+            v[u][0] = y.x, v[u][1] = y.y;
+          }
+        }
       }
+      float next = top;
 #pragma unroll
-      for (int e = 0; e < E; ++e) acc[e] = fmaf(f, v[e], acc[e]);
+      for (int u = 0; u < BATCH; ++u) next = fmaxf(next, x[u].x);
+      const float keep = top == -INFINITY ? 0.f : fast_exp2(top - next);
+      sum *= keep;
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[e] *= keep;
+#pragma unroll
+      for (int u = 0; u < BATCH; ++u) {
+        const float f = x[u].x == -INFINITY ? 0.f : fast_exp2(x[u].x - next);
+        sum = fmaf(x[u].y, f, sum);
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] = fmaf(f, v[u][e], acc[e]);
+      }
+      top = next;
     }
     if (shared) {
 #pragma unroll
       for (int e = 0; e < E; ++e) sums[warp][lane * E + e] = acc[e];
-      if (lane == 0) row_sum[warp] = sum;
+      if (lane == 0) row_max[warp] = top, row_sum[warp] = sum;
       __syncthreads();
       if (warp == 0) {
-        sum = (row_sum[0] + row_sum[1]) + (row_sum[2] + row_sum[3]);
+        top = -INFINITY;
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-          const int at = lane * E + e;
-          acc[e] = (sums[0][at] + sums[1][at]) + (sums[2][at] + sums[3][at]);
+        for (int w = 0; w < kJoinWarps; ++w) top = fmaxf(top, row_max[w]);
+        sum = 0.f;
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] = 0.f;
+#pragma unroll
+        for (int w = 0; w < kJoinWarps; ++w) {
+          const float f = row_max[w] == -INFINITY ? 0.f : fast_exp2(row_max[w] - top);
+          sum = fmaf(row_sum[w], f, sum);
+#pragma unroll
+          for (int e = 0; e < E; ++e) acc[e] = fmaf(sums[w][lane * E + e], f, acc[e]);
         }
       }
       __syncthreads();
       if (warp != 0) continue;
     }
-    const int r = rt * rc + row, t = r / p.G, head = h * p.G + r - t * p.G;
+    const int r = rt * rc + row, t = token_of(r, p.T, p.G), head = h * p.G + r - t * p.G;
     const float inv = top == -INFINITY ? 0.f : 1.f / sum;  // a row that sees no key gives 0
     __nv_bfloat16* dst = p.o + it.x * p.o_sb + head * p.o_sh + t * p.o_sl + lane * E;
     if constexpr (E == 4) {
@@ -1042,7 +1086,7 @@ int launch(const PagedAttnParams& p, const CUtensorMap& mk, const CUtensorMap& m
   if (plan.split) {
     const int rows = p.R < X::RC ? p.R : X::RC;
     cfg.gridDim = dim3((unsigned)plan.ctas, (unsigned)(rows < 8 ? rows : 8));
-    cfg.blockDim = dim3(kThreads);
+    cfg.blockDim = dim3(kJoinWarps * 32);
     cfg.dynamicSmemBytes = 0;
     LVAR_CUDA_OK(cudaLaunchKernelEx(&cfg, paged_join_kernel<D>, p, X::RC));
   }
