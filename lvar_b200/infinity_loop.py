@@ -7,7 +7,7 @@ an unconditional copy of every prompt (classifier-free guidance on the logits), 
 bit-label sampling and the multi-scale code accumulation that produces the next scale's input.
 
 Every SELF-attention call goes through this package: the fused QKV prologue (L2-normalise, per-head scale,
-2-D RoPE, append to the bf16 KV cache) and :class:`lvar_b200.policy.SelfAttentionDispatch` (dense attention
+2-D RoPE, append to the KV cache, contiguous or in pages) and :class:`lvar_b200.policy.SelfAttentionDispatch` (dense attention
 below the decision scale, CS4A in the first layers and CSLA in the remaining ones from it on).  Everything
 off that path is plain PyTorch: linear layers (cuBLAS), layer norms, GELU, the 64-token cross-attention
 (``scaled_dot_product_attention``), sampling and interpolation.  Weights are random (there is no checkpoint to
@@ -24,6 +24,7 @@ import torch.nn.functional as F
 
 from . import kernels as K
 from . import policy as P
+from .paged import PagedKVCache, PageTable
 from .sparse_attn_config import GLOBAL_CONFIG
 
 
@@ -42,6 +43,13 @@ class LoopConfig:
     # "sparse": the per-(scale, layer) dispatch; "dense": dense self-attention everywhere (the baseline model);
     # "none": the prologue still runs but no attention does (o = q) - for measuring self-attention's share
     attn_mode: str = "sparse"
+    # the KV cache: "contiguous" (bf16 [2B, heads, total tokens, head_dim] per layer), or in pages, "paged" (bf16) and
+    # "paged_e4m3" (half the bytes).  With pages the first scales' dense attention runs over the pages themselves; from
+    # `few_tokens` tokens on a layer's cache is read back into one pair of contiguous buffers that all layers share, for
+    # the many-query kernels.
+    cache: str = "contiguous"
+    page_size: int = 64
+    few_tokens: int = 64
 
     @property
     def head_dim(self) -> int:
@@ -95,8 +103,8 @@ class _Block:
 
 class InfinityLoop:
     """``generate(text)``: text bf16 [B, text_len, text_dim] -> accumulated codes fp32 [B, code_dim, S, S]
-    (S = the last scale's side).  One instance holds the weights, the KV caches of every layer (bf16
-    [2B, heads, total tokens, head_dim]) and the per-layer attention state for a fixed batch size."""
+    (S = the last scale's side).  One instance holds the weights, the KV caches of every layer (see
+    ``LoopConfig.cache``) and the per-layer attention state for a fixed batch size."""
 
     def __init__(self, cfg: LoopConfig, batch: int, device="cuda", seed: int = 0):
         self.cfg, self.B, self.device = cfg, batch, torch.device(device)
@@ -118,9 +126,23 @@ class InfinityLoop:
         self.w_head = torch.randn(2 * cfg.code_dim, C, generator=gen, device=self.device) * (C ** -0.5)
         self.rope_cos, self.rope_sin = rope2d_tables(cfg.scales, c, device=self.device)
         bs = 2 * batch
-        self.k_cache = [torch.zeros(bs, Hn, self.cum[-1], c, device=self.device, dtype=torch.bfloat16)
-                        for _ in range(cfg.depth)]
-        self.v_cache = [torch.zeros_like(t) for t in self.k_cache]
+        if cfg.cache not in ("contiguous", "paged", "paged_e4m3"):
+            raise ValueError(f"cache must be 'contiguous', 'paged' or 'paged_e4m3', got {cfg.cache!r}")
+
+        def buffer():
+            return torch.zeros(bs, Hn, self.cum[-1], c, device=self.device, dtype=torch.bfloat16)
+        self.pages: Optional[PageTable] = None
+        if cfg.cache == "contiguous":
+            self.k_cache = [buffer() for _ in range(cfg.depth)]
+            self.v_cache = [torch.zeros_like(t) for t in self.k_cache]
+        else:
+            self.pages = PageTable(bs, self.cum[-1], cfg.page_size, device=self.device)
+            self.pages.reserve_all({s: self.cum[-1] for s in range(bs)})
+            kind = torch.bfloat16 if cfg.cache == "paged" else torch.float8_e4m3fn
+            self.paged = [PagedKVCache(self.pages.num_pages, Hn, c, cfg.page_size, kind, self.device) for _ in range(cfg.depth)]
+            # cum[si] tokens are cached before scale si, for every sequence
+            self.lens = [torch.full((bs,), n, dtype=torch.int32, device=self.device) for n in self.cum]
+            self.k_read, self.v_read = buffer(), buffer()
         attn_cfg = GLOBAL_CONFIG["attn"]
         self.dispatch = [P.SelfAttentionDispatch(i, attn_cfg, cfg.scales, scale=1.0) for i in range(cfg.depth)]
         if cfg.attn_mode not in ("sparse", "dense", "none"):
@@ -137,20 +159,40 @@ class InfinityLoop:
         bs, L, C = xn.shape
         qkv = F.linear(xn, blk.w_qkv, blk.b_qkv).view(bs, L, 3, cfg.heads, cfg.head_dim)
         pos = self.cum[si]
+        d = self.dispatch[li]
+        if self.pages is not None:
+            o = self._paged_attention(blk, li, qkv, si)
+            self.routes[d.last_route] = self.routes.get(d.last_route, 0) + 1
+            return F.linear(o.transpose(1, 2).reshape(bs, L, C), blk.w_proj, blk.b_proj)
         q = K.qkv_prologue(qkv, blk.scale_mul, self.rope_cos, self.rope_sin, pos, self.k_cache[li], self.v_cache[li], pos)
         k = self.k_cache[li][:, :, :self.cum[si + 1]]
         v = self.v_cache[li][:, :, :self.cum[si + 1]]
-        d = self.dispatch[li]
-        if cfg.attn_mode == "sparse":
-            o = d(q, k, v, scale_ind=si, layer_ind=li, spattn_fn=self.csla[si])
-        elif cfg.attn_mode == "dense":
-            o = K.dense_attn_fwd(q, k, v, 1.0, return_stats=False)[0]
-            d.last_route = "dense"
-        else:
-            o = q
-            d.last_route = "none"
+        o = self._attention(d, q, k, v, li, si)
         self.routes[d.last_route] = self.routes.get(d.last_route, 0) + 1
         return F.linear(o.transpose(1, 2).reshape(bs, L, C), blk.w_proj, blk.b_proj)
+
+    def _attention(self, d: P.SelfAttentionDispatch, q, k, v, li: int, si: int) -> torch.Tensor:
+        if self.cfg.attn_mode == "sparse":
+            return d(q, k, v, scale_ind=si, layer_ind=li, spattn_fn=self.csla[si])
+        if self.cfg.attn_mode == "dense":
+            d.last_route = "dense"
+            return K.dense_attn_fwd(q, k, v, 1.0, return_stats=False)[0]
+        d.last_route = "none"
+        return q
+
+    def _paged_attention(self, blk: _Block, li: int, qkv: torch.Tensor, si: int) -> torch.Tensor:
+        cfg, cache, table, d = self.cfg, self.paged[li], self.pages.table, self.dispatch[li]
+        n, tokens = self.cum[si + 1], qkv.shape[1]
+        q = cache.prologue(qkv[:, :, 0], qkv[:, :, 1], qkv[:, :, 2], table, self.lens[si], scale_mul=blk.scale_mul,
+                           rope_cos=self.rope_cos, rope_sin=self.rope_sin)
+        dense = cfg.attn_mode == "dense" or (cfg.attn_mode == "sparse" and d.route(si, li, self.csla[si]) == "dense")
+        if dense and tokens <= cfg.few_tokens:
+            d.last_route = "dense"
+            return cache.attend(q, table, self.lens[si + 1], 1.0, max_len=n)
+        k, v = self.k_read[:, :, :n], self.v_read[:, :, :n]
+        if cfg.attn_mode != "none":
+            cache.read(table, self.lens[si + 1], n, out=(k, v))
+        return self._attention(d, q, k, v, li, si)
 
     def _cross_attention(self, blk: _Block, x: torch.Tensor, text_kv) -> torch.Tensor:
         cfg = self.cfg

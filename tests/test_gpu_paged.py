@@ -575,3 +575,107 @@ def test_refusals(K):
     assert K.paged_attn_fwd(q[:, :, :0], kb, vb, table, n).shape == (2, 4, 0, 64)
     assert K.paged_kv_read(kb, vb, table, n, 0)[0].shape == (2, 2, 0, 64)
     K.paged_kv_append(x[:, :, :0], x[:, :, :0], kb, vb, table, n)
+
+
+def test_cache_object_and_table(K):
+    """Sequences that come, grow and go over fewer pages than all of them at full length would take."""
+    from lvar_b200.paged import PagedKVCache, PageTable
+    table = PageTable(3, 200, page_size=16, num_pages=20)
+    for dtype in (torch.bfloat16, torch.float8_e4m3fn):
+        cache = PagedKVCache(20, 2, 64, 16, dtype)
+        g = torch.Generator(device="cuda").manual_seed(91)
+        held = [torch.zeros(2, 0, 64, device="cuda") for _ in range(3)]
+        for grow in ([30, 100, 0], [40, 0, 90], [0, -1, 0], [33, 60, 17]):
+            for s, n in enumerate(grow):
+                if n < 0:
+                    table.release(s)
+                    held[s] = held[s][:, :0]
+            start = torch.tensor([h.shape[1] for h in held], dtype=torch.int32, device="cuda")
+            count = torch.tensor([max(n, 0) for n in grow], dtype=torch.int32, device="cuda")
+            table.reserve_all({s: held[s].shape[1] + max(n, 0) for s, n in enumerate(grow)})
+            if max(grow) > 0:
+                x = torch.randn(3, 2, max(grow), 64, generator=g, device="cuda").bfloat16()
+                st = K.new_status("cuda")
+                cache.append(x, x, table.table, start, count=count, status=st)
+                assert K.read_status(st)[0] == 0
+                for s, n in enumerate(grow):
+                    held[s] = torch.cat([held[s], x[s, :, :max(n, 0)].float()], 1)
+        lens = torch.tensor([h.shape[1] for h in held], dtype=torch.int32, device="cuda")
+        k, v = cache.read(table.table, lens, int(lens.max()))
+        for s in range(3):
+            want = held[s].double()
+            if dtype != torch.bfloat16:
+                y, e = op.quantise(want)
+                want = y * torch.exp2(e.double())
+            assert torch.equal(k[s, :, :int(lens[s])].double(), want) and torch.equal(k[s], v[s])
+        q = torch.randn(3, 4, 1, 64, generator=g, device="cuda").bfloat16()
+        assert torch.equal(cache.attend(q, table.table, lens, 0.2), K.paged_attn_fwd(q, cache.k, cache.v, table.table, lens, 0.2,
+                                                                                    scales=cache.scales))
+        for s in range(3):
+            table.release(s)
+
+
+def test_a_wait_that_runs_out_ends_in_a_status(K):
+    """A wait limit of zero: the call gives up at its first unfinished wait and returns, and the next one is whole."""
+    for bits in (16, 8):
+        for T, G in ((1, 1), (5, 7)):
+            for n in (100, 9000):
+                k, v, sc, table = make_cache(2, 2, 128, 64, n, bits, 95)
+                q = torch.randn(2, 2 * G, T, 128, device="cuda").bfloat16()
+                lens = torch.tensor([n, n // 3], dtype=torch.int32, device="cuda")
+                st = K.new_status("cuda")
+                K.paged_attn_fwd(q, k, v, table, lens, scales=sc, status=st, wait_limit_ns=0)
+                assert K.read_status(st)[0] in (0, 6)  # 0: nothing had to wait
+                check_attn(K, q, k, v, table, lens, 128 ** -0.5, sc)
+
+
+def loop_of(cache, mode, seed=1):
+    from lvar_b200 import infinity_loop as IL
+    lc = IL.LoopConfig(depth=4, width=256, heads=2, ffn=512, text_dim=64, text_len=8, code_dim=8, scales=(1, 2, 4, 8, 16, 24),
+                       attn_mode=mode, cache=cache)
+    return IL.InfinityLoop(lc, batch=2, seed=seed)
+
+
+@pytest.mark.parametrize("mode", ["sparse", "dense"])
+def test_generation_loop_over_pages(K, mode):
+    """The generation loop with its cache in pages: the routes are the contiguous one's, a captured graph replays the eager
+    result bit for bit, and after the same layer inputs a layer's cache is the contiguous one's up to roundings (with e4m3
+    pages: up to those of the rows)."""
+    from lvar_b200 import sparse_attn_config as cfg
+    saved = dict(cfg.GLOBAL_CONFIG["attn"])
+    try:
+        cfg.GLOBAL_CONFIG["attn"].update(decision_scale=3, bound_layer=1, top_keys=0.3, cs4a_ws=[1, 1, 1, 1, 3, 5],
+                                         attn_sink=2, win_size=[-1, -1, 1, 1, 3, 5])
+        text = torch.randn(2, 8, 64, generator=torch.Generator().manual_seed(3)).bfloat16().cuda()
+        base = loop_of("contiguous", mode)
+        base.generate(text, seed=4)
+        routes = dict(base.routes)
+        for cache in ("paged", "paged_e4m3"):
+            loop = loop_of(cache, mode)
+            out = loop.generate(text, seed=4).clone()
+            assert loop.routes == routes and torch.isfinite(out).all()
+            assert torch.equal(loop.generate(text, seed=4), out)
+            loop.capture(text, seed=4)
+            assert torch.equal(loop.replay(), out)
+            # one layer's step on the same projection: contiguous and paged caches with the same history
+            for si in range(len(base.cum) - 1):
+                gen = torch.Generator(device="cuda").manual_seed(si)
+                xn = torch.randn(4, base.cum[si + 1] - base.cum[si], 256, generator=gen, device="cuda").bfloat16()
+                for x in (base, loop):
+                    assert torch.isfinite(x._self_attention(x.blocks[3], 3, xn, si)).all()
+                k, v = loop.paged[3].read(loop.pages.table, loop.lens[si + 1], base.cum[si + 1])
+                kc, vc = base.k_cache[3][:, :, :base.cum[si + 1]], base.v_cache[3][:, :, :base.cum[si + 1]]
+                assert torch.equal(loop.lens[si], torch.full_like(loop.lens[si], base.cum[si]))
+                if cache == "paged":
+                    assert torch.equal(v, vc)
+                    # two roundings of values at most 70 u32 of the rotated magnitudes (below 1) apart
+                    assert ((k.double() - kc.double()).abs() <= 2 * U16 * kc.double().abs() + 140 * U32).all()
+                else:
+                    for x, y in ((k, kc), (v, vc)):
+                        # e4m3 rounds by 2^-4 of an element or half the row's smallest step, 2^-10 * 2^e with
+                        # 2^e <= max / 224; the bf16 rounding of the other side comes on top
+                        most = y.double().abs().amax(-1, keepdim=True)
+                        assert ((x.double() - y.double()).abs() <= (2.0 ** -4 + 2 * U16) * y.double().abs() + most / 224 * 2.0 ** -9 + 140 * U32).all()
+    finally:
+        cfg.GLOBAL_CONFIG["attn"].clear()
+        cfg.GLOBAL_CONFIG["attn"].update(saved)
