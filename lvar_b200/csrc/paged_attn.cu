@@ -24,8 +24,11 @@
 // for elements 2^-24 below the row's largest).  K's row scale multiplies the score.  V's row scale 2^e joins the exponent
 // of the weight, w = exp2(s + e - running maximum of (s + e)), so that the fp16 weights are always taken relative to the
 // largest CONTRIBUTION; the row sum keeps a maximum of its own.
-// Weights are rounded once, to bf16 (bf16 cache) or fp16 (e4m3 cache; scaled by 2^7, so that only weights 2^-21 of the
-// largest or less are subnormal); sums, maxima and accumulators are fp32.
+// Weights against an e4m3 cache are rounded to fp16 (scaled by 2^7, so that only weights 2^-21 of the largest or less are
+// subnormal).  Against a bf16 cache up to 16 rows take them as the sum of two bf16 numbers, 2^-17 of them off: rounded once
+// they add as much again to the error of the output's own rounding, and next to HBM the second product costs nothing (24 x 16
+// heads x 10521 keys 311 us either way).  With more rows the matrix instructions count (64 rows, 16 x 8 heads x 8192 keys:
+// 131 us with one product, 159 with two), and weights are rounded to bf16.  Sums, maxima and accumulators are fp32.
 #include <math.h>
 
 #include "paged.cuh"
@@ -157,6 +160,7 @@ struct Geo {
   static constexpr int OS = WIDE ? 128 : RS, OSUB = KT * OS;
   static constexpr int RW = 8 * NB;                       // rows per warp
   static constexpr int RC = RW * WR;                      // rows per CTA
+  static constexpr bool TWO = !Q8 && WR == 1;             // weights as the sum of two bf16 numbers
   static constexpr int COST = WR == 1 ? 1 : 4;            // of an item beside its tiles, in tiles
   static constexpr int ML = 4 * RW * 2;                   // maxima and sums of the four warps' rows, floats; twice
   static constexpr int SMEM = RING + 2 * ML * 4 + 2 * STAGES * 8 + 16 + 1024;  // and the start's alignment
@@ -367,11 +371,18 @@ __device__ __forceinline__ void weigh(State<D, NB>& st, const float (&sc)[NK][NB
   const int lane = threadIdx.x & 31, quad = lane & 3;
 #pragma unroll
   for (int k = 0; k < NK; ++k) {
-    uint32_t b[NB][2];
+    uint32_t b[NB][2], rest[NB][2];
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
-      b[nb][0] = transpose8(Q8 ? pack_f16x2(sc[k][nb][0], sc[k][nb][1]) : pack_bf16x2(sc[k][nb][0], sc[k][nb][1]));
-      b[nb][1] = transpose8(Q8 ? pack_f16x2(sc[k][nb][2], sc[k][nb][3]) : pack_bf16x2(sc[k][nb][2], sc[k][nb][3]));
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+        const float w0 = sc[k][nb][2 * y], w1 = sc[k][nb][2 * y + 1];
+        const uint32_t two = Q8 ? pack_f16x2(w0, w1) : pack_bf16x2(w0, w1);
+        b[nb][y] = transpose8(two);
+        // what the rounding to bf16 left of the weights
+        if constexpr (X::TWO)
+          rest[nb][y] = transpose8(pack_bf16x2(w0 - __uint_as_float(two << 16), w1 - __uint_as_float(two & 0xffff0000u)));
+      }
     }
     if constexpr (!Q8 || X::WIDE) {
       const uint32_t v0 = vs + (s0 + k * 16 + (lane & 7) + ((lane >> 4) << 3)) * X::OS + ((((lane >> 3) & 1) ^ (lane & 7)) << 4);
@@ -390,7 +401,10 @@ __device__ __forceinline__ void weigh(State<D, NB>& st, const float (&sc)[NK][NB
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
           if constexpr (Q8) mma_f16(st.acc[t][nb], a, b[nb][0], b[nb][1]);
-          else mma_bf16(st.acc[t][nb], a, b[nb][0], b[nb][1]);
+          else {
+            mma_bf16(st.acc[t][nb], a, b[nb][0], b[nb][1]);
+            if constexpr (X::TWO) mma_bf16(st.acc[t][nb], a, rest[nb][0], rest[nb][1]);
+          }
         }
       }
     } else {
