@@ -121,10 +121,10 @@ __device__ __forceinline__ int exponent_for(float most) {
 // for packed arithmetic: with pairs (2i, 2i + 1) these are the halves of a 32-bit word, with `HALVES` four elements of either
 // half of the row.  The rotation table is read once for the warp's rows; indices are 32-bit but for the final addresses.
 // A row whose kind is decided row by row, with a library root, reciprocal and unpacked arithmetic, cost 210 instructions a
-// lane and bound the kernel by issue: 52 us for 2 x 4096 tokens x 48 heads x 128, 41 us now (0.75 of the
-// measured copy rate; two rows a lane 48 us, eight 41).
+// lane and bound the kernel by issue: 52 us for 2 x 4096 tokens x 48 heads x 128, 38 us now (0.81 of the
+// measured copy rate; two rows a lane instead of four 48 us).
 template <int C, bool HALVES, bool Q8, int U>
-__global__ void __launch_bounds__(256, 4) paged_write_kernel(const __grid_constant__ WriteParams p, int cq, int ck) {
+__global__ void __launch_bounds__(256, 3) paged_write_kernel(const __grid_constant__ WriteParams p, int cq, int ck) {
   constexpr int LPR = C / 8, RPW = 32 / LPR;
   const int lane = threadIdx.x & 31;
   const int t = (int)blockIdx.x * 8 + (int)(threadIdx.x >> 5);
@@ -159,6 +159,9 @@ __global__ void __launch_bounds__(256, 4) paged_write_kernel(const __grid_consta
     }
     src += step;
   }
+  float mul[U];  // the heads' factors
+#pragma unroll
+  for (int u = 0; u < U; ++u) mul[u] = kind == 0 && p.norm == 1 && h0 + u * RPW < heads ? __ldg(p.scale_mul + h0 + u * RPW) : 1.f;
   const int first = p.start[b];
   const int pos = first < 0 || first > kMaxTokens ? -1 : first + l;
   Place at{-1, 0};
@@ -196,119 +199,157 @@ __global__ void __launch_bounds__(256, 4) paged_write_kernel(const __grid_consta
     base = reinterpret_cast<uint8_t*>(p.q_out + b * p.q_sb + h0 * p.q_sh + l * p.q_sl);
     out_step = RPW * p.q_sh * 2;
   }
-#pragma unroll
-  for (int u = 0; u < U; ++u, base += out_step) {
-    const int h = h0 + u * RPW;
-    const bool live = h < heads;
-    uint32_t o[4] = {raw[u][0].x, raw[u][0].y, raw[u][1].x, raw[u][1].y};
-    if (kind == 2 && !Q8) {
-      // as they are
-    } else {
-      uint64_t A[2], B[2];
-      if constexpr (HALVES) {
-        A[0] = pack_f32x2(__uint_as_float(o[0] << 16), __uint_as_float(o[0] & 0xffff0000u));
-        A[1] = pack_f32x2(__uint_as_float(o[1] << 16), __uint_as_float(o[1] & 0xffff0000u));
-        B[0] = pack_f32x2(__uint_as_float(o[2] << 16), __uint_as_float(o[2] & 0xffff0000u));
-        B[1] = pack_f32x2(__uint_as_float(o[3] << 16), __uint_as_float(o[3] & 0xffff0000u));
-      } else {
-        A[0] = pack_f32x2(__uint_as_float(o[0] << 16), __uint_as_float(o[1] << 16));
-        B[0] = pack_f32x2(__uint_as_float(o[0] & 0xffff0000u), __uint_as_float(o[1] & 0xffff0000u));
-        A[1] = pack_f32x2(__uint_as_float(o[2] << 16), __uint_as_float(o[3] << 16));
-        B[1] = pack_f32x2(__uint_as_float(o[2] & 0xffff0000u), __uint_as_float(o[3] & 0xffff0000u));
-      }
-      if (kind < 2 && p.norm != 0) {
-        float s0, s1;
-        unpack_f32x2(ffma2(B[1], B[1], ffma2(B[0], B[0], ffma2(A[1], A[1], fmul2(A[0], A[0])))), s0, s1);
-        float ss = s0 + s1;
-#pragma unroll
-        for (int d = LPR / 2; d >= 1; d >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, d);
-        float f;
-        const float y = p.norm == 1 ? ss : fmaf(ss, 1.f / C, p.eps);
-        if (y > 1e-24f && y < 1e38f) {
-          // the hardware's reciprocal root and one Newton step: half an ulp more than the nearest at most
-          f = rsqrtf(y);
-          f = fmaf(0.5f * f, fmaf(-y * f, f, 1.f), f);
-        } else {
-          f = p.norm == 1 ? 1.f / fmaxf(sqrtf(y), 1e-12f) : 1.f / sqrtf(y);
-        }
-        if (kind == 0 && p.norm == 1 && live) f *= p.scale_mul[h];
-        const uint64_t ff = pack_f32x2(f, f);
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          A[i] = fmul2(A[i], ff);
-          B[i] = fmul2(B[i], ff);
-          if (wt != nullptr) {
-            A[i] = fmul2(A[i], wa[i]);
-            B[i] = fmul2(B[i], wb[i]);
-          }
-        }
-      }
-      if (kind < 2 && p.cos_t != nullptr) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const uint64_t a = ffma2(B[i], ns[i], fmul2(A[i], cs[i]));
-          B[i] = ffma2(B[i], cs[i], fmul2(A[i], sn[i]));
-          A[i] = a;
-        }
-      }
-      if (!Q8 || kind == 0) {
-        float a[4], c[4];
-        unpack_f32x2(A[0], a[0], a[1]), unpack_f32x2(A[1], a[2], a[3]);
-        unpack_f32x2(B[0], c[0], c[1]), unpack_f32x2(B[1], c[2], c[3]);
-        if constexpr (HALVES) {
-          o[0] = pack_bf16x2(a[0], a[1]), o[1] = pack_bf16x2(a[2], a[3]);
-          o[2] = pack_bf16x2(c[0], c[1]), o[3] = pack_bf16x2(c[2], c[3]);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) o[i] = pack_bf16x2(a[i], c[i]);
-        }
-      } else {
-        float a[4], c[4];
-        unpack_f32x2(A[0], a[0], a[1]), unpack_f32x2(A[1], a[2], a[3]);
-        unpack_f32x2(B[0], c[0], c[1]), unpack_f32x2(B[1], c[2], c[3]);
-        float most = fmax3(fabsf(a[0]), fabsf(a[1]), fabsf(a[2]));
-        most = fmax3(most, fabsf(a[3]), fabsf(c[0]));
-        most = fmax3(most, fabsf(c[1]), fabsf(c[2]));
-        most = fmaxf(most, fabsf(c[3]));  // passes over NaN, which stays NaN below
-#pragma unroll
-        for (int d = LPR / 2; d >= 1; d >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
-        if (__any_sync(0xffffffffu, most == INFINITY)) {
-          most = 0.f;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            a[i] = fabsf(a[i]) < INFINITY ? a[i] : NAN;
-            c[i] = fabsf(c[i]) < INFINITY ? c[i] : NAN;
-            most = fmax3(most, fabsf(a[i]), fabsf(c[i]));
-          }
-#pragma unroll
-          for (int d = LPR / 2; d >= 1; d >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
-        }
-        const int e = exponent_for(most);
-        const float down = __uint_as_float((uint32_t)(127 - e) << 23);
-        const uint64_t dd = pack_f32x2(down, down);
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          unpack_f32x2(fmul2(pack_f32x2(a[2 * i], a[2 * i + 1]), dd), a[2 * i], a[2 * i + 1]);
-          unpack_f32x2(fmul2(pack_f32x2(c[2 * i], c[2 * i + 1]), dd), c[2 * i], c[2 * i + 1]);
-        }
-        if (!live) continue;
-        if constexpr (HALVES) {
-          *reinterpret_cast<uint32_t*>(base + e0) = narrow4(a[0], a[1], a[2], a[3]);
-          *reinterpret_cast<uint32_t*>(base + e0 + kHigh) = narrow4(c[0], c[1], c[2], c[3]);
-        } else {
-          *reinterpret_cast<uint2*>(base + e0) = make_uint2(narrow4(a[0], c[0], a[1], c[1]), narrow4(a[2], c[2], a[3], c[3]));
-        }
-        if (x == 0) p.c.scales[at.page * p.c.s_sp + h * p.c.s_sh + at.row * 2 + (kind - 1)] = (uint8_t)(e + 127);
-        continue;
-      }
-    }
-    if (!live) continue;
+  auto store = [&](int u, const uint32_t (&o)[4]) {
+    if (h0 + u * RPW >= heads) return;
+    uint8_t* dst = base + u * out_step;
     if constexpr (HALVES) {
-      *reinterpret_cast<uint2*>(base + e0 * 2) = make_uint2(o[0], o[1]);
-      *reinterpret_cast<uint2*>(base + (e0 + kHigh) * 2) = make_uint2(o[2], o[3]);
+      *reinterpret_cast<uint2*>(dst + e0 * 2) = make_uint2(o[0], o[1]);
+      *reinterpret_cast<uint2*>(dst + (e0 + kHigh) * 2) = make_uint2(o[2], o[3]);
     } else {
-      *reinterpret_cast<uint4*>(base + e0 * 2) = make_uint4(o[0], o[1], o[2], o[3]);
+      *reinterpret_cast<uint4*>(dst + e0 * 2) = make_uint4(o[0], o[1], o[2], o[3]);
     }
+  };
+  if (kind == 2 && !Q8) {  // as they are
+#pragma unroll
+    for (int u = 0; u < U; ++u) store(u, {raw[u][0].x, raw[u][0].y, raw[u][1].x, raw[u][1].y});
+    return;
+  }
+
+  // Step by step for all rows, so that their chains of shuffles and roots overlap.
+  uint64_t A[U][2], B[U][2];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const uint32_t w[4] = {raw[u][0].x, raw[u][0].y, raw[u][1].x, raw[u][1].y};
+    auto lo = [&](int i) { return __uint_as_float(w[i] << 16); };
+    auto hi = [&](int i) { return __uint_as_float(w[i] & 0xffff0000u); };
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      A[u][i] = HALVES ? pack_f32x2(lo(i), hi(i)) : pack_f32x2(lo(2 * i), lo(2 * i + 1));
+      B[u][i] = HALVES ? pack_f32x2(lo(i + 2), hi(i + 2)) : pack_f32x2(hi(2 * i), hi(2 * i + 1));
+    }
+  }
+  if (kind < 2 && p.norm != 0) {
+    float y[U], f[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      float s0, s1;
+      unpack_f32x2(ffma2(B[u][1], B[u][1], ffma2(B[u][0], B[u][0], ffma2(A[u][1], A[u][1], fmul2(A[u][0], A[u][0])))), s0, s1);
+      y[u] = s0 + s1;
+    }
+#pragma unroll
+    for (int d = LPR / 2; d >= 1; d >>= 1)
+#pragma unroll
+      for (int u = 0; u < U; ++u) y[u] += __shfl_xor_sync(0xffffffffu, y[u], d);
+    bool plain = true;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (p.norm == 2) y[u] = fmaf(y[u], 1.f / C, p.eps);
+      // the hardware's reciprocal root and one Newton step: half an ulp more than the nearest at most
+      f[u] = rsqrtf(y[u]);
+      f[u] = fmaf(0.5f * f[u], fmaf(-y[u] * f[u], f[u], 1.f), f[u]);
+      plain = plain && y[u] > 1e-24f && y[u] < 1e38f;
+    }
+    if (!plain) {  // a norm that is clamped, zero or not finite
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (!(y[u] > 1e-24f && y[u] < 1e38f)) f[u] = p.norm == 1 ? 1.f / fmaxf(sqrtf(y[u]), 1e-12f) : 1.f / sqrtf(y[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const uint64_t ff = pack_f32x2(f[u] * mul[u], f[u] * mul[u]);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        A[u][i] = fmul2(A[u][i], ff);
+        B[u][i] = fmul2(B[u][i], ff);
+      }
+    }
+    if (wt != nullptr) {
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          A[u][i] = fmul2(A[u][i], wa[i]);
+          B[u][i] = fmul2(B[u][i], wb[i]);
+        }
+    }
+  }
+  if (kind < 2 && p.cos_t != nullptr) {
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const uint64_t a = ffma2(B[u][i], ns[i], fmul2(A[u][i], cs[i]));
+        B[u][i] = ffma2(B[u][i], cs[i], fmul2(A[u][i], sn[i]));
+        A[u][i] = a;
+      }
+  }
+  if (!Q8 || kind == 0) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      float a[4], c[4];
+      unpack_f32x2(A[u][0], a[0], a[1]), unpack_f32x2(A[u][1], a[2], a[3]);
+      unpack_f32x2(B[u][0], c[0], c[1]), unpack_f32x2(B[u][1], c[2], c[3]);
+      if constexpr (HALVES) {
+        store(u, {pack_bf16x2(a[0], a[1]), pack_bf16x2(a[2], a[3]), pack_bf16x2(c[0], c[1]), pack_bf16x2(c[2], c[3])});
+      } else {
+        store(u, {pack_bf16x2(a[0], c[0]), pack_bf16x2(a[1], c[1]), pack_bf16x2(a[2], c[2]), pack_bf16x2(a[3], c[3])});
+      }
+    }
+    return;
+  }
+  // an 8-bit row
+  float most[U];
+  auto largest = [&](int u) {  // passes over NaN
+    float a[4], c[4];
+    unpack_f32x2(A[u][0], a[0], a[1]), unpack_f32x2(A[u][1], a[2], a[3]);
+    unpack_f32x2(B[u][0], c[0], c[1]), unpack_f32x2(B[u][1], c[2], c[3]);
+    return fmaxf(fmax3(fmax3(fabsf(a[0]), fabsf(a[1]), fabsf(a[2])), fabsf(a[3]), fabsf(c[0])),
+                 fmax3(fabsf(c[1]), fabsf(c[2]), fabsf(c[3])));
+  };
+  bool endless = false;
+#pragma unroll
+  for (int u = 0; u < U; ++u) most[u] = largest(u);
+#pragma unroll
+  for (int d = LPR / 2; d >= 1; d >>= 1)
+#pragma unroll
+    for (int u = 0; u < U; ++u) most[u] = fmaxf(most[u], __shfl_xor_sync(0xffffffffu, most[u], d));
+#pragma unroll
+  for (int u = 0; u < U; ++u) endless = endless || most[u] == INFINITY;
+  if (__any_sync(0xffffffffu, endless)) {  // infinities become NaN and the maximum is taken again
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        float a, c;
+        unpack_f32x2(A[u][i], a, c);
+        A[u][i] = pack_f32x2(fabsf(a) < INFINITY ? a : NAN, fabsf(c) < INFINITY ? c : NAN);
+        unpack_f32x2(B[u][i], a, c);
+        B[u][i] = pack_f32x2(fabsf(a) < INFINITY ? a : NAN, fabsf(c) < INFINITY ? c : NAN);
+      }
+      most[u] = largest(u);
+      most[u] = most[u] < INFINITY ? most[u] : 0.f;  // all NaN
+#pragma unroll
+      for (int d = LPR / 2; d >= 1; d >>= 1) most[u] = fmaxf(most[u], __shfl_xor_sync(0xffffffffu, most[u], d));
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int e = exponent_for(most[u]);
+    const float down = __uint_as_float((uint32_t)(127 - e) << 23);
+    const uint64_t dd = pack_f32x2(down, down);
+    float a[4], c[4];
+    unpack_f32x2(fmul2(A[u][0], dd), a[0], a[1]), unpack_f32x2(fmul2(A[u][1], dd), a[2], a[3]);
+    unpack_f32x2(fmul2(B[u][0], dd), c[0], c[1]), unpack_f32x2(fmul2(B[u][1], dd), c[2], c[3]);
+    const int h = h0 + u * RPW;
+    if (h >= heads) continue;
+    uint8_t* dst = base + u * out_step;
+    if constexpr (HALVES) {
+      *reinterpret_cast<uint32_t*>(dst + e0) = narrow4(a[0], a[1], a[2], a[3]);
+      *reinterpret_cast<uint32_t*>(dst + e0 + kHigh) = narrow4(c[0], c[1], c[2], c[3]);
+    } else {
+      *reinterpret_cast<uint2*>(dst + e0) = make_uint2(narrow4(a[0], c[0], a[1], c[1]), narrow4(a[2], c[2], a[3], c[3]));
+    }
+    if (x == 0) p.c.scales[at.page * p.c.s_sp + h * p.c.s_sh + at.row * 2 + (kind - 1)] = (uint8_t)(e + 127);
   }
 }
 
