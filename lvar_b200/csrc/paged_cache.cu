@@ -123,8 +123,9 @@ __device__ __forceinline__ int exponent_for(float most) {
 // A row whose kind is decided row by row, with a library root, reciprocal and unpacked arithmetic, cost 210 instructions a
 // lane and bound the kernel by issue: 52 us for 2 x 4096 tokens x 48 heads x 128, 38 us now (0.81 of the
 // measured copy rate; two rows a lane instead of four 48 us).
-template <int C, bool HALVES, bool Q8, int U>
-__global__ void __launch_bounds__(256, 3) paged_write_kernel(const __grid_constant__ WriteParams p, int cq, int ck) {
+// PLAIN: rows go as they are, without norm, rotation or a change of type.
+template <int C, bool HALVES, bool Q8, bool PLAIN, int U>
+__global__ void __launch_bounds__(256, PLAIN ? 6 : 3) paged_write_kernel(const __grid_constant__ WriteParams p, int cq, int ck) {
   constexpr int LPR = C / 8, RPW = 32 / LPR;
   const int lane = threadIdx.x & 31;
   const int t = (int)blockIdx.x * 8 + (int)(threadIdx.x >> 5);
@@ -161,7 +162,7 @@ __global__ void __launch_bounds__(256, 3) paged_write_kernel(const __grid_consta
   }
   float mul[U];  // the heads' factors
 #pragma unroll
-  for (int u = 0; u < U; ++u) mul[u] = kind == 0 && p.norm == 1 && h0 + u * RPW < heads ? __ldg(p.scale_mul + h0 + u * RPW) : 1.f;
+  for (int u = 0; u < U; ++u) mul[u] = !PLAIN && kind == 0 && p.norm == 1 && h0 + u * RPW < heads ? __ldg(p.scale_mul + h0 + u * RPW) : 1.f;
   const int first = p.start[b];
   const int pos = first < 0 || first > kMaxTokens ? -1 : first + l;
   Place at{-1, 0};
@@ -170,7 +171,7 @@ __global__ void __launch_bounds__(256, 3) paged_write_kernel(const __grid_consta
     if (at.page < 0) return;  // padding, or nowhere to go: the same for the whole warp
   }
   uint64_t cs[2], sn[2], ns[2];  // cosines and sines of the lane's four rotations, and the sines negated
-  if (p.cos_t != nullptr && kind < 2) {
+  if (!PLAIN && p.cos_t != nullptr && kind < 2) {
     if (there && (uint32_t)pos >= (uint32_t)p.rope_rows && p.status) atomicCAS(p.status, 0, (int)DEV_BAD_INDEX);
     const int64_t row = min(max(pos, 0), p.rope_rows - 1);
     const float4 c4 = __ldg(reinterpret_cast<const float4*>(p.cos_t + row * (C / 2) + x * 4));
@@ -179,7 +180,7 @@ __global__ void __launch_bounds__(256, 3) paged_write_kernel(const __grid_consta
     sn[0] = pack_f32x2(s4.x, s4.y), sn[1] = pack_f32x2(s4.z, s4.w);
     ns[0] = pack_f32x2(-s4.x, -s4.y), ns[1] = pack_f32x2(-s4.z, -s4.w);
   }
-  const float* wt = p.norm == 2 && kind < 2 ? (kind == 0 ? p.wq : p.wk) : nullptr;
+  const float* wt = !PLAIN && p.norm == 2 && kind < 2 ? (kind == 0 ? p.wq : p.wk) : nullptr;
   uint64_t wa[2], wb[2];  // norm weights of the first and second elements
   if (wt != nullptr) {
     const float4 a = __ldg(reinterpret_cast<const float4*>(wt + e0)), c = __ldg(reinterpret_cast<const float4*>(wt + e0 + kHigh));
@@ -209,7 +210,7 @@ __global__ void __launch_bounds__(256, 3) paged_write_kernel(const __grid_consta
       *reinterpret_cast<uint4*>(dst + e0 * 2) = make_uint4(o[0], o[1], o[2], o[3]);
     }
   };
-  if (kind == 2 && !Q8) {  // as they are
+  if (PLAIN || (kind == 2 && !Q8)) {  // as they are
 #pragma unroll
     for (int u = 0; u < U; ++u) store(u, {raw[u][0].x, raw[u][0].y, raw[u][1].x, raw[u][1].y});
     return;
@@ -353,33 +354,34 @@ __global__ void __launch_bounds__(256, 3) paged_write_kernel(const __grid_consta
   }
 }
 
-template <int C, bool HALVES, bool Q8, int U>
+template <int C, bool HALVES, bool Q8, bool PLAIN, int U>
 int launch_write_u(const WriteParams& p, cudaStream_t stream) {
   constexpr int ROWS = 32 / (C / 8) * U;
   const int cq = (p.Hq + ROWS - 1) / ROWS, ck = (p.Hkv + ROWS - 1) / ROWS;
   LVAR_REQUIRE((int64_t)cq + 2 * ck <= 65535, LVAR_ERR_LIMIT, "too many heads");
   const dim3 grid((unsigned)(((int64_t)p.B * p.L + 7) / 8), (unsigned)(cq + 2 * ck));
-  paged_write_kernel<C, HALVES, Q8, U><<<grid, 256, 0, stream>>>(p, cq, ck);
+  paged_write_kernel<C, HALVES, Q8, PLAIN, U><<<grid, 256, 0, stream>>>(p, cq, ck);
   LVAR_CUDA_OK(cudaGetLastError());
   return LVAR_OK;
 }
 // Several rows per lane once one row each would fill the chip twice over, as many as leave at most a quarter of the lanes
 // without a row; one row otherwise: the shortest chain of dependent steps, which is all that a small call waits for.
-template <int C, bool HALVES, bool Q8>
+template <int C, bool HALVES, bool Q8, bool PLAIN>
 int launch_write_q(const WriteParams& p, cudaStream_t stream) {
   constexpr int RPW = 32 / (C / 8);
   const int64_t tokens = (int64_t)p.B * p.L, rows = (int64_t)p.Hq + 2ll * p.Hkv;
   auto padded = [&](int n) { return ((int64_t)(p.Hq + n - 1) / n + 2 * ((p.Hkv + n - 1) / n)) * n; };
   if (tokens * rows >= 2 * 148 * 40 * RPW) {
-    if (4 * rows >= 3 * padded(4 * RPW)) return launch_write_u<C, HALVES, Q8, 4>(p, stream);
-    if (4 * rows >= 3 * padded(2 * RPW)) return launch_write_u<C, HALVES, Q8, 2>(p, stream);
+    if (4 * rows >= 3 * padded(4 * RPW)) return launch_write_u<C, HALVES, Q8, PLAIN, 4>(p, stream);
+    if (4 * rows >= 3 * padded(2 * RPW)) return launch_write_u<C, HALVES, Q8, PLAIN, 2>(p, stream);
   }
-  return launch_write_u<C, HALVES, Q8, 1>(p, stream);
+  return launch_write_u<C, HALVES, Q8, PLAIN, 1>(p, stream);
 }
 template <int C>
 int launch_write_c(const WriteParams& p, bool halves, cudaStream_t stream) {
-  if (p.c.scales) return halves ? launch_write_q<C, true, true>(p, stream) : launch_write_q<C, false, true>(p, stream);
-  return halves ? launch_write_q<C, true, false>(p, stream) : launch_write_q<C, false, false>(p, stream);
+  if (p.c.scales) return halves ? launch_write_q<C, true, true, false>(p, stream) : launch_write_q<C, false, true, false>(p, stream);
+  if (p.norm == 0 && p.cos_t == nullptr) return launch_write_q<C, false, false, true>(p, stream);
+  return halves ? launch_write_q<C, true, false, false>(p, stream) : launch_write_q<C, false, false, false>(p, stream);
 }
 
 struct ReadParams {
