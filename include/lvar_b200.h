@@ -285,7 +285,7 @@ int lvar_qkv_prologue(const void* qkv, int64_t s_b, int64_t s_l, int64_t s_w, in
                       int32_t H, int32_t c, lvar_stream_t stream);
 
 /* A key/value cache in pages, for sequences of different length.  k, v: [num_pages, Hkv, page_size, D] with the given
- * strides in elements (innermost 1, 16-byte aligned rows), bf16, or e4m3 when `scales` is set: uint8
+ * strides in elements (innermost 1, 16-byte aligned rows; attention needs them positive), bf16, or e4m3 when `scales` is set: uint8
  * [num_pages, Hkv, page_size, 2] (innermost two contiguous; 16-byte aligned, page and head strides multiples of 16), for every row of K ([0])
  * and V ([1]) the biased exponent x of the power of two 2^(x - 127) that its e4m3 values are multiplied by.
  * table: int32 [B, max_pages] (rows t_sb apart): position j of sequence b lies in page table[b, j / page_size], row

@@ -210,6 +210,11 @@ __global__ void __launch_bounds__(256, PLAIN ? 6 : 3) paged_write_kernel(const _
       *reinterpret_cast<uint4*>(dst + e0 * 2) = make_uint4(o[0], o[1], o[2], o[3]);
     }
   };
+  if (!there) {  // padding: only a query row has a place
+#pragma unroll
+    for (int u = 0; u < U; ++u) store(u, {0u, 0u, 0u, 0u});
+    return;
+  }
   if (PLAIN || (kind == 2 && !Q8)) {  // as they are
 #pragma unroll
     for (int u = 0; u < U; ++u) store(u, {raw[u][0].x, raw[u][0].y, raw[u][1].x, raw[u][1].y});

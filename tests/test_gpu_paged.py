@@ -108,10 +108,10 @@ def test_attention_over_many_lengths(K, bits, D, Hq, H, T, page, causal):
 
 
 @pytest.mark.parametrize("bits", [16, 8])
-@pytest.mark.parametrize("max_len", [1, 64, 128, 129, 256, 257])
+@pytest.mark.parametrize("max_len", [0, 1, 64, 128, 129, 256, 257])
 def test_attention_short_bounds(K, bits, max_len):
     """Launches without a split (few tiles) and with one."""
-    lens = torch.tensor([max_len, 0, max(1, max_len // 2)], dtype=torch.int32, device="cuda")
+    lens = torch.tensor([max_len, 0, (max_len + 1) // 2], dtype=torch.int32, device="cuda")
     k, v, scales, table = make_cache(3, 4, 128, 16, max_len, bits, max_len)
     q = torch.randn(3, 8, 2, 128, generator=torch.Generator(device="cuda").manual_seed(4), device="cuda").bfloat16()
     check_attn(K, q, k, v, table, lens, 0.3, scales, True, max_len=max_len)
@@ -575,6 +575,43 @@ def test_refusals(K):
     assert K.paged_attn_fwd(q[:, :, :0], kb, vb, table, n).shape == (2, 4, 0, 64)
     assert K.paged_kv_read(kb, vb, table, n, 0)[0].shape == (2, 2, 0, 64)
     K.paged_kv_append(x[:, :, :0], x[:, :, :0], kb, vb, table, n)
+
+
+def test_padding_stays_zero_without_eps(K):
+    """A root-mean-square norm without eps is 0 / 0 for a row of zeros, but a row of padding is 0."""
+    x = torch.zeros(2, 3, 6, 64, dtype=torch.bfloat16, device="cuda")
+    kp, vp, _ = empty_cache(2, 2, 16, 64, 16)
+    table = torch.tensor([[0], [1]], dtype=torch.int32, device="cuda")
+    zero, count = torch.zeros(2, dtype=torch.int32, device="cuda"), torch.tensor([1, 0], dtype=torch.int32, device="cuda")
+    o = K.paged_qkv_prologue(x[:, :, :2], x[:, :, 2:4], x[:, :, 4:], kp, vp, table, zero, eps=0.0, count=count)
+    assert torch.isnan(o[0, :, 0]).all() and (o[0, :, 1:] == 0).all() and (o[1] == 0).all()
+    assert torch.isnan(kp[0, :, 0]).all() and (kp[0, :, 1:] == 7).all() and (kp[1] == 7).all()
+
+
+@pytest.mark.parametrize("bits", [16, 8])
+def test_many_sequences(K, bits):
+    """Thousands of sequences, most of them empty or of a few keys."""
+    r = random.Random(5)
+    B = 3001
+    n = [r.choice([0, 0, 1, r.randint(1, 30), 300]) for _ in range(B)]
+    k, v, scales, _ = make_cache(40, 1, 64, 16, 300, bits, 101)
+    if bits == 16:
+        k, v = torch.nan_to_num(k), torch.nan_to_num(v)
+    table = torch.randint(0, k.shape[0], (B, 19), generator=torch.Generator(device="cuda").manual_seed(6), device="cuda").to(torch.int32)
+    q = torch.randn(B, 2, 1, 64, generator=torch.Generator(device="cuda").manual_seed(7), device="cuda").bfloat16()
+    check_attn(K, q, k, v, table, torch.tensor(n, dtype=torch.int32, device="cuda"), 0.125, scales)
+
+
+@pytest.mark.parametrize("bits", [16, 8])
+def test_a_million_keys(K, bits):
+    """One sequence whose table names the same few pages over and over."""
+    n = 1200003
+    k, v, scales, _ = make_cache(30, 1, 64, 512, 512, bits, 103)
+    if bits == 16:
+        k, v = torch.nan_to_num(k), torch.nan_to_num(v)
+    table = (torch.arange(-(-n // 512), device="cuda") * 7 % k.shape[0]).to(torch.int32)[None]
+    q = 2 * torch.randn(1, 4, 2, 64, generator=torch.Generator(device="cuda").manual_seed(8), device="cuda")
+    check_attn(K, q.bfloat16(), k, v, table, torch.tensor([n], dtype=torch.int32, device="cuda"), 0.125, scales, True)
 
 
 def test_cache_object_and_table(K):
