@@ -3,26 +3,30 @@
 //
 // Bound by reading the cache (4 D bytes per cached row in bf16, 2 D + 2 in e4m3; 4 D flops per row and query row): the
 // G = Hq / Hkv query heads of a key head and the T tokens are the rows of one tile, so that a cached row crosses HBM
-// once for all of them.  A tile of 16 rows is what one warp-level matrix instruction takes (m16n8k16); the tensor-memory
-// instructions start at 64 rows, of which one to sixteen would be used, and their accumulators would have to come back
-// through tensor memory for the running softmax of every 64 keys.  16 rows per warp leave the matrix pipe several times
-// ahead of HBM (16 flops per byte against the 250 that the chip's ratio allows), so it is not what bounds the kernel.
+// once for all of them.  Products are warp-level matrix instructions (m16n8k16) with the keys, and in the second product the
+// elements of V, along their 16 rows and the query rows along their 8 columns: S^T = K Q^T, O^T = V^T P^T, P^T made from S^T
+// by an 8 x 8 transposition in registers.  One query row so pays for 8; the tensor-memory instructions start at 64, and
+// their accumulators would have to come back through tensor memory for every step of the running softmax.  With up to 8 rows
+// the tensor pipe is 15 to 17 % busy and HBM bounds the kernel (24 x 16 heads x 10521 keys in bf16: 303 to 315 us, 6.6 to
+// 6.8 TB/s); with 64 rows tensor pipe (58 %) and shared memory (64 %) do (16 x 8 heads x 8192 keys: 125 us, 0.66 of HBM).
 //
 // A CTA is four warps that compute and one that loads.  The loader follows the page table (one lane per box of 16 to 128
 // rows that lie together in a page) and streams tiles of keys through a ring in shared memory with tensor-map copies,
 // swizzled; the others wait for a tile and hand its place back, and meet only at an item's end.  Rows of a box behind the
-// sequence's end are copied too: their scores are masked and their V rows made zeros.  With up to 16 rows the four warps take a quarter of a tile's keys each and have a running maximum, sum and
-// accumulator of their own, joined once at the end of the piece; with more rows (up to 64 per CTA) two or four warps share
-// the keys and differ in their rows.
+// sequence's end are copied too: their scores are masked and their V rows made zeros.  With up to 16 rows the four warps
+// take a quarter of a tile's keys each and have a reference, sum and accumulator of their own, joined once at the end of the
+// piece; with more rows (up to 64 per CTA) two or four warps share the keys and differ in their rows.
+// (16-byte copies by all threads: 98 us for 16 x 8 heads x 8192 keys in e4m3; with the loader 68; keys along the 16 rows 55;
+// the loader's registers to the others 53.)
 //
-// Split over the cache's length: all tiles of all (sequence, key head, row tile) items form one line that the CTAs (two
-// per SM) share evenly, whatever the lengths are: they are read on the device.  An item that falls to several CTAs leaves
-// at most two pieces per CTA in the workspace (unnormalised sums, maximum, sum), and a second kernel joins them in a
-// fixed order.  Where no item has more than a few tiles a CTA takes one item and there is no second kernel.
+// Split over the cache's length: all items (sequence, key head, row tile) lie on one line that the CTAs (two per SM) share
+// evenly, whatever the lengths are: they are read on the device.  An item that falls to several CTAs leaves at most two pieces
+// per CTA in the workspace (unnormalised sums, maximum, sum), and a second kernel joins them in a fixed order.  Where items
+// are short a CTA takes one item and there is no second kernel (see plan_of).
 //
 // e4m3 cache: K and V rows are widened to fp16 (exact), q is scaled by a power of two per row into fp16's range (exact but
 // for elements 2^-24 below the row's largest).  K's row scale multiplies the score.  V's row scale 2^e joins the exponent
-// of the weight, w = exp2(s + e - running maximum of (s + e)), so that the fp16 weights are always taken relative to the
+// of the weight, w = exp2(s + e - reference of (s + e)), so that the fp16 weights are always taken relative to the
 // largest CONTRIBUTION; the row sum keeps a maximum of its own.
 // Weights against an e4m3 cache are rounded to fp16 (scaled by 2^7, so that only weights 2^-21 of the largest or less are
 // subnormal).  Against a bf16 cache up to 16 rows take them as the sum of two bf16 numbers, 2^-17 of them off: rounded once
@@ -1075,8 +1079,16 @@ int plan_of(int B, int Hq, int Hkv, int T, int D, bool q8, int max_len, int sms,
   const int64_t items = B * (int64_t)Hkv * rt;
   LVAR_REQUIRE(items < (1ll << 24), LVAR_ERR_LIMIT, "too many (sequence, key head, row tile) items");
   out->rt = (int)rt;
-  out->split = tiles > 2;
-  out->ctas = out->split ? ctas_per_sm(D, q8, out->nb) * sms : (int)items;
+  // Whether items are split.  A split costs the second kernel and a longer start, as much as six tiles of an item take one
+  // after the other; without it the longest item's tiles count, whatever the others have.  Where all items are under way at
+  // once that is worth it while the tiles that a CTA would be spared are at most six, taking the lengths to be half the bound
+  // on average (bf16, D = 128, keys: 32 items 256: 6.6 against 8.6 us split, 512: 9.5 / 9.1; 256 items 256: 7.4 / 13.0,
+  // 512: 10.6 / 15.4, 1024: 24.4 / 30.5; e4m3, 64 rows, 256 items 256: 19.9 / 32.2).  With more items a CTA per item pays
+  // for its start each time (1024 items, bf16 128: 19.9 / 18.9, e4m3 512: 36.9 / 34.3), least where rows are many (e4m3, 64
+  // rows, 384: 101.8 / 110.4).
+  const int64_t slots = (int64_t)ctas_per_sm(D, q8, out->nb) * sms;
+  out->split = items <= slots ? tiles * (2 * slots - items) > 12 * slots : tiles > (out->wr == 1 ? 2 : 6);
+  out->ctas = (int)(out->split ? slots : items);
   out->workspace = out->split ? (int64_t)out->ctas * (kSlotsPerCta * rc * (D + 2) * 4 + 16) : 0;
   return LVAR_OK;
 }
