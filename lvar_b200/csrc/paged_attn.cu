@@ -133,7 +133,9 @@ __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
   return r;
 }
 // Token of a (token, query head) row.
-__device__ __forceinline__ int token_of(int r, int T, int G) { return T == 1 ? 0 : (int)((uint32_t)r / (uint32_t)G); }
+__device__ __forceinline__ int token_of(int r, int T, int G) {
+  return T == 1 ? 0 : G == 1 ? r : (int)((uint32_t)r / (uint32_t)G);
+}
 __device__ __forceinline__ float pow2i(int e) { return __int_as_float((e + 127) << 23); }  // -126 <= e <= 127
 
 // CTAs per SM: two; three of smaller tiles' worth where a warp's state is small and a key's bytes are few.
@@ -897,6 +899,7 @@ __global__ void __launch_bounds__(kAllThreads, (Geo<D, Q8, NB, WR>::CTAS))
       constexpr int TPR = D / 8, RPP = kThreads / TPR;
       const int e0 = (tid % TPR) * 8;
       const int live = min(X::RC, p.R - rt * X::RC);
+#pragma unroll 4
       for (int row = tid / TPR; row < live; row += RPP) {
         const int w0 = row / X::RW, in = row % X::RW, ex = e0 ^ ((in >> 1 & 3) * 8);
         float top = -INFINITY, sum = 0.f, v[8] = {};
@@ -906,7 +909,7 @@ __global__ void __launch_bounds__(kAllThreads, (Geo<D, Q8, NB, WR>::CTAS))
         for (int w = 0; w < WK; ++w) {
           const int at = (w * WR + w0) * X::RW + in;
           const float mw = ml[at * 2];
-          sum += mw == -INFINITY ? 0.f : ml[at * 2 + 1] * fast_exp2(mw - top);
+          sum += WK == 1 ? ml[at * 2 + 1] : mw == -INFINITY ? 0.f : ml[at * 2 + 1] * fast_exp2(mw - top);
           const float4 x = *reinterpret_cast<const float4*>(buf + at * D + ex);
           const float4 y = *reinterpret_cast<const float4*>(buf + at * D + ex + 4);
           v[0] += x.x, v[1] += x.y, v[2] += x.z, v[3] += x.w;
