@@ -1,7 +1,8 @@
 """In-tree build of ``liblvar_b200.so`` (sm_100a only) with plain nvcc.
 
 ``python -m lvar_b200.build`` compiles every ``csrc/*.cu`` to an object file and links them into
-``lvar_b200/liblvar_b200.so``.  Objects are rebuilt only when a source or header is newer.  nvcc
+``lvar_b200/liblvar_b200.so``, and ``csrc/paged_host.cpp`` (the Python entry of the paged-cache calls, over the same
+library and torch's headers) into ``lvar_b200/_paged_host.so``.  Objects are rebuilt only when a source or header is newer.  nvcc
 cross-compiles for sm_100a, so this also runs on a machine without a GPU.
 """
 from __future__ import annotations
@@ -10,6 +11,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
@@ -18,6 +20,7 @@ CSRC = PKG_DIR / "csrc"
 INCLUDE = PKG_DIR.parent / "include"
 BUILD_DIR = PKG_DIR / "build"
 LIB_PATH = PKG_DIR / "liblvar_b200.so"
+HOST_PATH = PKG_DIR / "_paged_host.so"
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -39,6 +42,25 @@ def _stale(target: Path, deps: list[Path]) -> bool:
         return True
     t = target.stat().st_mtime
     return any(d.stat().st_mtime > t for d in deps)
+
+
+def _build_host(force: bool) -> None:
+    """The C++ entry of the paged-cache calls: a CPython module that links the library beside it and torch."""
+    src = CSRC / "paged_host.cpp"
+    if not (force or _stale(HOST_PATH, [src, INCLUDE / "lvar_b200.h"])):
+        return
+    import torch
+    root = Path(torch.__file__).resolve().parent
+    cuda = Path(os.environ.get("CUDA_HOME", Path(_nvcc()).resolve().parent.parent))
+    cmd = [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-shared", "-fPIC",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           "-isystem", str(root / "include"), "-isystem", str(root / "include" / "torch" / "csrc" / "api" / "include"),
+           "-isystem", str(cuda / "include"), "-isystem", sysconfig.get_paths()["include"], str(src), "-o", str(HOST_PATH),
+           "-L", str(PKG_DIR), "-l:liblvar_b200.so", "-Wl,-rpath,$ORIGIN",
+           "-L", str(root / "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python"]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"g++ failed on {src.name}:\n{res.stdout}\n{res.stderr}")
 
 
 def build(force: bool = False, verbose: bool = False) -> Path:
@@ -67,6 +89,7 @@ def build(force: bool = False, verbose: bool = False) -> Path:
         res = subprocess.run(cmd, capture_output=True, text=True)
         if res.returncode != 0:
             raise RuntimeError(f"link failed:\n{res.stdout}\n{res.stderr}")
+    _build_host(force)
     if verbose:
         for name, log in logs:
             keep = [ln for ln in log.splitlines() if "registers" in ln or "spill" in ln or "warning" in ln]

@@ -15,6 +15,11 @@ import torch
 from . import _lib
 from ._lib import AttnArgs, check, lib
 
+try:
+    from . import _paged_host  # links the library that _lib has loaded
+except ImportError as e:
+    raise ImportError("lvar_b200/_paged_host.so is missing or does not load: build it with `python -m lvar_b200.build`") from e
+
 
 _raw_stream = torch._C._cuda_getCurrentRawStream  # (device index) -> cudaStream_t of torch's current stream
 
@@ -675,8 +680,9 @@ def qkv_prologue(qkv: torch.Tensor, scale_mul: Optional[torch.Tensor], rope_cos:
 
 
 # -- paged key/value cache -------------------------------------------------------------------------
-# These calls serve steps of one token, where the host's share counts: a call makes one pass of cheap comparisons and packs
-# the C structure in one go; what it refuses is worked out in detail only then.
+# These calls serve steps of one token, where the host's share counts.  Ordinary ones go through the compiled entry
+# (``csrc/paged_host.cpp``); what it does not take - outputs of the caller's, tensors on a device that is not current, and
+# everything that has to be refused - comes here, where each field is checked and named.
 _BF16, _E4M3, _I32, _F32, _U8 = torch.bfloat16, torch.float8_e4m3fn, torch.int32, torch.float32, torch.uint8
 _current_device = torch._C._cuda_getDevice
 _PACK_WRITE, _PACK_READ, _PACK_ATTN = _lib.packer(_lib.PagedWriteArgs), _lib.packer(_lib.PagedReadArgs), _lib.packer(_lib.PagedAttnArgs)
@@ -781,6 +787,8 @@ def paged_kv_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_p
     bf16, or float8_e4m3fn with ``scales`` uint8 [pages, H, page_size, 2]: the biased exponents of every row's power of two,
     K's and V's.  ``table`` int32 [B, n]: position p lies in page ``table[b, p // page_size]``.  ``start``, ``count``: int32
     [B] on the device.  A position without a page is not written and sets ``status`` (see :func:`new_status`)."""
+    if _paged_host.append(k, v, k_pages, v_pages, table, start, scales, count, status):
+        return
     c, dev = _paged_cache(k_pages, v_pages, table, scales)
     shape = k.shape
     if (len(shape) != 4 or k.dtype is not _BF16 or v.dtype is not _BF16 or v.shape != shape or shape[0] != c[17] or
@@ -816,6 +824,10 @@ def paged_qkv_prologue(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_page
     ``rope_cos``, ``rope_sin`` fp32 [P, D/2]: row p rotates the token at cache position p, element pairs (2i, 2i + 1), or
     (i, i + D/2) with ``rope_halves``.  The cache arguments, ``start``, ``count`` and ``status`` are those of
     :func:`paged_kv_append`; q rows of padding are 0."""
+    done = _paged_host.prologue(q, k, v, k_pages, v_pages, table, start, scales, scale_mul, q_weight, k_weight, eps, rope_cos,
+                                rope_sin, rope_halves, count, status)
+    if done is not None:
+        return done
     c, dev = _paged_cache(k_pages, v_pages, table, scales)
     shape, kshape = q.shape, k.shape
     if (len(shape) != 4 or q.dtype is not _BF16 or k.dtype is not _BF16 or v.dtype is not _BF16 or v.shape != kshape or
@@ -874,8 +886,14 @@ def paged_kv_read(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Ten
     rows at or behind ``lens[b]`` (int32 [B] on the device): the contiguous tensors that the many-query attention calls
     take.  ``out``: an optional pair of destinations (bf16, unit stride along D, other strides in multiples of 8).  An e4m3
     row comes back exactly as the values it stands for.  The cache arguments are those of :func:`paged_kv_append`."""
+    if out is None:
+        done = _paged_host.read(k_pages, v_pages, table, lens, n, scales, start, status)
+        if done is not None:
+            return done
     c, dev = _paged_cache(k_pages, v_pages, table, scales)
-    B, n = c[17], int(n)
+    B, n, start = c[17], int(n), int(start)
+    if n < 0 or start < 0 or start + n > 1 << 30:
+        raise RuntimeError(f"rows {start} .. {start + n - 1} are no range below 2^30")
     shape = (B, c[15], n, c[16])
     lens_ptr = _paged_ints("lens", lens, B, dev)
     st = _paged_status(status, dev)
@@ -892,7 +910,7 @@ def paged_kv_read(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Ten
         k_sb, k_sh, k_sl, _ = k.stride()
         v_sb, v_sh, v_sl, _ = v.stride()
         _paged_call(lib.lvar_paged_read, _PACK_READ(*c, k.data_ptr(), k_sb, k_sh, k_sl, v.data_ptr(), v_sb, v_sh, v_sl, lens_ptr,
-                                                    st, int(start), n), dev)
+                                                    st, start, n), dev)
     return k, v
 
 
@@ -910,6 +928,11 @@ def paged_attn_fwd(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
     A row that sees no key is 0 (M = -inf, L = 0).  ``max_len``: a bound on the lengths that shapes the launch (default: what
     the table holds); a longer sequence is cut there and sets ``status``.  ``out``: see :func:`_output_like`.  The cache
     arguments are those of :func:`paged_kv_append`."""
+    if out is None:
+        done = _paged_host.attn(q, k_pages, v_pages, table, lens, scale, scales, causal, max_len, return_stats, status,
+                                wait_limit_ns)
+        if done is not None:
+            return done
     c, dev = _paged_cache(k_pages, v_pages, table, scales)
     shape = q.shape
     if (len(shape) != 4 or q.dtype is not _BF16 or shape[0] != c[17] or shape[3] != c[16] or q.get_device() != dev):
@@ -924,6 +947,8 @@ def paged_attn_fwd(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
     lens_ptr = _paged_ints("lens", lens, B, dev)
     st = _paged_status(status, dev)
     most = min(c[18] * c[14], 1 << 30) if max_len is None else int(max_len)
+    if not 0 <= most <= 1 << 30:
+        raise RuntimeError(f"max_len must lie in 0 .. 2^30, got {most}")
     if out is None:
         o_sb, o_sh, o_sl = Hq * T * D, T * D, D
         o = torch.empty_strided((B, Hq, T, D), (o_sb, o_sh, o_sl, 1), dtype=_BF16, device=q.device)

@@ -556,6 +556,7 @@ def test_refusals(K):
         lambda: K.paged_attn_fwd(q, kb, vb, table, n, status=torch.zeros(1, device="cuda")),
         lambda: K.paged_kv_append(x, x[:1], kb, vb, table, n), lambda: K.paged_kv_append(q, q, kb, vb, table, n),
         lambda: K.paged_kv_append(x, x, kb, vb, table, n, count=n.float()),
+        lambda: K.paged_attn_fwd(q, kb, vb, table, n, max_len=1 << 40), lambda: K.paged_kv_read(kb, vb, table, n, 1 << 40),
         lambda: K.paged_kv_read(kb, vb, table, n, 5, start=-1), lambda: K.paged_kv_read(kb, vb, table, n, -1),
         lambda: K.paged_kv_read(kb, vb, table, n, 5, out=(x, x)),
         lambda: K.paged_qkv_prologue(t, t, t, kb, vb, table, n, scale_mul=one, eps=1e-6),
@@ -716,3 +717,73 @@ def test_generation_loop_over_pages(K, mode):
     finally:
         cfg.GLOBAL_CONFIG["attn"].clear()
         cfg.GLOBAL_CONFIG["attn"].update(saved)
+
+
+class _TakesNothing:
+    """The compiled entry as it answers calls that it leaves to the checks in Python."""
+
+    @staticmethod
+    def _none(*_):
+        return None
+    attn = append = prologue = read = _none
+
+
+@pytest.mark.parametrize("bits", [16, 8])
+def test_both_entries_make_the_same_call(K, bits, monkeypatch):
+    """The compiled entry and the Python one: the same launches from the same arguments, bit for bit."""
+    B, L, Hq, H, D, page = 3, 5, 6, 2, 64, 32
+    g = torch.Generator(device="cuda").manual_seed(111)
+    x = torch.randn(B, L, Hq + 2 * H, D, generator=g, device="cuda").bfloat16()
+    q, k, v = x[:, :, :Hq], x[:, :, Hq:Hq + H], x[:, :, Hq + H:]
+    start = torch.tensor([0, 40, 17], dtype=torch.int32, device="cuda")
+    count = torch.tensor([5, 2, 0], dtype=torch.int32, device="cuda")
+    table = torch.arange(6, device="cuda").view(3, 2).to(torch.int32)
+    ang = torch.rand(64, D // 2, generator=g, device="cuda")
+    kinds = [{}, {"scale_mul": torch.rand(Hq, generator=g, device="cuda")}, {"eps": 1e-5},
+             {"eps": 1e-5, "q_weight": torch.rand(D, generator=g, device="cuda"), "k_weight": torch.rand(D, generator=g, device="cuda")}]
+
+    def all_of_them():
+        out = []
+        for kw in kinds:
+            for rope in ({}, {"rope_cos": ang, "rope_sin": ang, "rope_halves": True}):
+                kp, vp, sc = empty_cache(6, H, page, D, bits)
+                st = K.new_status("cuda")
+                out.append(K.paged_qkv_prologue(q, k, v, kp, vp, table, start, scales=sc, count=count, status=st, **kw, **rope))
+                K.paged_kv_append(k.transpose(1, 2), v.transpose(1, 2), kp, vp, table, start + 6, scales=sc, status=st)
+                out += [kp, vp, st] + ([] if sc is None else [sc])
+                out += K.paged_kv_read(kp, vp, table, start + 11, 60, scales=sc, start=1, status=st)
+                qh = q.transpose(1, 2)
+                out.append(K.paged_attn_fwd(qh, kp, vp, table, start + 11, scales=sc, status=st))
+                out += K.paged_attn_fwd(qh, kp, vp, table, start + 11, 0.3, scales=sc, causal=True, max_len=60, return_stats=True,
+                                        status=st, wait_limit_ns=10 ** 9)
+                out += K.paged_attn_fwd(qh, kp, vp, table.repeat(1, 20), start + 11, scales=sc, return_stats=True)
+                assert K.read_status(st)[0] == 0
+        return [t.clone().view(torch.uint8) for t in out]
+    a = all_of_them()
+    monkeypatch.setattr(K, "_paged_host", _TakesNothing)
+    b = all_of_them()
+    assert len(a) == len(b) and all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+def test_the_compiled_entry_leaves_wrong_calls_alone(K):
+    """It answers None, raises only where a number is none, and keeps no reference that it should not."""
+    import sys
+    from lvar_b200 import _paged_host as host
+    k, v, sc, table = make_cache(2, 2, 64, 16, 64, 16, 81)
+    n = torch.tensor([3, 4], dtype=torch.int32, device="cuda")
+    q = torch.zeros(2, 4, 1, 64, dtype=torch.bfloat16, device="cuda")
+    good = [q, k, v, table, n, 0.1, None, False, None, False, None, None]
+    for i, wrong in ((0, q.cpu()), (0, q.half()), (0, None), (0, q[:, :3]), (1, k[:, :, :, ::2]), (3, table.long()), (4, n.long()),
+                     (4, None), (6, torch.zeros(1)), (8, -1), (8, 1 << 40), (8, "x"), (10, q), (11, -1)):
+        args = list(good)
+        args[i] = wrong
+        assert host.attn(*args) is None, i
+    with pytest.raises(TypeError):
+        host.attn(*good[:-1])
+    with pytest.raises(TypeError):
+        host.attn(*good[:5], "scale", *good[6:])
+    before = [sys.getrefcount(x) for x in (q, k, v, table, n)]
+    for _ in range(50):
+        host.attn(*good)
+    assert before == [sys.getrefcount(x) for x in (q, k, v, table, n)]
+    assert sys.getrefcount(host.attn(*good)) <= 2
