@@ -140,37 +140,34 @@ __device__ __forceinline__ float pow2i(int e) { return __int_as_float((e + 127) 
 
 // CTAs per SM: two; three of smaller tiles' worth where a warp's state is small and a key's bytes are few.
 __host__ __device__ constexpr int ctas_per_sm(int D, bool q8, int nb) { return D == 64 && q8 && nb == 1 ? 3 : 2; }
-__host__ __device__ constexpr int keys_per_tile(int D, bool q8, int wr) { return D == 64 || (q8 && wr == 1) ? 128 : 64; }
+__host__ __device__ constexpr int keys_per_tile(int D, bool q8) { return D == 64 || q8 ? 128 : 64; }
 
 template <int D, bool Q8, int NB, int WR>
 struct Geo {
-  static constexpr bool WIDE = Q8 && WR > 1;              // tiles are widened to fp16 once for the warps that share them
   static constexpr int RB = D * (Q8 ? 1 : 2);             // bytes of a cached row
   static constexpr int RS = RB < 128 ? RB : 128;          // bytes of a row of a sub-tile, the widest that a copy swizzles
   static constexpr int SUBS = RB / RS;                    // sub-tiles side by side
-  static constexpr int KT = keys_per_tile(D, Q8, WR);     // keys per tile
+  static constexpr int KT = keys_per_tile(D, Q8);         // keys per tile
   static constexpr int SUB = KT * RS;                     // bytes of a sub-tile
   static constexpr int STAGE = 2 * KT * RB;               // K and V
   static constexpr int CTAS = ctas_per_sm(D, Q8, NB);     // per SM
   static constexpr int LAUNCH_REGS = CTAS == 3 ? 80 : 128;
   static constexpr int COMPUTE_REGS = 2 * LAUNCH_REGS - 24;
-  static constexpr int STAGES = WIDE ? 65536 / STAGE : (CTAS == 3 ? 65536 : 98304) / STAGE;
+  static constexpr int STAGES = (CTAS == 3 ? 65536 : STAGE <= 16384 ? 81920 : 98304) / STAGE;
   static constexpr int SCALE_STAGE = Q8 ? KT * 2 : 0;
-  static constexpr int WIDE_BYTES = WIDE ? 2 * KT * D * 2 : 0;
   // Queries come with an item's first tile where they are few; otherwise their readers load them.
   static constexpr int QROW = D * 2 + 16;                 // a row's bytes, padded so that eight rows differ in their banks
   static constexpr int Q_STAGE = WR == 1 ? 8 * NB * QROW : 0;
-  static constexpr int WIDE_AT = STAGES * (STAGE + SCALE_STAGE), Q_AT = WIDE_AT + WIDE_BYTES;
+  static constexpr int Q_AT = STAGES * (STAGE + SCALE_STAGE);
   static constexpr int RING = Q_AT + STAGES * Q_STAGE;
-  // what the matrix instructions' operands are read from: rows of 16-bit elements in sub-tiles of 128 bytes, or the stage
-  static constexpr int OS = WIDE ? 128 : RS, OSUB = KT * OS;
   static constexpr int RW = 8 * NB;                       // rows per warp
   static constexpr int RC = RW * WR;                      // rows per CTA
   static constexpr bool TWO = !Q8 && WR == 1;             // weights as the sum of two bf16 numbers
-  static constexpr int COST = WR == 1 ? 1 : 4;            // of an item beside its tiles, in tiles
+  static constexpr int COST = WR == 1 ? 1 : KT == 128 ? 2 : 4;  // of an item beside its tiles, in tiles
   static constexpr int ML = 4 * RW * 2;                   // maxima and sums of the four warps' rows, floats; twice
   static constexpr int SMEM = RING + 2 * ML * 4 + 2 * STAGES * 8 + 16 + 1024;  // and the start's alignment
-  static_assert(4 * RW * D * 4 <= (WIDE ? WIDE_BYTES : STAGE), "the warps' accumulators are joined in a consumed tile");
+  static_assert(4 * RW * D * 4 <= STAGE, "the warps' accumulators are joined in a consumed tile");
+  static_assert(CTAS * (SMEM + 1024) <= 228 * 1024, "what an SM has for that many CTAs");
 };
 
 // The swizzle of a sub-tile's row: what its 16-byte chunk numbers are XORed with (as the copies do).
@@ -390,27 +387,23 @@ __device__ __forceinline__ void weigh(State<D, NB>& st, const float (&sc)[NK][NB
           rest[nb][y] = transpose8(pack_bf16x2(w0 - __uint_as_float(two << 16), w1 - __uint_as_float(two & 0xffff0000u)));
       }
     }
-    if constexpr (!Q8 || X::WIDE) {
-      const uint32_t v0 = vs + (s0 + k * 16 + (lane & 7) + ((lane >> 4) << 3)) * X::OS + ((((lane >> 3) & 1) ^ (lane & 7)) << 4);
-      constexpr uint32_t kOdd = Q8 ? 0x7c00u : 0x7f80u;  // the exponent of an element that is not finite
+    if constexpr (!Q8) {
+      const uint32_t v0 = vs + (s0 + k * 16 + (lane & 7) + ((lane >> 4) << 3)) * X::RS + ((((lane >> 3) & 1) ^ (lane & 7)) << 4);
 #pragma unroll
       for (int t = 0; t < D / 16; ++t) {
         uint32_t a[4];
-        ldsm_x4_t((v0 ^ ((t & 3) << 5)) + (t >> 2) * X::OSUB, a);
+        ldsm_x4_t((v0 ^ ((t & 3) << 5)) + (t >> 2) * X::SUB, a);
         if constexpr (CLEAN) {
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            if ((a[j] & kOdd) == kOdd) a[j] &= 0xffff0000u;
-            if ((a[j] & (kOdd << 16)) == kOdd << 16) a[j] &= 0xffffu;
+            if ((a[j] & 0x7f80u) == 0x7f80u) a[j] &= 0xffff0000u;
+            if ((a[j] & 0x7f800000u) == 0x7f800000u) a[j] &= 0xffffu;
           }
         }
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
-          if constexpr (Q8) mma_f16(st.acc[t][nb], a, b[nb][0], b[nb][1]);
-          else {
-            mma_bf16(st.acc[t][nb], a, b[nb][0], b[nb][1]);
-            if constexpr (X::TWO) mma_bf16(st.acc[t][nb], a, rest[nb][0], rest[nb][1]);
-          }
+          mma_bf16(st.acc[t][nb], a, b[nb][0], b[nb][1]);
+          if constexpr (X::TWO) mma_bf16(st.acc[t][nb], a, rest[nb][0], rest[nb][1]);
         }
       }
     } else {
@@ -472,9 +465,9 @@ __device__ __forceinline__ bool any_odd(uint32_t vs, int s0, int rows) {
 
 // O^T += V^T P^T of a step with elements of V that are not finite: without them, and then row by row those that a row sees.
 template <class X, int D, bool Q8, int NB, int NK>
-__device__ __noinline__ void weigh_odd(State<D, NB>& st, const float (&sc)[NK][NB][4], const int (&seen)[NB][2], uint32_t operand,
-                                       uint32_t vs, int s0) {
-  weigh<X, D, Q8, NB, NK, true>(st, sc, operand, s0);
+__device__ __noinline__ void weigh_odd(State<D, NB>& st, const float (&sc)[NK][NB][4], const int (&seen)[NB][2], uint32_t vs,
+                                       int s0) {
+  weigh<X, D, Q8, NB, NK, true>(st, sc, vs, s0);
   const int quad = threadIdx.x & 3;
   for (int j = 0; j < NK * 16; ++j) {
     const int row = s0 + j, from = ((j & 7) << 2) | quad;  // the lane that has these rows' weights of key j
@@ -483,7 +476,7 @@ __device__ __noinline__ void weigh_odd(State<D, NB>& st, const float (&sc)[NK][N
         const float w = __shfl_sync(0xffffffffu, sc[j >> 4][nb][((j >> 3) & 1) * 2 + e], from);
         for (int t = 0; t < D / 16; ++t)
           for (int second = 0; second < 2; ++second) {
-            const int byte = element_of<D, Q8 && !X::WIDE>(t, second) * (Q8 ? 1 : 2), chunk = (byte % X::RS) >> 4;
+            const int byte = element_of<D, Q8>(t, second) * (Q8 ? 1 : 2), chunk = (byte % X::RS) >> 4;
             const uint32_t at = vs + byte / X::RS * X::SUB + row * X::RS + ((chunk ^ swizzle_of<X::RS>(row)) << 4) + (byte & 15);
             const uint32_t bits = lds32(at & ~3u) >> ((at & 3u) * 8);
             const float val = Q8 ? NAN : __uint_as_float(bits << 16);
@@ -610,21 +603,14 @@ __global__ void __launch_bounds__(kAllThreads, (Geo<D, Q8, NB, WR>::CTAS))
             qf[kk][nb][1] = live ? *reinterpret_cast<const uint32_t*>(src + kk * 16 + quad * 2 + 8) : 0u;
           }
         } else {
-          // operands widened in registers: matrix step 4 i + s takes elements 16 (2 quad + i) + 4 s + {0..3} (D = 64:
-          // 16 quad + 4 s) from this thread; else 16 kk + 2 quad + {0, 1} and + 8
+          // matrix step 4 i + s takes elements 16 (2 quad + i) + 4 s + {0..3} (D = 64: 16 quad + 4 s) from this thread
           constexpr int CH = D / 64;
           uint2 raw[D / 16];
           float most = 0.f;
           bool fine = true;
 #pragma unroll
-          for (int kk = 0; kk < D / 16; ++kk) {
-            if constexpr (X::WIDE) {
-              raw[kk].x = live ? *reinterpret_cast<const uint32_t*>(src + kk * 16 + quad * 2) : 0u;
-              raw[kk].y = live ? *reinterpret_cast<const uint32_t*>(src + kk * 16 + quad * 2 + 8) : 0u;
-            } else {
-              raw[kk] = live ? *reinterpret_cast<const uint2*>(src + 16 * (CH * quad + kk / 4) + 4 * (kk % 4)) : make_uint2(0u, 0u);
-            }
-          }
+          for (int kk = 0; kk < D / 16; ++kk)
+            raw[kk] = live ? *reinterpret_cast<const uint2*>(src + 16 * (CH * quad + kk / 4) + 4 * (kk % 4)) : make_uint2(0u, 0u);
 #pragma unroll
           for (int kk = 0; kk < D / 16; ++kk) {
             const uint32_t w[2] = {raw[kk].x, raw[kk].y};
@@ -655,35 +641,14 @@ __global__ void __launch_bounds__(kAllThreads, (Geo<D, Q8, NB, WR>::CTAS))
     if (!X::Q_STAGE) alive = alive && mbar_wait(&full[stage], phase, wait, DEV_TIMEOUT_SOFTMAX);
 
     const bool idle = rt * X::RC + wr * X::RW >= p.R || !alive;  // none of the warp's rows exists
-    const uint32_t raw_v = ring + stage * X::STAGE + X::KT * X::RB;
+    const uint32_t ks = ring + stage * X::STAGE, vs = ks + X::KT * X::RB;
     const uint32_t ss = ring + X::STAGES * X::STAGE + stage * X::SCALE_STAGE;
-    const uint32_t ks = X::WIDE ? ring + X::WIDE_AT : ring + stage * X::STAGE;
-    const uint32_t vs = ks + X::SUBS * X::KT * (X::WIDE ? D * 2 : X::RS);
-    if constexpr (X::WIDE) {
-      constexpr int CPR = X::RB / 16;
-      compute_sync();  // the last tile's readers are done
-#pragma unroll
-      for (int j = 0; j < 2 * X::KT * CPR / kThreads; ++j) {
-        const int at = j * kThreads + tid, row = at / CPR % X::KT, c = at % CPR, v = at / (CPR * X::KT);
-        uint4 w = lds128(ring + stage * X::STAGE + v * X::KT * X::RB + row * X::RB + ((c ^ swizzle_of<X::RS>(row)) << 4));
-        if (v && cons.tile * X::KT + row >= cons.len) w = make_uint4(0u, 0u, 0u, 0u);  // behind the sequence's end: anything
-        uint32_t o[8];
-        widen4(w.x, o[0], o[1]);
-        widen4(w.y, o[2], o[3]);
-        widen4(w.z, o[4], o[5]);
-        widen4(w.w, o[6], o[7]);
-        const uint32_t dst = (v ? vs : ks) + (c >> 2) * X::OSUB + row * 128;
-        sts128(dst + (((2 * c & 7) ^ (row & 7)) << 4), o[0], o[1], o[2], o[3]);
-        sts128(dst + (((2 * c & 7) + 1 ^ (row & 7)) << 4), o[4], o[5], o[6], o[7]);
-      }
-      compute_sync();
-    }
 #pragma unroll 1
     for (int s0 = wk * KW; s0 < (wk + 1) * KW; s0 += NS) {
       const int key0 = cons.tile * X::KT + s0;
       if (key0 >= cons.len || idle) break;  // the same for the whole warp
       const int rows = cons.len - key0;  // of the step's keys
-      if (!X::WIDE && rows < NS) {
+      if (rows < NS) {
         // V rows behind the sequence's end become zeros: what a copy brought along or an earlier tile left may be anything
 #pragma unroll
         for (int s = 0; s < X::SUBS; ++s)
@@ -696,19 +661,16 @@ __global__ void __launch_bounds__(kAllThreads, (Geo<D, Q8, NB, WR>::CTAS))
       for (int k = 0; k < NK; ++k)
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) sc[k][nb][0] = sc[k][nb][1] = sc[k][nb][2] = sc[k][nb][3] = 0.f;
-      if constexpr (!Q8 || X::WIDE) {
-        const uint32_t k0 = ks + (s0 + (lane & 15)) * X::OS + (((lane >> 4) ^ (lane & 7)) << 4);
+      if constexpr (!Q8) {
+        const uint32_t k0 = ks + (s0 + (lane & 15)) * X::RS + (((lane >> 4) ^ (lane & 7)) << 4);
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) {
 #pragma unroll
           for (int k = 0; k < NK; ++k) {
             uint32_t a[4];
-            ldsm_x4((k0 ^ ((kk & 3) << 5)) + (kk >> 2) * X::OSUB + k * 16 * X::OS, a);
+            ldsm_x4((k0 ^ ((kk & 3) << 5)) + (kk >> 2) * X::SUB + k * 16 * X::RS, a);
 #pragma unroll
-            for (int nb = 0; nb < NB; ++nb) {
-              if constexpr (Q8) mma_f16(sc[k][nb], a, qf[kk][nb][0], qf[kk][nb][1]);
-              else mma_bf16(sc[k][nb], a, qf[kk][nb][0], qf[kk][nb][1]);
-            }
+            for (int nb = 0; nb < NB; ++nb) mma_bf16(sc[k][nb], a, qf[kk][nb][0], qf[kk][nb][1]);
           }
         }
       } else {
@@ -833,7 +795,7 @@ __global__ void __launch_bounds__(kAllThreads, (Geo<D, Q8, NB, WR>::CTAS))
       }
       // In a step that some row does not see all of, elements of V that are not finite come in row by row: a weight of zero
       // would make NaN of them in rows that do not see them.
-      if (edge && any_odd<X, Q8, NS>(raw_v, s0, rows)) {
+      if (edge && any_odd<X, Q8, NS>(vs, s0, rows)) {
         State<D, NB> st2 = st;
         float w[NK][NB][4];
         int seen[NB][2];
@@ -846,7 +808,7 @@ __global__ void __launch_bounds__(kAllThreads, (Geo<D, Q8, NB, WR>::CTAS))
           seen[nb][0] = limit[nb][0] - key0;
           seen[nb][1] = limit[nb][1] - key0;
         }
-        weigh_odd<X, D, Q8, NB, NK>(st2, w, seen, vs, raw_v, s0);
+        weigh_odd<X, D, Q8, NB, NK>(st2, w, seen, vs, s0);
         st = st2;
       } else {
         weigh<X, D, Q8, NB, NK, false>(st, sc, vs, s0);
@@ -867,7 +829,7 @@ __global__ void __launch_bounds__(kAllThreads, (Geo<D, Q8, NB, WR>::CTAS))
         }
       compute_sync();
       // [warp][row][D]; elements are XORed with 8 times bits 1 and 2 of the row, so that a warp's rows differ in their banks
-      float* buf = reinterpret_cast<float*>(smem + (X::WIDE ? X::WIDE_AT : stage * X::STAGE));
+      float* buf = reinterpret_cast<float*>(smem + stage * X::STAGE);
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
@@ -880,7 +842,7 @@ __global__ void __launch_bounds__(kAllThreads, (Geo<D, Q8, NB, WR>::CTAS))
           const float own = Q8 ? st.tref[nb][e] - kUp : st.ref[nb][e];
           const float f = own == -INFINITY ? 0.f : fast_exp2(own - top);
           float* dst = buf + (warp * X::RW + row) * D;
-          if constexpr (!Q8 || X::WIDE) {
+          if constexpr (!Q8) {
 #pragma unroll
             for (int t = 0; t < D / 16; ++t) {
               dst[element_of<D, false>(t, 0) ^ (quad * 8)] = st.acc[t][nb][e] * f;
@@ -1077,20 +1039,19 @@ int plan_of(int B, int Hq, int Hkv, int T, int D, bool q8, int max_len, int sms,
   out->wr = R <= 16 ? 1 : R <= 32 ? 2 : 4;
   const int rc = 8 * out->nb * out->wr;
   const int64_t rt = (R + rc - 1) / rc;
-  const int kt = keys_per_tile(D, q8, out->wr);
+  const int kt = keys_per_tile(D, q8);
   const int64_t tiles = max_len <= kt ? 1 : ((int64_t)max_len + kt - 1) / kt;
   const int64_t items = B * (int64_t)Hkv * rt;
   LVAR_REQUIRE(items < (1ll << 24), LVAR_ERR_LIMIT, "too many (sequence, key head, row tile) items");
   out->rt = (int)rt;
-  // Whether items are split.  A split costs the second kernel and a longer start, as much as six tiles of an item take one
+  // Whether items are split.  A split costs the second kernel and a longer start, as much as `spare` tiles of an item take one
   // after the other; without it the longest item's tiles count, whatever the others have.  Where all items are under way at
-  // once that is worth it while the tiles that a CTA would be spared are at most six, taking the lengths to be half the bound
-  // on average (bf16, D = 128, keys: 32 items 256: 6.6 against 8.6 us split, 512: 9.5 / 9.1; 256 items 256: 7.4 / 13.0,
-  // 512: 10.6 / 15.4, 1024: 24.4 / 30.5; e4m3, 64 rows, 256 items 256: 19.9 / 32.2).  With more items a CTA per item pays
-  // for its start each time (1024 items, bf16 128: 19.9 / 18.9, e4m3 512: 36.9 / 34.3), least where rows are many (e4m3, 64
-  // rows, 384: 101.8 / 110.4).
-  const int64_t slots = (int64_t)ctas_per_sm(D, q8, out->nb) * sms;
-  out->split = items <= slots ? tiles * (2 * slots - items) > 12 * slots : tiles > (out->wr == 1 ? 2 : 6);
+  // once that is worth it while the tiles that a CTA would be spared are at most `spare`, taking the lengths to be half the
+  // bound on average (bf16, D = 128, keys: 32 items 256: 6.6 against 8.6 us split, 512: 9.5 / 9.1; 256 items 256: 7.4 / 13.0,
+  // 512: 10.6 / 15.4, 1024: 24.4 / 30.5; e4m3, 64 rows, 32 items 512: 21.2 / 21.1).  With more items a CTA per item pays for
+  // its start each time (1024 items, bf16 128: 19.9 / 18.9, e4m3 512: 36.9 / 34.3), least where rows are many.
+  const int64_t slots = (int64_t)ctas_per_sm(D, q8, out->nb) * sms, spare = out->wr == 4 && kt == 128 ? 4 : 6;
+  out->split = items <= slots ? tiles * (2 * slots - items) > 2 * spare * slots : tiles > (out->wr == 1 ? 2 : spare);
   out->ctas = (int)(out->split ? slots : items);
   out->workspace = out->split ? (int64_t)out->ctas * (kSlotsPerCta * rc * (D + 2) * 4 + 16) : 0;
   return LVAR_OK;
@@ -1124,7 +1085,7 @@ int launch(const PagedAttnParams& p, const CUtensorMap& mk, const CUtensorMap& m
 
 template <int D, bool Q8>
 int launch_wr(PagedAttnParams& p, const lvar_paged_cache& c, const Plan& plan, cudaStream_t stream) {
-  const int KT = keys_per_tile(D, Q8, plan.wr);
+  const int KT = keys_per_tile(D, Q8);
   // Rows per copy: what page and tile have in common, and not far more than the longest sequence has.
   int box = KT;
   while (c.page_size % box != 0 || KT % box != 0) box -= 16;
