@@ -138,8 +138,9 @@ __device__ __forceinline__ int token_of(int r, int T, int G) {
 }
 __device__ __forceinline__ float pow2i(int e) { return __int_as_float((e + 127) << 23); }  // -126 <= e <= 127
 
-// CTAs per SM: two; three of smaller tiles' worth where a warp's state is small and a key's bytes are few.
-__host__ __device__ constexpr int ctas_per_sm(int D, bool q8, int nb) { return D == 64 && q8 && nb == 1 ? 3 : 2; }
+// CTAs per SM: two; three where a warp's state is small, a key's bytes are few and the warps have keys of their own (e4m3,
+// D = 64: 496 items of 10 rows x 5775 keys 102 against 117 us with two; 104 items of 32 rows x 3185 keys 35 against 31).
+__host__ __device__ constexpr int ctas_per_sm(int D, bool q8, int wr) { return D == 64 && q8 && wr == 1 ? 3 : 2; }
 __host__ __device__ constexpr int keys_per_tile(int D, bool q8) { return D == 64 || q8 ? 128 : 64; }
 
 template <int D, bool Q8, int NB, int WR>
@@ -150,10 +151,10 @@ struct Geo {
   static constexpr int KT = keys_per_tile(D, Q8);         // keys per tile
   static constexpr int SUB = KT * RS;                     // bytes of a sub-tile
   static constexpr int STAGE = 2 * KT * RB;               // K and V
-  static constexpr int CTAS = ctas_per_sm(D, Q8, NB);     // per SM
+  static constexpr int CTAS = ctas_per_sm(D, Q8, WR);     // per SM
   static constexpr int LAUNCH_REGS = CTAS == 3 ? 80 : 128;
   static constexpr int COMPUTE_REGS = 2 * LAUNCH_REGS - 24;
-  static constexpr int STAGES = (CTAS == 3 ? 65536 : STAGE <= 16384 ? 81920 : 98304) / STAGE;
+  static constexpr int STAGES = (CTAS == 3 ? (NB == 1 ? 65536 : 49152) : STAGE <= 16384 ? 81920 : 98304) / STAGE;
   static constexpr int SCALE_STAGE = Q8 ? KT * 2 : 0;
   // Queries come with an item's first tile where they are few; otherwise their readers load them.
   static constexpr int QROW = D * 2 + 16;                 // a row's bytes, padded so that eight rows differ in their banks
@@ -1050,7 +1051,7 @@ int plan_of(int B, int Hq, int Hkv, int T, int D, bool q8, int max_len, int sms,
   // bound on average (bf16, D = 128, keys: 32 items 256: 6.6 against 8.6 us split, 512: 9.5 / 9.1; 256 items 256: 7.4 / 13.0,
   // 512: 10.6 / 15.4, 1024: 24.4 / 30.5; e4m3, 64 rows, 32 items 512: 21.2 / 21.1).  With more items a CTA per item pays for
   // its start each time (1024 items, bf16 128: 19.9 / 18.9, e4m3 512: 36.9 / 34.3), least where rows are many.
-  const int64_t slots = (int64_t)ctas_per_sm(D, q8, out->nb) * sms, spare = out->wr == 4 && kt == 128 ? 4 : 6;
+  const int64_t slots = (int64_t)ctas_per_sm(D, q8, out->wr) * sms, spare = out->wr == 4 && kt == 128 ? 4 : 6;
   out->split = items <= slots ? tiles * (2 * slots - items) > 2 * spare * slots : tiles > (out->wr == 1 ? 2 : spare);
   out->ctas = (int)(out->split ? slots : items);
   out->workspace = out->split ? (int64_t)out->ctas * (kSlotsPerCta * rc * (D + 2) * 4 + 16) : 0;

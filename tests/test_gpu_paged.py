@@ -245,7 +245,7 @@ def place(table, page, start, b, l):
 
 
 @pytest.mark.parametrize("bits", [16, 8])
-@pytest.mark.parametrize("B,H,L,D,page", [(1, 1, 1, 128, 16), (3, 5, 37, 64, 16), (2, 3, 70, 128, 48), (4, 2, 300, 64, 64)])
+@pytest.mark.parametrize("B,H,L,D,page", [(1, 1, 1, 128, 16), (3, 5, 37, 64, 16), (2, 3, 70, 128, 48), (4, 2, 300, 64, 64), (3, 1, 51, 64, 16), (2, 1, 33, 128, 32)])
 def test_append_and_read(K, bits, B, H, L, D, page):
     """Exact: rows, their scales, everything around them, and the way back."""
     g = torch.Generator(device="cuda").manual_seed(L + D)
