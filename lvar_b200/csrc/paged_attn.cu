@@ -19,7 +19,7 @@
 // (16-byte copies by all threads: 98 us for 16 x 8 heads x 8192 keys in e4m3; with the loader 68; keys along the 16 rows 55;
 // the loader's registers to the others 53.)
 //
-// Split over the cache's length: all items (sequence, key head, row tile) lie on one line that the CTAs (two per SM) share
+// Split over the cache's length: all items (sequence, key head, row tile) lie on one line that the CTAs (two or three per SM) share
 // evenly, whatever the lengths are: they are read on the device.  An item that falls to several CTAs leaves at most two pieces
 // per CTA in the workspace (unnormalised sums, maximum, sum), and a second kernel joins them in a fixed order.  Where items
 // are short a CTA takes one item and there is no second kernel (see plan_of).

@@ -108,12 +108,10 @@ __device__ __forceinline__ uint32_t narrow4(float a, float b, float c, float d) 
   return r;
 }
 
-// Row scales of an e4m3 cache: the least e with most * 2^-e <= 448, for most = s * 2^q with 1 <= s < 2 and 448 = 1.75 * 2^8:
-// q - 8, and one more where s > 1.75.
-__device__ __forceinline__ int exponent_for(float most) {
-  const uint32_t bits = __float_as_uint(most);
-  const int e = (int)(bits >> 23) - 127 - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0);
-  return most == 0.f ? -100 : min(max(e, -100), 120);
+// Biased exponent of a row's scale: the least e with most * 2^-e <= 448 = 1.75 * 2^8, -100 <= e <= 120.  For most = s * 2^q
+// with 1 <= s < 2 that is q - 8, and one more where s > 1.75: the addend carries into the exponent just then.
+__device__ __forceinline__ int scale_byte(float most) {
+  return min(max((int)((__float_as_uint(most) + 0x1fffffu) >> 23) - 8, 27), 247);
 }
 
 // A CTA's eight warps take a token each; a warp takes RPW * U rows of one kind (q, k or v heads), grid.y says which.  Where
@@ -221,7 +219,9 @@ __global__ void __launch_bounds__(256, PLAIN ? 6 : 3) paged_write_kernel(const _
     for (int u = 0; u < U; ++u) store(u, {0u, 0u, 0u, 0u});
     return;
   }
-  if (PLAIN || (kind == 2 && !Q8)) {  // as they are
+  bool copy = kind == 2 && !Q8;
+  if (PLAIN) copy = true;
+  if (copy) {  // as they are
 #pragma unroll
     for (int u = 0; u < U; ++u) store(u, {raw[u][0].x, raw[u][0].y, raw[u][1].x, raw[u][1].y});
     return;
@@ -346,8 +346,8 @@ __global__ void __launch_bounds__(256, PLAIN ? 6 : 3) paged_write_kernel(const _
   }
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    const int e = exponent_for(most[u]);
-    const float down = __uint_as_float((uint32_t)(127 - e) << 23);
+    const int byte = scale_byte(most[u]);
+    const float down = __uint_as_float((uint32_t)(254 - byte) << 23);
     const uint64_t dd = pack_f32x2(down, down);
     float a[4], c[4];
     unpack_f32x2(fmul2(A[u][0], dd), a[0], a[1]), unpack_f32x2(fmul2(A[u][1], dd), a[2], a[3]);
@@ -361,7 +361,7 @@ __global__ void __launch_bounds__(256, PLAIN ? 6 : 3) paged_write_kernel(const _
     } else {
       *reinterpret_cast<uint2*>(dst + e0) = make_uint2(narrow4(a[0], c[0], a[1], c[1]), narrow4(a[2], c[2], a[3], c[3]));
     }
-    if (x == 0) p.c.scales[at.page * p.c.s_sp + h * p.c.s_sh + at.row * 2 + (kind - 1)] = (uint8_t)(e + 127);
+    if (x == 0) p.c.scales[at.page * p.c.s_sp + h * p.c.s_sh + at.row * 2 + (kind - 1)] = (uint8_t)byte;
   }
 }
 
