@@ -122,9 +122,9 @@ __device__ __forceinline__ int scale_byte(float most) {
 // A row whose kind is decided row by row, with a library root, reciprocal and unpacked arithmetic, cost 210 instructions a
 // lane and bound the kernel by issue: 52 us for 2 x 4096 tokens x 48 heads x 128, 38 us now (0.81 of the
 // measured copy rate; two rows a lane instead of four 48 us).
-// PLAIN: rows go as they are, without norm, rotation or a change of type.
-template <int C, bool HALVES, bool Q8, bool PLAIN, int U>
-__global__ void __launch_bounds__(256, PLAIN ? 6 : 3) paged_write_kernel(const __grid_constant__ WriteParams p, int cq, int ck, int tsh) {
+// BARE: rows go without norm and rotation (to a bf16 cache: as they are).
+template <int C, bool HALVES, bool Q8, bool BARE, int U>
+__global__ void __launch_bounds__(256, BARE ? (Q8 ? 4 : 6) : 3) paged_write_kernel(const __grid_constant__ WriteParams p, int cq, int ck, int tsh) {
   constexpr int LPR = C / 8, RPW = 32 / LPR;
   const int lane = threadIdx.x & 31;
   constexpr int LOG_RPW = C == 128 ? 1 : 2;
@@ -165,7 +165,7 @@ __global__ void __launch_bounds__(256, PLAIN ? 6 : 3) paged_write_kernel(const _
   }
   float mul[U];  // the heads' factors
 #pragma unroll
-  for (int u = 0; u < U; ++u) mul[u] = !PLAIN && kind == 0 && p.norm == 1 && h0 + u * RPW < heads ? __ldg(p.scale_mul + h0 + u * RPW) : 1.f;
+  for (int u = 0; u < U; ++u) mul[u] = !BARE && kind == 0 && p.norm == 1 && h0 + u * RPW < heads ? __ldg(p.scale_mul + h0 + u * RPW) : 1.f;
   const int first = p.start[b];
   const int pos = first < 0 || first > kMaxTokens ? -1 : first + l;
   Place at{-1, 0};
@@ -175,7 +175,7 @@ __global__ void __launch_bounds__(256, PLAIN ? 6 : 3) paged_write_kernel(const _
     if (!__any_sync(0xffffffffu, alive)) return;
   }
   uint64_t cs[2], sn[2], ns[2];  // cosines and sines of the lane's four rotations, and the sines negated
-  if (!PLAIN && p.cos_t != nullptr && kind < 2) {
+  if (!BARE && p.cos_t != nullptr && kind < 2) {
     if (there && (uint32_t)pos >= (uint32_t)p.rope_rows && p.status) atomicCAS(p.status, 0, (int)DEV_BAD_INDEX);
     const int64_t row = min(max(pos, 0), p.rope_rows - 1);
     const float4 c4 = __ldg(reinterpret_cast<const float4*>(p.cos_t + row * (C / 2) + x * 4));
@@ -184,7 +184,7 @@ __global__ void __launch_bounds__(256, PLAIN ? 6 : 3) paged_write_kernel(const _
     sn[0] = pack_f32x2(s4.x, s4.y), sn[1] = pack_f32x2(s4.z, s4.w);
     ns[0] = pack_f32x2(-s4.x, -s4.y), ns[1] = pack_f32x2(-s4.z, -s4.w);
   }
-  const float* wt = !PLAIN && p.norm == 2 && kind < 2 ? (kind == 0 ? p.wq : p.wk) : nullptr;
+  const float* wt = !BARE && p.norm == 2 && kind < 2 ? (kind == 0 ? p.wq : p.wk) : nullptr;
   uint64_t wa[2], wb[2];  // norm weights of the first and second elements
   if (wt != nullptr) {
     const float4 a = __ldg(reinterpret_cast<const float4*>(wt + e0)), c = __ldg(reinterpret_cast<const float4*>(wt + e0 + kHigh));
@@ -220,7 +220,7 @@ __global__ void __launch_bounds__(256, PLAIN ? 6 : 3) paged_write_kernel(const _
     return;
   }
   bool copy = kind == 2 && !Q8;
-  if (PLAIN) copy = true;
+  if (BARE && !Q8) copy = true;
   if (copy) {  // as they are
 #pragma unroll
     for (int u = 0; u < U; ++u) store(u, {raw[u][0].x, raw[u][0].y, raw[u][1].x, raw[u][1].y});
@@ -240,7 +240,7 @@ __global__ void __launch_bounds__(256, PLAIN ? 6 : 3) paged_write_kernel(const _
       B[u][i] = HALVES ? pack_f32x2(lo(i + 2), hi(i + 2)) : pack_f32x2(hi(2 * i), hi(2 * i + 1));
     }
   }
-  if (kind < 2 && p.norm != 0) {
+  if (!BARE && kind < 2 && p.norm != 0) {
     float y[U], f[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -285,7 +285,7 @@ __global__ void __launch_bounds__(256, PLAIN ? 6 : 3) paged_write_kernel(const _
         }
     }
   }
-  if (kind < 2 && p.cos_t != nullptr) {
+  if (!BARE && kind < 2 && p.cos_t != nullptr) {
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
@@ -365,7 +365,7 @@ __global__ void __launch_bounds__(256, PLAIN ? 6 : 3) paged_write_kernel(const _
   }
 }
 
-template <int C, bool HALVES, bool Q8, bool PLAIN, int U>
+template <int C, bool HALVES, bool Q8, bool BARE, int U>
 int launch_write_u(const WriteParams& p, cudaStream_t stream) {
   constexpr int ROWS = 32 / (C / 8) * U;
   const int cq = (p.Hq + ROWS - 1) / ROWS, ck = (p.Hkv + ROWS - 1) / ROWS;
@@ -377,27 +377,28 @@ int launch_write_u(const WriteParams& p, cudaStream_t stream) {
   }
   const int64_t warps = ((int64_t)p.B * p.L + (1 << tsh) - 1) >> tsh;
   const dim3 grid((unsigned)((warps + 7) / 8), (unsigned)(cq + 2 * ck));
-  paged_write_kernel<C, HALVES, Q8, PLAIN, U><<<grid, 256, 0, stream>>>(p, cq, ck, tsh);
+  paged_write_kernel<C, HALVES, Q8, BARE, U><<<grid, 256, 0, stream>>>(p, cq, ck, tsh);
   LVAR_CUDA_OK(cudaGetLastError());
   return LVAR_OK;
 }
 // Several rows per lane once one row each would fill the chip twice over, as many as leave at most a quarter of the lanes
 // without a row; one row otherwise: the shortest chain of dependent steps, which is all that a small call waits for.
-template <int C, bool HALVES, bool Q8, bool PLAIN>
+template <int C, bool HALVES, bool Q8, bool BARE>
 int launch_write_q(const WriteParams& p, cudaStream_t stream) {
   constexpr int RPW = 32 / (C / 8);
   const int64_t tokens = (int64_t)p.B * p.L, rows = (int64_t)p.Hq + 2ll * p.Hkv;
   auto padded = [&](int n) { return ((int64_t)(p.Hq + n - 1) / n + 2 * ((p.Hkv + n - 1) / n)) * n; };
   if (tokens * rows >= 2 * 148 * 40 * RPW) {
-    if (4 * rows >= 3 * padded(4 * RPW)) return launch_write_u<C, HALVES, Q8, PLAIN, 4>(p, stream);
-    if (4 * rows >= 3 * padded(2 * RPW)) return launch_write_u<C, HALVES, Q8, PLAIN, 2>(p, stream);
+    if (4 * rows >= 3 * padded(4 * RPW)) return launch_write_u<C, HALVES, Q8, BARE, 4>(p, stream);
+    if (4 * rows >= 3 * padded(2 * RPW)) return launch_write_u<C, HALVES, Q8, BARE, 2>(p, stream);
   }
-  return launch_write_u<C, HALVES, Q8, PLAIN, 1>(p, stream);
+  return launch_write_u<C, HALVES, Q8, BARE, 1>(p, stream);
 }
 template <int C>
 int launch_write_c(const WriteParams& p, bool halves, cudaStream_t stream) {
+  const bool bare = p.norm == 0 && p.cos_t == nullptr;  // the layout of rotations does not matter then
+  if (bare) return p.c.scales ? launch_write_q<C, false, true, true>(p, stream) : launch_write_q<C, false, false, true>(p, stream);
   if (p.c.scales) return halves ? launch_write_q<C, true, true, false>(p, stream) : launch_write_q<C, false, true, false>(p, stream);
-  if (p.norm == 0 && p.cos_t == nullptr) return launch_write_q<C, false, false, true>(p, stream);
   return halves ? launch_write_q<C, true, false, false>(p, stream) : launch_write_q<C, false, false, false>(p, stream);
 }
 
@@ -486,7 +487,7 @@ int launch_paged_write(const lvar_paged_write_args* a, cudaStream_t stream) {
   LVAR_REQUIRE((a->q == nullptr) == (a->Hq == 0) && (a->q == nullptr) == (a->q_out == nullptr) && a->Hq >= 0, LVAR_ERR_ARG,
                "q, q_out and Hq go together");
   LVAR_REQUIRE(a->L >= 1 && a->L <= kMaxTokens, LVAR_ERR_ARG, "bad number of tokens");
-  LVAR_REQUIRE((int64_t)c.B * a->L < (1ll << 31), LVAR_ERR_LIMIT, "too many tokens");
+  LVAR_REQUIRE((int64_t)c.B * a->L <= kMaxTokens, LVAR_ERR_LIMIT, "too many tokens");
   LVAR_REQUIRE(a->norm >= 0 && a->norm <= 2, LVAR_ERR_ARG, "norm must be 0, 1 or 2");
   LVAR_REQUIRE(a->norm != 1 || a->scale_mul || a->Hq == 0, LVAR_ERR_ARG, "the L2 norm takes scale_mul");
   LVAR_REQUIRE(a->norm != 2 || a->eps >= 0.f, LVAR_ERR_ARG, "eps must not be negative");
