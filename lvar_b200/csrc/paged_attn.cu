@@ -202,8 +202,8 @@ __device__ __forceinline__ void look_ahead(const PagedAttnParams& p, Cursor& c) 
 // All items lie on a line that the CTAs share evenly, each with COST units and one unit per tile behind them: what an item
 // costs beside its tiles counts too, or a CTA over many short sequences would be the last by far (64 sequences of 0 to 2521
 // keys x 16 heads, e4m3, head dimension 64: 66 us without, 50 with one unit, 53 with four; 16 sequences of 0 to 4121 keys x
-// 35 rows x 4 heads, bf16: 37, 34 and 30 us).  A CTA takes the tiles
-// whose units lie in its range; every warp works that out for itself, by prefix sums over the sequences, a few per lane.
+// 35 rows x 4 heads, bf16: 37, 34 and 30 us, 31 with seven).  A CTA takes the tiles whose units lie in its range; every warp
+// works that out for itself, by prefix sums over the sequences, a few per lane.
 struct Range {
   int64_t total;       // units
   int64_t item_start;  // unit of the first tile of the item at the range's start
