@@ -303,6 +303,21 @@ __device__ __forceinline__ int element_of(int tile, int second) {
   return RAW8 ? g * (D / 8) + 2 * tile + second : tile * 16 + 8 * second + g;
 }
 
+// Waits for a stage by a whole warp, with one answer for all lanes: false where the wait ran out.  With a limit of zero a
+// phase that is not complete at the first look fails: mbar_wait's first look may itself be held for some microseconds.
+__device__ __forceinline__ bool stage_wait(uint64_t* bar, uint32_t phase, const WaitCtx& w, int code) {
+  bool ok = mbar_test_wait(bar, phase);
+  if (!ok) {
+    if (w.limit_ns == 0) {
+      if (w.status) atomicCAS(w.status, 0, (int)DEV_FORCED_TIMEOUT);
+      *w.abort_flag = 1;
+    } else {
+      ok = mbar_wait(bar, phase, w, code);
+    }
+  }
+  return __all_sync(0xffffffffu, ok);
+}
+
 // Fetches the tiles of a CTA's range, `nt` from `cur` on, into the ring.
 template <class X, int D, bool Q8>
 __device__ __forceinline__ void loader(const CUtensorMap& mk, const CUtensorMap& mv, const PagedAttnParams& p, Cursor cur, int nt,
@@ -328,7 +343,9 @@ __device__ __forceinline__ void loader(const CUtensorMap& mk, const CUtensorMap&
     const int now = boxes, now_row = row;
     int now_page = page;
     if (issued + 1 < nt) look_up(next);
-    if (issued >= X::STAGES && !mbar_wait(&empty[stage], phase ^ 1, w, DEV_TIMEOUT_PRODUCER)) break;
+    // A stage is filled again only when all four warps have seen its last tile arrive and have let go of it: no barrier is
+    // armed while bytes of its phase before are under way.
+    if (issued >= X::STAGES && !stage_wait(&empty[stage], phase ^ 1, w, DEV_TIMEOUT_PRODUCER)) break;
     const int r0 = cur.rt * X::RC;
     const int queries = X::Q_STAGE && (issued == 0 || cur.tile == 0) ? min(X::RC, p.R - r0) : 0;
     if (lane == 0) mbar_arrive_expect_tx(&full[stage], now * box_bytes + queries * D * 2);
@@ -357,7 +374,7 @@ __device__ __forceinline__ void loader(const CUtensorMap& mk, const CUtensorMap&
     cur = next;
     if (++stage == X::STAGES) stage = 0, phase ^= 1;
   }
-  // Shared memory must not go while a copy is in flight, also after a wait that ran out.
+  // Shared memory must not go while a copy is in flight, also after a wait that ran out: the last copies into every stage.
   for (int i = issued > X::STAGES ? issued - X::STAGES : 0; i < issued; ++i) {
     const uint64_t t0 = globaltimer_ns();
     while (!mbar_try_wait(&full[i % X::STAGES], (i / X::STAGES) & 1)) {
@@ -500,6 +517,20 @@ __device__ __forceinline__ float sum_of_keys(float x) {
   return x + __shfl_xor_sync(0xffffffffu, x, 16);
 }
 
+// The rest of a computing warp's way, `tiles` from `c` on, after a wait that ran out: to the barriers at the items' ends,
+// where the other warps wait for it.  It lets go of no stage any more: the copies into the one it did not wait for may be in
+// flight, and the loader, which needs all four warps to fill a stage again, gives up in turn.
+template <class X>
+__device__ __forceinline__ void give_up(const PagedAttnParams& p, Cursor c, int tiles) {
+  for (; tiles > 0; --tiles) {
+    if (c.tile == c.ntile - 1 || tiles == 1) {
+      compute_sync();
+      compute_sync();
+    }
+    advance<X::KT>(p, c);
+  }
+}
+
 template <int D, bool Q8, int NB, int WR>
 __global__ void __launch_bounds__(kAllThreads, (Geo<D, Q8, NB, WR>::CTAS))
     paged_attn_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
@@ -566,7 +597,7 @@ __global__ void __launch_bounds__(kAllThreads, (Geo<D, Q8, NB, WR>::CTAS))
   int limit[NB][2];     // keys that the row sees
   int see_all = 0;      // keys that every row of the item sees
   const bool whole_first = cons.tile == 0;  // the CTA's first piece begins at its item's start
-  bool first_piece = true, fresh = true, alive = true;
+  bool first_piece = true, fresh = true;
   int4 head = make_int4(0, 0, 0, 0);
   int64_t item_unit = range.item_start;  // of the item's first tile, on the line
   int stage = 0;
@@ -574,7 +605,10 @@ __global__ void __launch_bounds__(kAllThreads, (Geo<D, Q8, NB, WR>::CTAS))
 
   for (int i = 0; i < nt; ++i) {
     const int rt = cons.rt, h = cons.h;
-    if (X::Q_STAGE) alive = alive && mbar_wait(&full[stage], phase, wait, DEV_TIMEOUT_SOFTMAX);
+    if (X::Q_STAGE && !stage_wait(&full[stage], phase, wait, DEV_TIMEOUT_SOFTMAX)) {
+      give_up<X>(p, cons, nt - i);
+      break;
+    }
     if (fresh) {
       fresh = false;
       see_all = p.causal ? cons.len - p.T + 1 : cons.len;
@@ -639,9 +673,12 @@ __global__ void __launch_bounds__(kAllThreads, (Geo<D, Q8, NB, WR>::CTAS))
         }
       }
     }
-    if (!X::Q_STAGE) alive = alive && mbar_wait(&full[stage], phase, wait, DEV_TIMEOUT_SOFTMAX);
+    if (!X::Q_STAGE && !stage_wait(&full[stage], phase, wait, DEV_TIMEOUT_SOFTMAX)) {
+      give_up<X>(p, cons, nt - i);
+      break;
+    }
 
-    const bool idle = rt * X::RC + wr * X::RW >= p.R || !alive;  // none of the warp's rows exists
+    const bool idle = rt * X::RC + wr * X::RW >= p.R;  // none of the warp's rows exists
     const uint32_t ks = ring + stage * X::STAGE, vs = ks + X::KT * X::RB;
     const uint32_t ss = ring + X::STAGES * X::STAGE + stage * X::SCALE_STAGE;
 #pragma unroll 1

@@ -787,3 +787,27 @@ def test_the_compiled_entry_leaves_wrong_calls_alone(K):
         host.attn(*good)
     assert before == [sys.getrefcount(x) for x in (q, k, v, table, n)]
     assert sys.getrefcount(host.attn(*good)) <= 2
+
+
+@pytest.mark.parametrize("bits,D", [(16, 128), (8, 128), (16, 64), (8, 64)])
+@pytest.mark.parametrize("G,T", [(1, 1), (2, 5), (4, 8), (7, 5)])
+def test_a_wait_that_runs_out_many_tiles_into_a_ring(K, bits, D, G, T):
+    """Every CTA has more tiles than its ring has stages: a call whose waits run out ends with a status (always, where the
+    limit is zero; one that ends without a status is whole), and the next call has the bits it had before."""
+    B, H, n = 2, 4, 80000
+    k, v, sc, table = make_cache(B, H, D, 64, n, bits, 191)
+    q = torch.randn(B, H * G, T, D, generator=torch.Generator(device="cuda").manual_seed(9), device="cuda").bfloat16()
+    lens = torch.tensor([n, n - 777], dtype=torch.int32, device="cuda")
+    good = K.new_status("cuda")
+    want = K.paged_attn_fwd(q, k, v, table, lens, scales=sc, causal=True, status=good)
+    for limit in (0, 0, 0, 1000, 5000, 20000, 0):
+        st = K.new_status("cuda")
+        got = K.paged_attn_fwd(q, k, v, table, lens, scales=sc, causal=True, status=st, wait_limit_ns=limit)
+        code = K.read_status(st)[0]
+        if limit == 0:
+            assert code == 6
+        else:
+            assert code in (0, 1, 3)
+            assert code != 0 or torch.equal(got, want)
+        assert torch.equal(K.paged_attn_fwd(q, k, v, table, lens, scales=sc, causal=True, status=good), want)
+    assert K.read_status(good)[0] == 0
