@@ -132,6 +132,20 @@ __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
 }
+// The larger magnitude of either half's two bf16, or NaN (with a sign that means nothing).
+__device__ __forceinline__ uint32_t max_abs_bf16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("max.NaN.xorsign.abs.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+// Zeros in place of bf16 elements that are not finite.
+__device__ __forceinline__ void finite_only(uint32_t (&a)[4]) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    if ((a[j] & 0x7f80u) == 0x7f80u) a[j] &= 0xffff0000u;
+    if ((a[j] & 0x7f800000u) == 0x7f800000u) a[j] &= 0xffffu;
+  }
+}
 // Token of a (token, query head) row.
 __device__ __forceinline__ int token_of(int r, int T, int G) {
   return T == 1 ? 0 : G == 1 ? r : (int)((uint32_t)r / (uint32_t)G);
@@ -407,22 +421,26 @@ __device__ __forceinline__ void weigh(State<D, NB>& st, const float (&sc)[NK][NB
     }
     if constexpr (!Q8) {
       const uint32_t v0 = vs + (s0 + k * 16 + (lane & 7) + ((lane >> 4) << 3)) * X::RS + ((((lane >> 3) & 1) ^ (lane & 7)) << 4);
+      uint32_t a[D / 16][4], most = 0;
 #pragma unroll
       for (int t = 0; t < D / 16; ++t) {
-        uint32_t a[4];
-        ldsm_x4_t((v0 ^ ((t & 3) << 5)) + (t >> 2) * X::SUB, a);
-        if constexpr (CLEAN) {
+        ldsm_x4_t((v0 ^ ((t & 3) << 5)) + (t >> 2) * X::SUB, a[t]);
+        if constexpr (CLEAN) finite_only(a[t]);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            if ((a[j] & 0x7f80u) == 0x7f80u) a[j] &= 0xffff0000u;
-            if ((a[j] & 0x7f800000u) == 0x7f800000u) a[j] &= 0xffffu;
-          }
-        }
+        for (int nb = 0; nb < NB; ++nb) mma_bf16(st.acc[t][nb], a[t], b[nb][0], b[nb][1]);
+        if constexpr (X::TWO && !CLEAN)
 #pragma unroll
-        for (int nb = 0; nb < NB; ++nb) {
-          mma_bf16(st.acc[t][nb], a, b[nb][0], b[nb][1]);
-          if constexpr (X::TWO) mma_bf16(st.acc[t][nb], a, rest[nb][0], rest[nb][1]);
-        }
+          for (int j = 0; j < 4; ++j) most = max_abs_bf16x2(most, a[t][j]);
+      }
+      if constexpr (X::TWO) {
+        // An infinity has its product above; a rest of zero or below would make NaN of it.
+        if (!CLEAN && __any_sync(0xffffffffu, (((most & 0x7f807f80u) + 0x00800080u) & 0x80008000u) != 0))
+#pragma unroll
+          for (int t = 0; t < D / 16; ++t) finite_only(a[t]);
+#pragma unroll
+        for (int t = 0; t < D / 16; ++t)
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb) mma_bf16(st.acc[t][nb], a[t], rest[nb][0], rest[nb][1]);
       }
     } else {
       constexpr int W = D / 32;  // words per thread and key: D / 8 consecutive elements, lane / 4 says which

@@ -811,3 +811,31 @@ def test_a_wait_that_runs_out_many_tiles_into_a_ring(K, bits, D, G, T):
             assert code != 0 or torch.equal(got, want)
         assert torch.equal(K.paged_attn_fwd(q, k, v, table, lens, scales=sc, causal=True, status=good), want)
     assert K.read_status(good)[0] == 0
+
+
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("D,G,T", [(128, 1, 1), (64, 8, 1), (128, 4, 4), (64, 3, 3), (128, 5, 7), (64, 8, 8)])
+def test_infinite_values_wherever_they_lie(K, D, G, T, causal):
+    """An element of V that is +inf or -inf makes the output's element the same infinity (its weight is positive), and two
+    of opposite signs make NaN, whatever the key's place in a tile, whatever the weights' last bits and however many rows
+    share the key; the other columns keep their bits.  Rows of 1, 8, 16, 9, 35 and 64; every place of two tiles and some
+    behind them."""
+    H, page, n = 2, 32, 400
+    at = list(range(0, 150)) + list(range(150, n - T, 23)) + [n - T]
+    B = len(at)
+    k, v, _, _ = make_cache(B, H, D, page, n, 16, 11)
+    per = -(-n // page)
+    table = torch.arange(B * per, device="cuda").view(B, per).to(torch.int32)
+    k, v = torch.nan_to_num(k), torch.nan_to_num(v)
+    q = torch.randn(B, H * G, T, D, generator=torch.Generator(device="cuda").manual_seed(9), device="cuda").bfloat16()
+    lens = torch.full((B,), n, dtype=torch.int32, device="cuda")
+    clean = K.paged_attn_fwd(q, k, v, table, lens, 0.1, causal=causal)
+    for b, p in enumerate(at):
+        row = v[int(table[b, p // page]), :, p % page]
+        row[:, 20:30], row[:, 30:40], row[:, 40:41] = math.inf, -math.inf, math.inf
+        p2 = (p + 37) % (n - T)  # another key that every token sees
+        if p2 != p:
+            v[int(table[b, p2 // page]), :, p2 % page, 40] = -math.inf
+    got = K.paged_attn_fwd(q, k, v, table, lens, 0.1, causal=causal)
+    assert (got[..., 20:30] == math.inf).all() and (got[..., 30:40] == -math.inf).all() and torch.isnan(got[..., 40]).all()
+    assert torch.equal(got[..., :20], clean[..., :20]) and torch.equal(got[..., 41:], clean[..., 41:])
