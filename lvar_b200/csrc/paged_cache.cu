@@ -261,10 +261,13 @@ __global__ void __launch_bounds__(256, BARE ? (Q8 ? 4 : 6) : 3) paged_write_kern
       f[u] = fmaf(0.5f * f[u], fmaf(-y[u] * f[u], f[u], 1.f), f[u]);
       plain = plain && y[u] > 1e-24f && y[u] < 1e38f;
     }
-    if (!plain) {  // a norm that is clamped, zero or not finite
+    if (!plain) {  // a norm that is clamped (by a comparison: a NaN stays one), zero or not finite
 #pragma unroll
-      for (int u = 0; u < U; ++u)
-        if (!(y[u] > 1e-24f && y[u] < 1e38f)) f[u] = p.norm == 1 ? 1.f / fmaxf(sqrtf(y[u]), 1e-12f) : 1.f / sqrtf(y[u]);
+      for (int u = 0; u < U; ++u) {
+        if (y[u] > 1e-24f && y[u] < 1e38f) continue;
+        const float norm = sqrtf(y[u]);
+        f[u] = 1.f / (p.norm == 1 && norm < 1e-12f ? 1e-12f : norm);
+      }
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {

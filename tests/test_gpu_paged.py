@@ -839,3 +839,38 @@ def test_infinite_values_wherever_they_lie(K, D, G, T, causal):
     got = K.paged_attn_fwd(q, k, v, table, lens, 0.1, causal=causal)
     assert (got[..., 20:30] == math.inf).all() and (got[..., 30:40] == -math.inf).all() and torch.isnan(got[..., 40]).all()
     assert torch.equal(got[..., :20], clean[..., :20]) and torch.equal(got[..., 41:], clean[..., 41:])
+
+
+@pytest.mark.parametrize("bits", [16, 8])
+@pytest.mark.parametrize("B,L,Hq,H,D", [(1, 2, 3, 1, 128), (2, 5, 4, 4, 64), (1, 900, 16, 16, 128), (1, 1100, 16, 16, 64)])
+def test_norms_of_rows_that_are_not_finite(K, bits, B, L, Hq, H, D):
+    """A NaN makes its row's norm NaN and with it the whole row; an infinity makes its own element NaN and the others 0, with
+    either norm.  Few and many rows per lane."""
+    g = torch.Generator(device="cuda").manual_seed(131 + L)
+    clean = torch.randn(B, L, Hq + 2 * H, D, generator=g, device="cuda").bfloat16()
+    x = clean.clone()
+    x[0, 0, 0, 3] = math.nan                 # a query row
+    x[0, L - 1, Hq, D - 1] = math.nan        # a key row
+    x[B - 1, 1, Hq - 1, 7] = -math.inf
+    x[B - 1, 0, Hq + H - 1, 0] = math.inf
+    x[0, L // 2, Hq + H, 1] = math.nan       # a value row
+    page = 16
+    per = -(-L // page)
+    table = torch.arange(B * per, device="cuda").view(B, per).to(torch.int32)
+    start, lens = (torch.full((B,), n, dtype=torch.int32, device="cuda") for n in (0, L))
+    for kw in ({"scale_mul": torch.rand(Hq, generator=g, device="cuda") + 0.5}, {"eps": 1e-6}):
+        out = []
+        for y in (clean, x):
+            kp, vp, sc = empty_cache(B * per, H, page, D, bits)
+            q = K.paged_qkv_prologue(y[:, :, :Hq], y[:, :, Hq:Hq + H], y[:, :, Hq + H:], kp, vp, table, start, scales=sc, **kw)
+            out.append((q, *K.paged_kv_read(kp, vp, table, lens, L, scales=sc)))
+        wq, wk, _, _ = op.prologue(x[:, :, :Hq], x[:, :, Hq:Hq + H], start=[0] * B, **kw)
+        wv = x[:, :, Hq + H:].double()
+        for i, want in enumerate((wq, wk, wv)):
+            want = want.transpose(1, 2)
+            bad = ~torch.isfinite(x[:, :, (0, Hq, Hq + H)[i]:(Hq, Hq + H, Hq + 2 * H)[i]]).all(-1).transpose(1, 2)
+            a, b = out[0][i], out[1][i]
+            assert bad.any() and torch.equal(a[~bad], b[~bad])
+            assert torch.equal(torch.isnan(b[bad]), torch.isnan(want[bad])), i
+            if i < 2:
+                assert (b[bad].nan_to_num(0.0) == 0).all()
