@@ -109,9 +109,10 @@ __device__ __forceinline__ uint32_t narrow4(float a, float b, float c, float d) 
 }
 
 // Biased exponent of a row's scale: the least e with most * 2^-e <= 448 = 1.75 * 2^8, -100 <= e <= 120.  For most = s * 2^q
-// with 1 <= s < 2 that is q - 8, and one more where s > 1.75: the addend carries into the exponent just then.
+// with 1 <= s < 2 that is q - 8, and one more where s > 1.75: the addend carries into the exponent just then.  A maximum over
+// nothing but NaN is NaN and counts as 0: fmaxf takes the number.
 __device__ __forceinline__ int scale_byte(float most) {
-  return min(max((int)((__float_as_uint(most) + 0x1fffffu) >> 23) - 8, 27), 247);
+  return min(max((int)((__float_as_uint(fmaxf(most, 0.f)) + 0x1fffffu) >> 23) - 8, 27), 247);
 }
 
 // A CTA's eight warps take a token each; a warp takes RPW * U rows of one kind (q, k or v heads), grid.y says which.  Where
@@ -342,7 +343,6 @@ __global__ void __launch_bounds__(256, BARE ? (Q8 ? 4 : 6) : 3) paged_write_kern
         B[u][i] = pack_f32x2(fabsf(a) < INFINITY ? a : NAN, fabsf(c) < INFINITY ? c : NAN);
       }
       most[u] = largest(u);
-      most[u] = most[u] < INFINITY ? most[u] : 0.f;  // all NaN
 #pragma unroll
       for (int d = LPR / 2; d >= 1; d >>= 1) most[u] = fmaxf(most[u], __shfl_xor_sync(0xffffffffu, most[u], d));
     }

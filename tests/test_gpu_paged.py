@@ -874,3 +874,28 @@ def test_norms_of_rows_that_are_not_finite(K, bits, B, L, Hq, H, D):
             assert torch.equal(torch.isnan(b[bad]), torch.isnan(want[bad])), i
             if i < 2:
                 assert (b[bad].nan_to_num(0.0) == 0).all()
+
+
+@pytest.mark.parametrize("B,H,L,D", [(1, 1, 3, 128), (1, 3, 5, 64), (1, 16, 1600, 128), (1, 16, 1600, 64), (1, 8, 3000, 64)])
+def test_scale_of_rows_without_a_finite_element(K, B, H, L, D):
+    """Elements that are not finite take no part in a row's maximum: a row of nothing else has the least exponent, whatever
+    the rows beside it hold."""
+    g = torch.Generator(device="cuda").manual_seed(141)
+    per = -(-L // 16)
+    table = torch.arange(per, device="cuda").view(1, per).to(torch.int32)
+    zero = torch.zeros(1, dtype=torch.int32, device="cuda")
+    for rows in ([math.nan], [math.nan, math.inf], [-math.inf]):
+        x = torch.randn(B, H, L, D, generator=g, device="cuda").bfloat16()
+        for i, value in enumerate(rows):
+            x[0, (H - 1) * (1 - i), i::3] = value
+        kp, vp, sc = empty_cache(per, H, 16, D, 8)
+        K.paged_kv_append(x, x.flip(1), kp, vp, table, zero, scales=sc)
+        for i, y in enumerate((x, x.flip(1))):
+            _, e = op.quantise(y)
+            got = sc[..., i].transpose(0, 1).reshape(H, -1)[:, :L]
+            assert torch.equal(got.int() - 127, e[0, :, :, 0].int())
+        qkv = x.transpose(1, 2)
+        K.paged_qkv_prologue(qkv, qkv, qkv, kp, vp, table, zero, scales=sc, scale_mul=torch.ones(H, device="cuda"))
+        bad = ~torch.isfinite(x[0]).any(-1)
+        got = sc.transpose(0, 1).reshape(H, -1, 2)[:, :L]
+        assert bad.any() and (got[bad] == 27).all() and (got[~bad] > 100).all()
