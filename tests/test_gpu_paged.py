@@ -899,3 +899,24 @@ def test_scale_of_rows_without_a_finite_element(K, B, H, L, D):
         bad = ~torch.isfinite(x[0]).any(-1)
         got = sc.transpose(0, 1).reshape(H, -1, 2)[:, :L]
         assert bad.any() and (got[bad] == 27).all() and (got[~bad] > 100).all()
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("Hq,H,T,n", [(2, 2, 1, 2), (8, 1, 1, 64), (16, 2, 2, 130), (3, 3, 5, 1000), (4, 1, 4, 20000)])
+def test_weights_of_few_rows_are_not_rounded_once(K, D, Hq, H, T, n):
+    """Up to 16 rows per key head over a bf16 cache: a weight is the sum of two bf16 numbers.  The first leaves at most 2^-8
+    of it (half a step), the second rounds that by 2^-9 of its own value (it lies below the half step of 1, or is exact), so
+    2^-17 of the weight is lost in place of 2^-8.  V rows come in pairs x, -x and scores are small, so that what an output
+    element has is the difference of nearly equal weights and its own rounding hides nothing."""
+    k, v, _, table = make_cache(2, H, D, 64, n, 16, 161)
+    k, v = torch.nan_to_num(k), torch.nan_to_num(v)
+    v[:, :, 1::2] = -v[:, :, 0::2]
+    q = torch.randn(2, Hq, T, D, generator=torch.Generator(device="cuda").manual_seed(9), device="cuda").bfloat16()
+    lens = torch.tensor([n, (n + 1) // 2], dtype=torch.int32, device="cuda")
+    scale = 0.1 / D
+    got = K.paged_attn_fwd(q, k, v, table, lens, scale)
+    o, _, _, A, S = op.attention(q, k, v, table, lens.tolist(), scale)
+    fp32 = 2 * (2 * (D + 8) * U32 * S + 2.0 ** -21) + n * U32
+    tol = U16 * o.abs() + (2.0 ** -17 + fp32).unsqueeze(-1) * A * (1 + U16) + 1e-30
+    err = (got.double() - o).abs()
+    assert (err <= tol).all(), f"off by up to {(err / tol).max().item():.2f} bounds"
