@@ -920,3 +920,111 @@ def test_weights_of_few_rows_are_not_rounded_once(K, D, Hq, H, T, n):
     tol = U16 * o.abs() + (2.0 ** -17 + fp32).unsqueeze(-1) * A * (1 + U16) + 1e-30
     err = (got.double() - o).abs()
     assert (err <= tol).all(), f"off by up to {(err / tol).max().item():.2f} bounds"
+
+
+def scatter(pool, table, page, start, count, rows):
+    """Puts rows [B, L, H, ...] (l < count[b]) at positions start[b] + l of a pool [pages, H, page, ...]."""
+    b, l = torch.nonzero(torch.arange(rows.shape[1], device="cuda")[None] < count[:, None], as_tuple=True)
+    pos = start.long()[b] + l
+    rows = rows.to(pool.dtype)
+    if pool.dtype == torch.float8_e4m3fn:
+        pool, rows = pool.view(torch.uint8), rows.view(torch.uint8)
+    pool[table.long()[b, pos // page], :, pos % page] = rows[b, l]
+
+
+def same(a, b):
+    """Equal bytes, but for which NaN stands where both have one."""
+    if a.dtype == torch.float8_e4m3fn:
+        a, b = a.view(torch.uint8), b.view(torch.uint8)
+        return bool(((a == b) | (((a & 0x7F) == 0x7F) & ((b & 0x7F) == 0x7F))).all())
+    return torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
+def with_odd_rows(x, g):
+    """x [B, L, H, D] in which every eleventh row or so is zero, tiny, huge, or has NaN and infinities in it."""
+    kind = torch.randint(0, 77, (*x.shape[:-1], 1), generator=g, device="cuda")
+    col = torch.arange(x.shape[-1], device="cuda")
+    for i, value in enumerate((0.0, 1e-35, 3e38, math.nan, math.inf, -math.inf)):
+        x = torch.where((kind == i) if i < 3 else (kind == i) & (col % 9 == i), torch.full_like(x, value), x)
+    return x.bfloat16()
+
+
+# The heads that make a lane take four or two rows (whole and partial last groups), and calls just large enough for that.
+MANY = [(64, 16, 1500), (64, 13, 1900), (64, 8, 3000), (64, 7, 3400), (128, 8, 1500), (128, 7, 1800), (128, 4, 3000), (128, 3, 4000)]
+
+
+@pytest.mark.parametrize("bits", [16, 8])
+@pytest.mark.parametrize("D,H,L", MANY)
+def test_append_with_several_rows_per_lane(K, bits, D, H, L):
+    """Exact, everything around the rows included; NaN and infinities among the rows of a warp."""
+    g = torch.Generator(device="cuda").manual_seed(171 + H)
+    B, page = 2, 48
+    x = torch.randn(B, L, 2 * H, D, generator=g, device="cuda") * torch.exp2(
+        torch.randint(-40, 41, (B, L, 2 * H, 1), generator=g, device="cuda").float())
+    x = with_odd_rows(x, g)
+    k, v = x[:, :, :H], x[:, :, H:]
+    start = torch.tensor([5, 50], dtype=torch.int32, device="cuda")
+    count = torch.tensor([L, L - 77], dtype=torch.int32, device="cuda")
+    per = -(-(50 + L) // page)
+    table = torch.randperm(B * per + 1, generator=g, device="cuda")[:B * per].view(B, per).to(torch.int32)
+    kp, vp, sc = empty_cache(B * per + 1, H, page, D, bits)
+    wk, wv, ws = empty_cache(B * per + 1, H, page, D, bits)
+    st = K.new_status("cuda")
+    K.paged_kv_append(k.transpose(1, 2), v.transpose(1, 2), kp, vp, table, start, scales=sc, count=count, status=st)
+    assert K.read_status(st)[0] == 0
+    for i, (src, pool) in enumerate(((k, wk), (v, wv))):
+        if bits == 8:
+            y, e = op.quantise(src)
+            scatter(pool, table, page, start, count, y.float().to(torch.float8_e4m3fn))
+            scatter(ws[..., i], table, page, start, count, (e + 127)[..., 0])
+        else:
+            scatter(pool, table, page, start, count, src)
+    assert same(kp, wk) and same(vp, wv) and (bits == 16 or same(sc, ws))
+
+
+@pytest.mark.parametrize("bits", [16, 8])
+@pytest.mark.parametrize("halves", [False, True])
+@pytest.mark.parametrize("norm", ["l2", "rms", "none"])
+@pytest.mark.parametrize("D,Hq,H,L", [(64, 16, 16, 600), (64, 20, 5, 900), (64, 8, 8, 1100), (128, 8, 8, 600), (128, 10, 5, 700),
+                                      (128, 4, 4, 1100)])
+def test_prologue_with_several_rows_per_lane(K, bits, halves, norm, D, Hq, H, L):
+    """The bounds of test_prologue, for every row."""
+    g = torch.Generator(device="cuda").manual_seed(181 + Hq)
+    B, page = 2, 48
+    x = torch.randn(B, L, Hq + 2 * H, D, generator=g, device="cuda").bfloat16()
+    odd = with_odd_rows(x[:, :, Hq + H:].float(), g)
+    q, k, v = x[:, :, :Hq], x[:, :, Hq:Hq + H], odd
+    start = torch.tensor([3, 16], dtype=torch.int32, device="cuda")
+    per = -(-(16 + L) // page)
+    table = torch.randperm(B * per, generator=g, device="cuda").view(B, per).to(torch.int32)
+    angle = torch.arange(per * page, dtype=torch.float64, device="cuda")[:, None] * 10000.0 ** (
+        -torch.arange(D // 2, dtype=torch.float64, device="cuda") * 2 / D)
+    kw = {"rope_cos": angle.cos().float(), "rope_sin": angle.sin().float(), "rope_halves": halves}
+    ref = {"cos": kw["rope_cos"], "sin": kw["rope_sin"], "halves": halves}
+    if norm == "l2":
+        kw["scale_mul"] = ref["scale_mul"] = torch.rand(Hq, generator=g, device="cuda") + 0.5
+    elif norm == "rms":
+        kw["eps"] = ref["eps"] = 1e-6
+        for n in ("q_weight", "k_weight"):
+            kw[n] = ref[n] = torch.randn(D, generator=g, device="cuda")
+    kp, vp, sc = empty_cache(B * per, H, page, D, bits)
+    st = K.new_status("cuda")
+    got = K.paged_qkv_prologue(q, k, v, kp, vp, table, start, scales=sc, status=st, **kw)
+    assert K.read_status(st)[0] == 0
+    wq, wk, sq, sk = op.prologue(q, k, start=start.tolist(), **ref)
+    assert ((got.transpose(1, 2).double() - wq).abs() <= U16 * wq.abs() + 33 * U32 * sq + 1e-38).all()
+    pos = start.long()[:, None] + torch.arange(L, device="cuda")
+    at = table.long().gather(1, pos // page)
+    rows = [t.view(torch.uint8)[at, :, pos % page].view(t.dtype) if bits == 8 else t[at, :, pos % page] for t in (kp, vp)]
+    if bits == 16:
+        assert ((rows[0].double() - wk).abs() <= U16 * wk.abs() + 33 * U32 * sk + 1e-38).all()
+        assert same(rows[1], v)
+    else:
+        e = sc[at, :, pos % page].double() - 127
+        y, ev = op.quantise(v)
+        assert torch.equal(e[..., 1], ev[..., 0].double()) and same(rows[1], y.float().to(torch.float8_e4m3fn))
+        most, slack, up = wk.abs().amax(-1), 33 * U32 * sk.amax(-1), torch.exp2(e[..., :1])
+        assert ((most - slack) * torch.exp2(-e[..., 0]) <= 448).all()
+        assert ((most + slack) * torch.exp2(1 - e[..., 0]) > 448).all()
+        tol = torch.maximum(2.0 ** -4 * wk.abs(), 2.0 ** -10 * up) + 40 * U32 * sk
+        assert ((rows[0].double() * up - wk).abs() <= tol).all()
