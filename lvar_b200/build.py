@@ -2,8 +2,9 @@
 
 ``python -m lvar_b200.build`` compiles every ``csrc/*.cu`` to an object file and links them into
 ``lvar_b200/liblvar_b200.so``, and ``csrc/paged_host.cpp`` (the Python entry of the paged-cache calls, over the same
-library and torch's headers) into ``lvar_b200/_paged_host.so``.  Objects are rebuilt only when a source or header is newer.  nvcc
-cross-compiles for sm_100a, so this also runs on a machine without a GPU.
+library and torch's headers) into ``lvar_b200/_paged_host.so``.  Objects are rebuilt only when a source or header is
+newer, the module also for another torch or Python.  nvcc cross-compiles for sm_100a, so this also runs on a machine
+without a GPU.
 """
 from __future__ import annotations
 
@@ -44,16 +45,23 @@ def _stale(target: Path, deps: list[Path]) -> bool:
     return any(d.stat().st_mtime > t for d in deps)
 
 
+def host_key() -> str:
+    """What the compiled entry of the paged-cache calls is made for: it uses torch's C++ classes and CPython's."""
+    import torch
+    return f"torch {torch.__version__}, {sysconfig.get_config_var('SOABI')}, abi {int(torch._C._GLIBCXX_USE_CXX11_ABI)}"
+
+
 def _build_host(force: bool) -> None:
-    """The C++ entry of the paged-cache calls: a CPython module that links the library beside it and torch."""
-    src = CSRC / "paged_host.cpp"
-    if not (force or _stale(HOST_PATH, [src, INCLUDE / "lvar_b200.h"])):
+    """The C++ entry of the paged-cache calls: a CPython module that links the library beside it and torch.  Built again when
+    a source is newer or when torch or Python is another one than it was made for."""
+    src, made_for, key = CSRC / "paged_host.cpp", BUILD_DIR / "paged_host.key", host_key()
+    if not force and made_for.exists() and made_for.read_text() == key and not _stale(HOST_PATH, [src, INCLUDE / "lvar_b200.h"]):
         return
     import torch
     root = Path(torch.__file__).resolve().parent
     cuda = Path(os.environ.get("CUDA_HOME", Path(_nvcc()).resolve().parent.parent))
     cmd = [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-shared", "-fPIC",
-           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f'-DLVAR_BUILT_FOR="{key}"',
            "-isystem", str(root / "include"), "-isystem", str(root / "include" / "torch" / "csrc" / "api" / "include"),
            "-isystem", str(cuda / "include"), "-isystem", sysconfig.get_paths()["include"], str(src), "-o", str(HOST_PATH),
            "-L", str(PKG_DIR), "-l:liblvar_b200.so", "-Wl,-rpath,$ORIGIN",
@@ -61,6 +69,7 @@ def _build_host(force: bool) -> None:
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         raise RuntimeError(f"g++ failed on {src.name}:\n{res.stdout}\n{res.stderr}")
+    made_for.write_text(key)
 
 
 def build(force: bool = False, verbose: bool = False) -> Path:

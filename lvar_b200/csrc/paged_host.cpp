@@ -289,4 +289,9 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_paged_host", nullptr, -1, methods
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__paged_host() { return PyModule_Create(&module); }
+PyMODINIT_FUNC PyInit__paged_host() {
+  PyObject* m = PyModule_Create(&module);
+  // the torch and the Python whose classes the code above was compiled against
+  if (m && PyModule_AddStringConstant(m, "built_for", LVAR_BUILT_FOR) < 0) Py_CLEAR(m);
+  return m;
+}

@@ -8,17 +8,23 @@ from __future__ import annotations
 import ctypes as C
 import functools
 import math
+import warnings
 from typing import Optional, Tuple
 
 import torch
 
 from . import _lib
 from ._lib import AttnArgs, check, lib
+from .build import host_key
 
 try:
     from . import _paged_host  # links the library that _lib has loaded
-except ImportError as e:
-    raise ImportError("lvar_b200/_paged_host.so is missing or does not load: build it with `python -m lvar_b200.build`") from e
+    if _paged_host.built_for != host_key():
+        raise ImportError(f"it was made for {_paged_host.built_for}, this is {host_key()}")
+except (ImportError, AttributeError) as e:
+    _paged_host = None  # the Python code of the paged-cache calls makes them all
+    warnings.warn(f"lvar_b200/_paged_host.so is not used ({e}): paged-cache calls take 5 to 9 us more of the host each; build it "
+                  f"with `python -m lvar_b200.build`", RuntimeWarning)
 
 
 _raw_stream = torch._C._cuda_getCurrentRawStream  # (device index) -> cudaStream_t of torch's current stream
@@ -787,7 +793,7 @@ def paged_kv_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_p
     bf16, or float8_e4m3fn with ``scales`` uint8 [pages, H, page_size, 2]: the biased exponents of every row's power of two,
     K's and V's.  ``table`` int32 [B, n]: position p lies in page ``table[b, p // page_size]``.  ``start``, ``count``: int32
     [B] on the device.  A position without a page is not written and sets ``status`` (see :func:`new_status`)."""
-    if _paged_host.append(k, v, k_pages, v_pages, table, start, scales, count, status):
+    if _paged_host and _paged_host.append(k, v, k_pages, v_pages, table, start, scales, count, status):
         return
     c, dev = _paged_cache(k_pages, v_pages, table, scales)
     shape = k.shape
@@ -824,10 +830,11 @@ def paged_qkv_prologue(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_page
     ``rope_cos``, ``rope_sin`` fp32 [P, D/2]: row p rotates the token at cache position p, element pairs (2i, 2i + 1), or
     (i, i + D/2) with ``rope_halves``.  The cache arguments, ``start``, ``count`` and ``status`` are those of
     :func:`paged_kv_append`; q rows of padding are 0."""
-    done = _paged_host.prologue(q, k, v, k_pages, v_pages, table, start, scales, scale_mul, q_weight, k_weight, eps, rope_cos,
-                                rope_sin, rope_halves, count, status)
-    if done is not None:
-        return done
+    if _paged_host:
+        done = _paged_host.prologue(q, k, v, k_pages, v_pages, table, start, scales, scale_mul, q_weight, k_weight, eps,
+                                    rope_cos, rope_sin, rope_halves, count, status)
+        if done is not None:
+            return done
     c, dev = _paged_cache(k_pages, v_pages, table, scales)
     shape, kshape = q.shape, k.shape
     if (len(shape) != 4 or q.dtype is not _BF16 or k.dtype is not _BF16 or v.dtype is not _BF16 or v.shape != kshape or
@@ -886,7 +893,7 @@ def paged_kv_read(k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Ten
     rows at or behind ``lens[b]`` (int32 [B] on the device): the contiguous tensors that the many-query attention calls
     take.  ``out``: an optional pair of destinations (bf16, unit stride along D, other strides in multiples of 8).  An e4m3
     row comes back exactly as the values it stands for.  The cache arguments are those of :func:`paged_kv_append`."""
-    if out is None:
+    if _paged_host and out is None:
         done = _paged_host.read(k_pages, v_pages, table, lens, n, scales, start, status)
         if done is not None:
             return done
@@ -928,7 +935,7 @@ def paged_attn_fwd(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
     A row that sees no key is 0 (M = -inf, L = 0).  ``max_len``: a bound on the lengths that shapes the launch (default: what
     the table holds); a longer sequence is cut there and sets ``status``.  ``out``: see :func:`_output_like`.  The cache
     arguments are those of :func:`paged_kv_append`."""
-    if out is None:
+    if _paged_host and out is None:
         done = _paged_host.attn(q, k_pages, v_pages, table, lens, scale, scales, causal, max_len, return_stats, status,
                                 wait_limit_ns)
         if done is not None:
