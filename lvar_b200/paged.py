@@ -39,18 +39,24 @@ class PageTable:
     def free_pages(self) -> int:
         return len(self._free)
 
+    def _check(self, sequence: int) -> None:
+        if not 0 <= sequence < self.batch:
+            raise IndexError(f"sequence {sequence} is none of 0 .. {self.batch - 1}")
+
     def pages_of(self, sequence: int) -> List[int]:
+        self._check(sequence)
         return list(self._owned[sequence])
 
     def reserve(self, sequence: int, tokens: int) -> None:
         """Gives the sequence pages for its first ``tokens`` tokens; those it has stay.  Raises, and changes nothing, where
-        it would be too long or the pages do not suffice."""
+        there is no such sequence, it would be too long or the pages do not suffice."""
         self.reserve_all({sequence: tokens})
 
     def reserve_all(self, tokens: dict) -> None:
         """:meth:`reserve` for several sequences {sequence: tokens} with one update of ``table``."""
         need = {}
         for s, n in tokens.items():
+            self._check(s)
             want = -(-n // self.page_size)
             if want > self.per_sequence:
                 raise RuntimeError(f"sequence {s}: {n} tokens exceed {self.per_sequence} pages of {self.page_size}")
@@ -67,6 +73,7 @@ class PageTable:
 
     def release(self, sequence: int) -> None:
         """Takes the sequence's pages back.  Work already submitted on other streams must be done with them."""
+        self._check(sequence)
         if self._owned[sequence]:
             self._free.extend(reversed(self._owned[sequence]))
             self._owned[sequence] = []

@@ -64,3 +64,15 @@ def test_cache_shapes_and_bytes():
     b = PagedKVCache(3, 2, 64, 32, dtype=torch.float8_e4m3fn, device="cpu")
     assert a.k.shape == (3, 2, 32, 64) and a.scales is None and a.nbytes == 2 * 3 * 2 * 32 * 64 * 2
     assert b.scales.shape == (3, 2, 32, 2) and b.nbytes == 3 * 2 * 32 * (2 * 64 + 2)
+
+
+def test_sequences_are_named_once():
+    """A negative number is no second name for a sequence, and a number that is none changes nothing."""
+    t = PageTable(3, 64, page_size=16, num_pages=12, device="cpu")
+    t.reserve(1, 20)
+    before = (t.table.clone(), [t.pages_of(i) for i in range(3)], t.free_pages)
+    for call in (lambda: t.reserve_all({2: 64, -1: 64}), lambda: t.reserve(-1, 16), lambda: t.reserve(3, 16),
+                 lambda: t.reserve_all({0: 16, 3: 16}), lambda: t.release(-2), lambda: t.release(3), lambda: t.pages_of(-2)):
+        with pytest.raises(IndexError):
+            call()
+        assert torch.equal(t.table, before[0]) and [t.pages_of(i) for i in range(3)] == before[1] and t.free_pages == before[2]
