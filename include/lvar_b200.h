@@ -287,7 +287,7 @@ int lvar_qkv_prologue(const void* qkv, int64_t s_b, int64_t s_l, int64_t s_w, in
 /* A key/value cache in pages, for sequences of different length.  k, v: [num_pages, Hkv, page_size, D] with the given
  * strides in elements (innermost 1, 16-byte aligned rows; attention needs them positive), bf16, or e4m3 when `scales` is set: uint8
  * [num_pages, Hkv, page_size, 2] (innermost two contiguous; 16-byte aligned, page and head strides multiples of 16), for every row of K ([0])
- * and V ([1]) the biased exponent x of the power of two 2^(x - 127) that its e4m3 values are multiplied by.
+ * and V ([1]) the biased exponent x, 1 .. 254, of the power of two 2^(x - 127) that its e4m3 values are multiplied by.
  * table: int32 [B, max_pages] (rows t_sb apart): position j of sequence b lies in page table[b, j / page_size], row
  * j mod page_size.  Entries behind a sequence's end are not read (any value may stand there); several sequences may share
  * a page that none of them writes.  page_size: a multiple of 16 up to 512; D in {64, 128}. */
@@ -318,8 +318,8 @@ typedef struct lvar_paged_write_args {
   int64_t qo_sb, qo_sh, qo_sl;
   const int32_t* start; /* [B]: token l of sequence b goes to position start[b] + l */
   const int32_t* count; /* [B] or null (all L): tokens l >= count[b] are padding: not written, q_out 0 */
-  /* norm 1: x / max(|x|, 1e-12), q times scale_mul[h] (fp32 [Hq]); norm 2: x * rsqrt(mean x^2 + eps) * weight (fp32 [D],
-     null: 1); norm 0: none.  q and k only. */
+  /* norm 1: x / max(|x|, 1e-12) (NaN where |x| is), q times scale_mul[h] (fp32 [Hq]); norm 2: x * rsqrt(mean x^2 + eps) *
+     weight (fp32 [D], null: 1); norm 0: none.  q and k only. */
   const float* scale_mul;
   const float* q_weight;
   const float* k_weight;
@@ -357,7 +357,8 @@ typedef struct lvar_paged_attn_args {
   void* workspace;     /* lvar_paged_attn_workspace bytes, 16-byte aligned, owned by this call until it completes */
   int64_t workspace_bytes;
   int32_t* dev_status; /* optional; LVAR_DEV_BAD_INDEX: a length above max_len (cut there) or a page number outside the
-                          cache (page 0 is read in its place); LVAR_DEV_TIMEOUT_* / LVAR_DEV_FORCED_TIMEOUT: a wait ran out */
+                          cache (page 0 is read in its place); LVAR_DEV_TIMEOUT_* / LVAR_DEV_FORCED_TIMEOUT: a wait ran out (o, M
+                          and L then hold anything) */
   uint64_t wait_limit_ns; /* per-wait limit of the kernel's bounded waits; 0 forces every pending wait to fail */
   float scale;
   int32_t Hq, T;

@@ -7,8 +7,8 @@
 // elements of V, along their 16 rows and the query rows along their 8 columns: S^T = K Q^T, O^T = V^T P^T, P^T made from S^T
 // by an 8 x 8 transposition in registers.  One query row so pays for 8; the tensor-memory instructions start at 64, and
 // their accumulators would have to come back through tensor memory for every step of the running softmax.  With up to 8 rows
-// the tensor pipe is 15 to 17 % busy and HBM bounds the kernel (24 x 16 heads x 10521 keys in bf16: 303 to 315 us, 6.6 to
-// 6.8 TB/s); with 64 rows tensor pipe (58 %) and shared memory (64 %) do (16 x 8 heads x 8192 keys: 125 us, 0.66 of HBM).
+// the tensor pipe is 15 to 17 % busy and HBM bounds the kernel (24 x 16 heads x 10521 keys in bf16: 313 to 320 us,
+// 6.5 TB/s); with 64 rows tensor pipe (58 %) and shared memory (65 %) do (16 x 8 heads x 8192 keys: 122 us, 0.67 of HBM).
 //
 // A CTA is four warps that compute and one that loads.  The loader follows the page table (one lane per box of 16 to 128
 // rows that lie together in a page) and streams tiles of keys through a ring in shared memory with tensor-map copies,
@@ -24,15 +24,17 @@
 // per CTA in the workspace (unnormalised sums, maximum, sum), and a second kernel joins them in a fixed order.  Where items
 // are short a CTA takes one item and there is no second kernel (see plan_of).
 //
-// e4m3 cache: K and V rows are widened to fp16 (exact), q is scaled by a power of two per row into fp16's range (exact but
-// for elements 2^-24 below the row's largest).  K's row scale multiplies the score.  V's row scale 2^e joins the exponent
+// e4m3 cache: K and V rows are widened to fp16 (exact), q is scaled by a power of two per row into fp16's range: exact for
+// elements down to 2^-17 of the row's largest; smaller ones are off by up to 2^-25 of it (fp16's steps end at 2^-24).  K's row scale multiplies the score.  V's row scale 2^e joins the exponent
 // of the weight, w = exp2(s + e - reference of (s + e)), so that the fp16 weights are always taken relative to the
 // largest CONTRIBUTION; the row sum keeps a maximum of its own.
 // Weights against an e4m3 cache are rounded to fp16 (scaled by 2^7, so that only weights 2^-21 of the largest or less are
 // subnormal).  Against a bf16 cache up to 16 rows take them as the sum of two bf16 numbers, 2^-17 of them off: rounded once
-// they add as much again to the error of the output's own rounding, and next to HBM the second product costs nothing (24 x 16
-// heads x 10521 keys 311 us either way).  With more rows the matrix instructions count (64 rows, 16 x 8 heads x 8192 keys:
-// 131 us with one product, 159 with two), and weights are rounded to bf16.  Sums, maxima and accumulators are fp32.
+// they add as much again to the error of the output's own rounding, and next to HBM the second product and its look for
+// elements of V that are not finite cost at most 1 % (24 x 16 heads x 10521 keys 311 us either way).  With more rows the
+// matrix instructions count, and weights are rounded to bf16, 2^-8 of them off (16 x 8 heads x 8192 keys, one product / two:
+// 32 rows 100 / 110 us, 48 rows 122 / 152, 64 rows 124 / 155; 16 x 4 heads x 35 rows x 4121 keys 31.7 / 35.9, error of the
+// output 2.2e-3 / 1.7e-3 of its norm).  Sums, maxima and accumulators are fp32.
 #include <math.h>
 
 #include "paged.cuh"

@@ -384,7 +384,7 @@ int launch_write_u(const WriteParams& p, cudaStream_t stream) {
   LVAR_CUDA_OK(cudaGetLastError());
   return LVAR_OK;
 }
-// Several rows per lane once one row each would fill the chip twice over, as many as leave at most a quarter of the lanes
+// Several rows per lane once one row each would fill the chip (148 SMs of 40 warps) twice over, as many as leave at most a quarter of the lanes
 // without a row; one row otherwise: the shortest chain of dependent steps, which is all that a small call waits for.
 template <int C, bool HALVES, bool Q8, bool BARE>
 int launch_write_q(const WriteParams& p, cudaStream_t stream) {

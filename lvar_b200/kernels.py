@@ -791,7 +791,7 @@ def paged_kv_append(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_p
 
     The cache: ``k_pages``, ``v_pages`` [pages, H, page_size, D] (page_size a multiple of 16 up to 512, D 64 or 128),
     bf16, or float8_e4m3fn with ``scales`` uint8 [pages, H, page_size, 2]: the biased exponents of every row's power of two,
-    K's and V's.  ``table`` int32 [B, n]: position p lies in page ``table[b, p // page_size]``.  ``start``, ``count``: int32
+    K's and V's (1 .. 254; the calls here write 27 .. 247).  ``table`` int32 [B, n]: position p lies in page ``table[b, p // page_size]``.  ``start``, ``count``: int32
     [B] on the device.  A position without a page is not written and sets ``status`` (see :func:`new_status`)."""
     if _paged_host and _paged_host.append(k, v, k_pages, v_pages, table, start, scales, count, status):
         return
@@ -825,7 +825,8 @@ def paged_qkv_prologue(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_page
     """Norms of queries and keys, position rotation and append to a paged cache in one pass; returns q bf16 [B, Hq, L, D].
 
     q bf16 [B, L, Hq, D], k and v bf16 [B, L, Hkv, D]: views of one projection's output or separate tensors, Hq a multiple
-    of Hkv.  ``scale_mul`` fp32 [Hq]: x / max(|x|, 1e-12), q times scale_mul of its head (as :func:`qkv_prologue`).
+    of Hkv.  ``scale_mul`` fp32 [Hq]: x / max(|x|, 1e-12), q times scale_mul of its head (as :func:`qkv_prologue`,
+    but that a NaN in a row makes the whole row NaN; there such a norm counts as 1e-12).
     ``eps`` (with optional ``q_weight``, ``k_weight`` fp32 [D]): x * rsqrt(mean x^2 + eps) * weight.  Neither: no norm.
     ``rope_cos``, ``rope_sin`` fp32 [P, D/2]: row p rotates the token at cache position p, element pairs (2i, 2i + 1), or
     (i, i + D/2) with ``rope_halves``.  The cache arguments, ``start``, ``count`` and ``status`` are those of
@@ -929,8 +930,9 @@ def paged_attn_fwd(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor
     [B, Hq, T, D]; with ``return_stats`` (o, M, L), fp32 [B, Hq, T] as :func:`dense_attn_fwd` returns them.
 
     q bf16 [B, Hq, T, D], Hq a multiple of the cache's heads (query head h reads key head h // (Hq // Hkv)); few tokens are
-    meant (a cached row is read once for up to 64 / (Hq // Hkv) of them): :func:`paged_kv_read` and the attention calls
-    above serve many.  ``lens`` int32 [B] on the device: the cached keys of each sequence, the new ones included; 0 marks
+    meant: a cached row is read again for every 64 / (Hq // Hkv) of them.  Many tokens of sequences of one length, with as many
+    key heads as query heads and without `causal`, are better served by :func:`paged_kv_read` and :func:`dense_attn_fwd`, which
+    takes neither of the others.  ``lens`` int32 [B] on the device: the cached keys of each sequence, the new ones included; 0 marks
     an empty slot.  ``causal``: token t sees the keys up to its own position, lens - T + t; else every token sees all keys.
     A row that sees no key is 0 (M = -inf, L = 0).  ``max_len``: a bound on the lengths that shapes the launch (default: what
     the table holds); a longer sequence is cut there and sets ``status``.  ``out``: see :func:`_output_like`.  The cache
